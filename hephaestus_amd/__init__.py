@@ -1,7 +1,8 @@
 """hephaestus_amd — MI355X (gfx950) backend for Hephaestus's reduction / scan
 path: full and row-wise reduce (sum, max, argmax, ...), inclusive and
 exclusive prefix scans, segmented sum and the fused y = fmaf(a, x, b)
-prologue, as hand-written HIP kernels behind the C ABI of include/hx.h.
+prologue, and the operators of a linear-attention layer served in 8 bits
+(layer_ops.py), as hand-written HIP kernels behind the C ABI of include/hx.h.
 
 This package is the Python host side of that ABI.  It has no compute path of
 its own: every operation is a call into the native library, which must have
@@ -18,6 +19,9 @@ from .device import (
     RocmBuffer,
     RocmDevice,
     Topology,
+    bfloat16,
+    bfloat16_from_float32,
+    float32_from_bfloat16,
 )
 from .device_api import LaunchGeometry, RocmCompiledKernel
 from .errors import (
@@ -30,6 +34,7 @@ from .errors import (
     LengthMismatch,
     TransferFailed,
 )
+from .layer_ops import RocmLinearAttentionOps, RocmMatrixOps, RocmNormOps
 from .layout import Layout, StridedView
 from .vector_ops import (
     PreparedMapReduction,

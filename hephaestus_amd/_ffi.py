@@ -43,7 +43,7 @@ INVALID_CONFIGURATION = 6
 TRANSFER_FAILED = 7
 
 # hx_dtype
-DTYPE_F32, DTYPE_U32, DTYPE_I32 = 0, 1, 2
+DTYPE_F32, DTYPE_U32, DTYPE_I32, DTYPE_BF16 = 0, 1, 2, 3
 # hx_op
 OP_SUM, OP_PROD, OP_MIN, OP_MAX, OP_ARGMAX, OP_MEAN = 0, 1, 2, 3, 4, 5
 # hx_scan_kind / hx_scan_direction
@@ -172,6 +172,15 @@ SIGNATURES = {
     "hx_trace": (I32, [P, I32, P, U64, LP, P, U64, P]),
     "hx_vector_update": (I32, [P, I32, I32, P, U64, P, U64, c_float, P]),
     "hx_vector_binary": (I32, [P, I32, I32, P, U64, P, U64, P, U64, P]),
+    "hx_rms_norm_quantize": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, c_float, P, U64, LP, P, U64, LP, P, U64, P]),
+    "hx_prepare_rms_norm_quantize": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, c_float, P, U64, LP, P, U64, LP, P,
+                                           U64, POINTER(P)]),
+    "hx_matmul_i8": (I32, [P, P, U64, LP, P, U64, P, U64, LP, P, U64, I32, P, U64, LP, P]),
+    "hx_prepare_matmul_i8": (I32, [P, P, U64, LP, P, U64, P, U64, LP, P, U64, I32, P, U64, LP, POINTER(P)]),
+    "hx_linear_attention": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, c_float, P, U64, LP, P, U64, LP,
+                                  P, U64, P, U64, LP, P]),
+    "hx_prepare_linear_attention": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, c_float, P, U64, LP, P,
+                                          U64, LP, P, U64, P, U64, LP, POINTER(P)]),
     "hx_plan_dispatch": (I32, [P, P]),
     "hx_plan_dispatch_batch": (I32, [P, U64, P]),
     "hx_plan_destroy": (I32, [P]),

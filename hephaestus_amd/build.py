@@ -32,6 +32,10 @@ SOURCES = [
     "csrc/dense_vector.cpp",
     "csrc/noalloc.hip",
     "csrc/device_api.cpp",
+    "csrc/layer_ops.cpp",
+    "csrc/norm_quantize.hip",
+    "csrc/matmul_i8.hip",
+    "csrc/linear_attention.hip",
 ]
 HEADERS = ["csrc/hx_device.hpp", "csrc/hx_internal.hpp"]
 ARCH = "gfx950"

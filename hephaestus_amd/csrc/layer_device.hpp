@@ -1,0 +1,57 @@
+// Device-side pieces shared by the layer operators: element types, vector
+// loads at element alignment, reductions over the lanes of a wave.
+#pragma once
+
+#include "hx_device.hpp"
+
+namespace hx {
+
+typedef __bf16 bf16;
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int32_t i32x4v __attribute__((ext_vector_type(4)));
+
+// 16 bytes at the alignment of the elements: global memory takes a dwordx4
+// at any byte address, so rows of odd width keep whole vectors.
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T> struct Pack16;
+template <> struct Pack16<float> { static constexpr int N = 4; };
+template <> struct Pack16<bf16> { static constexpr int N = 8; };
+
+// f32 values of the 16 bytes at p.
+__device__ __forceinline__ void load_pack(const float *p, float (&x)[4]) {
+    const f32x4 r = *(const f32x4_a4 *)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = r[i];
+}
+__device__ __forceinline__ void load_pack(const bf16 *p, float (&x)[8]) {
+    const u32x4 r = *(const u32x4_a2 *)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t two = r[i];
+        x[2 * i] = __builtin_bit_cast(float, two << 16);
+        x[2 * i + 1] = __builtin_bit_cast(float, two & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ void store_pack(float *p, const float (&x)[4]) {
+    *(f32x4_a4 *)p = f32x4{x[0], x[1], x[2], x[3]};
+}
+// Rounded to bf16, halfway cases to even.
+__device__ __forceinline__ void store_pack(bf16 *p, const float (&x)[8]) {
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (bf16)x[i];
+    *(u32x4_a2 *)p = __builtin_bit_cast(u32x4, r);
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+    return v;
+}
+
+} // namespace hx

@@ -467,6 +467,7 @@ hx_status launch_map_reduce(const MapReduceArgs &a, void *ws, uint64_t ws_bytes,
     case HX_DTYPE_F32: return launch_kind<float>(a, ws, ws_bytes, lb, stream);
     case HX_DTYPE_U32: return launch_kind<uint32_t>(a, ws, ws_bytes, lb, stream);
     case HX_DTYPE_I32: return launch_kind<int32_t>(a, ws, ws_bytes, lb, stream);
+    case HX_DTYPE_BF16: break;
     }
     return fail(HX_ERR_INVALID_CONFIGURATION, "unknown dtype %d", (int)a.dtype);
 }

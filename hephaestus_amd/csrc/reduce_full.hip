@@ -470,6 +470,7 @@ hx_status launch_full_reduce(const FullReduceArgs &a, void *ws, uint64_t ws_byte
                         : launch_kind<float, false>(a, ws, ws_bytes, lb, stream);
     case HX_DTYPE_U32: return launch_kind<uint32_t, false>(a, ws, ws_bytes, lb, stream);
     case HX_DTYPE_I32: return launch_kind<int32_t, false>(a, ws, ws_bytes, lb, stream);
+    case HX_DTYPE_BF16: break;
     }
     return fail(HX_ERR_INVALID_CONFIGURATION, "unknown dtype %d", (int)a.dtype);
 }

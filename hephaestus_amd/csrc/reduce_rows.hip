@@ -1205,6 +1205,7 @@ hx_status launch_rows_any(const RowParams &p, hx_dtype dtype, bool affine, int f
                       : launch_rows_flags<float, false>(p, flags, cols_layout, ws, ws_bytes, stream);
     case HX_DTYPE_U32: return launch_rows_flags<uint32_t, false>(p, flags, cols_layout, ws, ws_bytes, stream);
     case HX_DTYPE_I32: return launch_rows_flags<int32_t, false>(p, flags, cols_layout, ws, ws_bytes, stream);
+    case HX_DTYPE_BF16: break;
     }
     return fail(HX_ERR_INVALID_CONFIGURATION, "unknown dtype %d", (int)dtype);
 }

@@ -3159,6 +3159,7 @@ hx_status launch_scan(const ScanArgs &a, void *ws, uint64_t ws_bytes, LookbackSt
         // Two's complement: i32 sums and products have the bits of u32 ones.
         return prod ? launch_op<uint32_t, OpProd>(a, ws, ws_bytes, lb, stream)
                     : launch_op<uint32_t, OpSum>(a, ws, ws_bytes, lb, stream);
+    case HX_DTYPE_BF16: break;
     }
     return fail(HX_ERR_INVALID_CONFIGURATION, "unknown dtype %d", (int)a.dtype);
 }

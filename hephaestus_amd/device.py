@@ -15,11 +15,31 @@ import numpy as np
 
 from . import _ffi, errors
 
+# bfloat16 as numpy holds it: 16 bits an element, named so that it differs from
+# uint16.  `bfloat16_from_float32` and `float32_from_bfloat16` convert.
+bfloat16 = np.dtype([("bfloat16", "<u2")])
+
 DTYPES = {
     np.dtype(np.float32): _ffi.DTYPE_F32,
     np.dtype(np.uint32): _ffi.DTYPE_U32,
     np.dtype(np.int32): _ffi.DTYPE_I32,
+    bfloat16: _ffi.DTYPE_BF16,
 }
+
+
+def bfloat16_from_float32(values) -> np.ndarray:
+    """The nearest bfloat16 values, halfway cases to even; NaN stays NaN."""
+    values = np.ascontiguousarray(values, dtype=np.float32)
+    bits = values.view(np.uint32)
+    rounded = (bits + 0x7FFF + ((bits >> 16) & 1)) >> 16
+    rounded = np.where(np.isnan(values), (bits >> 16) | 0x40, rounded)
+    return rounded.astype(np.uint16).view(bfloat16)
+
+
+def float32_from_bfloat16(values) -> np.ndarray:
+    """bfloat16 values as float32, exactly."""
+    values = np.ascontiguousarray(values, dtype=bfloat16)
+    return (values.view(np.uint16).astype(np.uint32) << 16).view(np.float32)
 
 
 def hx_dtype(dtype) -> int:
@@ -133,11 +153,12 @@ class PlacementHint:
 class RocmBuffer:
     """A typed, device-resident linear buffer of `len` elements."""
 
-    def __init__(self, device: "RocmDevice", ptr: int | None, length: int, dtype):
+    def __init__(self, device: "RocmDevice", ptr: int | None, length: int, dtype, owner=None):
         self.device = device
         self.ptr = ptr or None
         self._len = int(length)
         self.dtype = np.dtype(dtype)
+        self.owner = owner  # of borrowed memory (RocmDevice.borrow); None: this buffer frees it
 
     def __len__(self) -> int:
         return self._len
@@ -156,7 +177,7 @@ class RocmBuffer:
         return self.dtype.itemsize
 
     def free(self) -> None:
-        if self.ptr and self.device is not None and self.device.handle:
+        if self.ptr and self.owner is None and self.device is not None and self.device.handle:
             _ffi.check(_ffi.lib().hx_free(self.device.handle, self.ptr))
         self.ptr = None
 
@@ -286,6 +307,19 @@ class RocmDevice:
 
     def alloc_uninitialized(self, dtype, length: int) -> RocmBuffer:
         return self._alloc(dtype, length, False)
+
+    def borrow(self, ptr: int, dtype, length: int, owner) -> RocmBuffer:
+        """`length` elements at device address `ptr` as a buffer that another
+        library owns: `owner` (any object that keeps the memory alive, such as
+        a torch tensor) is held by the buffer, which frees nothing.  Work that
+        the owner has queued on other streams is the caller's to order."""
+        if np.dtype(dtype).hasobject:
+            raise errors.InvalidConfiguration(f"unsupported element type {np.dtype(dtype)}")
+        if owner is None:
+            raise errors.InvalidConfiguration("borrowed memory needs the object that owns it")
+        if int(length) < 0 or (int(length) > 0 and not ptr):
+            raise errors.InvalidConfiguration("borrowed memory needs an address and a length")
+        return RocmBuffer(self, int(ptr or 0), length, dtype, owner)
 
     def upload(self, host) -> RocmBuffer:
         host = np.ascontiguousarray(host)

@@ -46,9 +46,11 @@
  * hx_reduce_full, hx_argmax_full, hx_reduce_axis, hx_reduce_rows,
  * hx_segmented_reduce, hx_map_reduce, hx_trace) draw a fresh tag per call
  * and may grow their stream's buffers, so on a capturing stream they fail
- * with HX_ERR_DISPATCH_FAILED before anything is queued; hx_scan_noalloc,
- * the vector forms, hx_copy_async and hx_fill_random queue plain kernels and
- * may be captured.
+ * with HX_ERR_DISPATCH_FAILED before anything is queued, and so do the
+ * immediate layer operators that take scratch (hx_matmul_i8,
+ * hx_linear_attention); hx_scan_noalloc, the vector forms, hx_copy_async,
+ * hx_fill_random and hx_rms_norm_quantize queue plain kernels and may be
+ * captured.
  */
 #ifndef HX_H
 #define HX_H
@@ -80,7 +82,8 @@ typedef enum hx_status {
 typedef enum hx_dtype {
     HX_DTYPE_F32 = 0, /* DialectScalar<HipC> "float"        core dialect.rs:116-126 */
     HX_DTYPE_U32 = 1, /* "unsigned int"; sums wrap mod 2^32 */
-    HX_DTYPE_I32 = 2  /* "int"; two's complement wrap       */
+    HX_DTYPE_I32 = 2, /* "int"; two's complement wrap       */
+    HX_DTYPE_BF16 = 3 /* bfloat16; layer operators only     */
 } hx_dtype;
 
 /* Combining operators: crates/hephaestus-core/src/domain/ops.rs:735-803
@@ -510,6 +513,99 @@ hx_status hx_vector_binary(hx_device *dev, hx_vector_op op, hx_dtype dtype,
                            const void *left, uint64_t left_len,
                            const void *right, uint64_t right_len, void *out,
                            uint64_t out_len, hx_stream stream);
+
+/* ------------------------------------------------------- layer operators */
+/* What a layer of a linear-attention model, served in 8 bits, is made of
+ * (no counterpart in the reference).  `dtype` is F32 or BF16 and sums are
+ * taken in 32 bits either way.  Operands are strided views whose last
+ * dimension is contiguous (stride 1, or an extent of at most 1); other
+ * strides are free, zero and negative ones included, at any alignment of
+ * the elements.  Outputs must not overlap themselves, each other or an
+ * input, except where stated.  Empty outputs are a no-op. */
+
+/* Rows of a residual stream, normalised and quantised in one pass over the
+ * data.  x is [rows, cols]:
+ *   h     = x + residual                     (residual may be NULL: h = x)
+ *   y     = h * (mean of h^2 + epsilon)^(-1/2) * weight   (weight[cols], dtype)
+ *   s     = max |y| / 127,  q = y / s rounded half to even, in [-127, 127]
+ * residual_out (may be NULL) receives h, rounded to dtype; y is taken from h
+ * before that rounding.  `quantized` is an int8 view of x's shape, `scales`
+ * f32[rows].  A row of zeros has s = 0 and q = 0; a row with a NaN or an
+ * infinity in h or h * weight, or whose sum of squares exceeds the range of
+ * f32, has s = NaN and q = 0.  residual_out may be the very view of x or of residual. */
+hx_status hx_rms_norm_quantize(hx_device *dev, hx_dtype dtype, const void *x,
+                               uint64_t x_buf_len, const hx_layout *x_layout,
+                               const void *residual, uint64_t residual_buf_len,
+                               const hx_layout *residual_layout,
+                               const void *weight, uint64_t weight_len,
+                               float epsilon, void *residual_out,
+                               uint64_t residual_out_buf_len,
+                               const hx_layout *residual_out_layout,
+                               void *quantized, uint64_t quantized_buf_len,
+                               const hx_layout *quantized_layout, float *scales,
+                               uint64_t scales_len, hx_stream stream);
+hx_status hx_prepare_rms_norm_quantize(
+    hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *residual, uint64_t residual_buf_len,
+    const hx_layout *residual_layout, const void *weight, uint64_t weight_len,
+    float epsilon, void *residual_out, uint64_t residual_out_buf_len,
+    const hx_layout *residual_out_layout, void *quantized,
+    uint64_t quantized_buf_len, const hx_layout *quantized_layout,
+    float *scales, uint64_t scales_len, hx_plan **plan);
+
+/* Product of 8-bit integers with a scale for each token (row of a) and each
+ * channel (row of b):
+ *   out[m, n] = a_scales[m] * b_scales[n] * sum over k of a[m, k] * b[n, k]
+ * a is int8 [m, k], b int8 [n, k], out [m, n] of `dtype`.  The sum is exact in
+ * 32-bit integers, so k is at most 131071; k = 0 gives zeros. */
+hx_status hx_matmul_i8(hx_device *dev, const void *a, uint64_t a_buf_len,
+                       const hx_layout *a_layout, const float *a_scales,
+                       uint64_t a_scales_len, const void *b, uint64_t b_buf_len,
+                       const hx_layout *b_layout, const float *b_scales,
+                       uint64_t b_scales_len, hx_dtype dtype, void *out,
+                       uint64_t out_buf_len, const hx_layout *out_layout,
+                       hx_stream stream);
+hx_status hx_prepare_matmul_i8(hx_device *dev, const void *a,
+                               uint64_t a_buf_len, const hx_layout *a_layout,
+                               const float *a_scales, uint64_t a_scales_len,
+                               const void *b, uint64_t b_buf_len,
+                               const hx_layout *b_layout, const float *b_scales,
+                               uint64_t b_scales_len, hx_dtype dtype, void *out,
+                               uint64_t out_buf_len, const hx_layout *out_layout,
+                               hx_plan **plan);
+
+/* Linear attention with a decay for each head: a prefix scan of matrices.
+ *   S_t = exp(log_decay[h]) * S_{t-1} + k_t^T v_t,   o_t = scale * q_t S_t
+ * q is [batch, tokens, heads, dk], k [batch, tokens, kv_heads, dk], v [batch,
+ * tokens, kv_heads, dv], out [batch, tokens, heads, dv], all of `dtype`, with
+ * heads a multiple of kv_heads (head h reads key/value head
+ * h * kv_heads / heads) and dk at most 256.  log_decay is f32[heads], each at
+ * most 0 (minus infinity: no memory).  state_in and state_out are f32 views
+ * [batch, heads, dk, dv] of the state before the first and after the last
+ * token; either may be NULL (state_in: zeros), and they may be the very same
+ * view.  `lengths` (u32[batch], or NULL for `tokens` everywhere) counts each
+ * sequence's tokens, at most `tokens`: later rows of q, k and v are not read,
+ * later rows of out are 0, and a sequence of no tokens keeps its state. */
+hx_status hx_linear_attention(
+    hx_device *dev, hx_dtype dtype, const void *q, uint64_t q_buf_len,
+    const hx_layout *q_layout, const void *k, uint64_t k_buf_len,
+    const hx_layout *k_layout, const void *v, uint64_t v_buf_len,
+    const hx_layout *v_layout, const float *log_decay, uint64_t log_decay_len,
+    float scale, const float *state_in, uint64_t state_in_buf_len,
+    const hx_layout *state_in_layout, float *state_out,
+    uint64_t state_out_buf_len, const hx_layout *state_out_layout,
+    const uint32_t *lengths, uint64_t lengths_len, void *out,
+    uint64_t out_buf_len, const hx_layout *out_layout, hx_stream stream);
+hx_status hx_prepare_linear_attention(
+    hx_device *dev, hx_dtype dtype, const void *q, uint64_t q_buf_len,
+    const hx_layout *q_layout, const void *k, uint64_t k_buf_len,
+    const hx_layout *k_layout, const void *v, uint64_t v_buf_len,
+    const hx_layout *v_layout, const float *log_decay, uint64_t log_decay_len,
+    float scale, const float *state_in, uint64_t state_in_buf_len,
+    const hx_layout *state_in_layout, float *state_out,
+    uint64_t state_out_buf_len, const hx_layout *state_out_layout,
+    const uint32_t *lengths, uint64_t lengths_len, void *out,
+    uint64_t out_buf_len, const hx_layout *out_layout, hx_plan **plan);
 
 /* ---------------------------------------------------------------- plans */
 
