@@ -21,7 +21,6 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kDepth = 128; // bytes of k a step
-constexpr int kWaitLoads = 0x0F70; // s_waitcnt vmcnt(0)
 
 __device__ __forceinline__ i32x4v mma(i32x4v b, i32x4v a, i32x4v sum) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, sum, 0, 0, 0);
@@ -62,105 +61,127 @@ __device__ __forceinline__ void store_scaled(T *row, uint64_t n, uint64_t end, i
 }
 
 // ------------------------------------------------------------------ skinny
-// Up to 16·MF tokens; a block takes 16·NF channels, each of its eight waves
-// every eighth 128 bytes of k.
+// Up to 16 tokens; a block takes 16·NF channels, each of its eight waves every
+// eighth 128 bytes of k.
 constexpr int kSkinnyWaves = 8;
 
-template <typename T, int MF, int NF>
+template <typename T, int NF>
 __global__ __launch_bounds__(kSkinnyWaves *kWave) void matmul_skinny_kernel(MatmulArgs p) {
-    __shared__ int sums[MF * NF * 4 * kWave];
+    __shared__ int sums[NF * 4 * kWave];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint64_t n0 = (uint64_t)blockIdx.x * (16 * NF);
     const uint32_t k_end = (uint32_t)p.k, at = lane / 16 * 16;
-    for (int i = threadIdx.x; i < MF * NF * 4 * kWave; i += kSkinnyWaves * kWave) sums[i] = 0;
-    const int8_t *a[MF], *b[NF];
-    uint32_t a_end[MF];
-#pragma unroll
-    for (int i = 0; i < MF; ++i) {
-        const uint64_t m = 16 * i + lane % 16;
-        a_end[i] = m < p.m ? k_end : 0; // rows that are not there are zeros
-        a[i] = p.a + (int64_t)(m < p.m ? m : 0) * p.a_stride;
-    }
+    for (int i = threadIdx.x; i < NF * 4 * kWave; i += kSkinnyWaves * kWave) sums[i] = 0;
+    const uint64_t m = lane % 16;
+    const uint32_t a_end = m < p.m ? k_end : 0; // rows that are not there are zeros
+    const int8_t *a = p.a + (int64_t)(m < p.m ? m : 0) * p.a_stride, *b[NF];
 #pragma unroll
     for (int j = 0; j < NF; ++j) // channels past the end are summed and dropped
         b[j] = p.b + (int64_t)min(n0 + 16 * j + lane % 16, p.n - 1) * p.b_stride;
-    i32x4v acc[MF][NF] = {};
+    i32x4v acc[NF] = {};
     const uint32_t whole = k_end / kDepth * kDepth;
-    for (uint32_t k = wave * kDepth; k < whole; k += kSkinnyWaves * kDepth) {
-        i32x4v fb[NF][2], fa[MF][2];
+    constexpr uint32_t kTurn = kSkinnyWaves * kDepth;
+    // The next turn's bytes are on their way while this turn is summed.
+    struct Turn {
+        i32x4v b[NF][2], a[2];
+    } now, next;
+    const auto fetch = [&](uint32_t k, Turn &t) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
             for (int j = 0; j < NF; ++j)
-                fb[j][s] = __builtin_bit_cast(i32x4v, __builtin_nontemporal_load((const u32x4_any *)(b[j] + k + 64 * s + at)));
-#pragma unroll
-            for (int i = 0; i < MF; ++i)
-                fa[i][s] = a_end[i] ? __builtin_bit_cast(i32x4v, (u32x4)*(const u32x4_any *)(a[i] + k + 64 * s + at))
-                                    : i32x4v{0, 0, 0, 0};
+                t.b[j][s] = __builtin_bit_cast(i32x4v, (u32x4)*(const u32x4_any *)(b[j] + k + 64 * s + at));
+            t.a[s] = a_end ? __builtin_bit_cast(i32x4v, (u32x4)*(const u32x4_any *)(a + k + 64 * s + at))
+                           : i32x4v{0, 0, 0, 0};
         }
+    };
+    // Blocks begin at different turns: rows a power of two apart lie on the
+    // same memory channels, and blocks in step would all ask the same ones
+    // (1 x 4096 x 4096: 7.1 us in step, 5.4 us so).
+    const uint32_t first = wave * kDepth, turns = whole > first ? (whole - first + kTurn - 1) / kTurn : 0;
+    uint32_t t = turns ? blockIdx.x / 8 % turns : 0;
+    if (turns) fetch(first + t * kTurn, now);
+    for (uint32_t left = turns; left; --left) {
+        t = t + 1 < turns ? t + 1 : 0;
+        if (left > 1) fetch(first + t * kTurn, next);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int j = 0; j < NF; ++j)
-#pragma unroll
-                for (int i = 0; i < MF; ++i) acc[i][j] = mma(fb[j][s], fa[i][s], acc[i][j]);
+            for (int j = 0; j < NF; ++j) acc[j] = mma(now.b[j][s], now.a[s], acc[j]);
+        now = next;
     }
     // The last, partial 128 bytes: to the wave whose turn it is.
     if (whole < k_end && wave == (int)(whole / kDepth % kSkinnyWaves)) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
+            const uint32_t k = whole + 64 * s + at;
+            const i32x4v fa = load_bytes(a, k, a_end);
 #pragma unroll
-            for (int j = 0; j < NF; ++j) {
-                const i32x4v fb = load_bytes(b[j], whole + 64 * s + at, k_end);
-#pragma unroll
-                for (int i = 0; i < MF; ++i)
-                    acc[i][j] = mma(fb, load_bytes(a[i], whole + 64 * s + at, a_end[i]), acc[i][j]);
-            }
+            for (int j = 0; j < NF; ++j) acc[j] = mma(load_bytes(b[j], k, k_end), fa, acc[j]);
+        }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < MF; ++i)
+    for (int j = 0; j < NF; ++j)
 #pragma unroll
-        for (int j = 0; j < NF; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) atomicAdd(&sums[((i * NF + j) * 4 + e) * kWave + lane], acc[i][j][e]);
+        for (int e = 0; e < 4; ++e) atomicAdd(&sums[(j * 4 + e) * kWave + lane], acc[j][e]);
     __syncthreads();
-    for (int f = wave; f < MF * NF; f += kSkinnyWaves) {
-        const uint64_t m = 16 * (f / NF) + lane % 16, n = n0 + 16 * (f % NF) + lane / 16 * 4;
-        if (m >= p.m) continue;
-        i32x4v s;
+    if (wave >= NF || m >= p.m) return;
+    i32x4v s;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = sums[(f * 4 + e) * kWave + lane];
-        store_scaled((T *)p.out + (int64_t)m * p.out_stride, n, p.n, s, p.a_scales[m], p.b_scales);
-    }
+    for (int e = 0; e < 4; ++e) s[e] = sums[(wave * 4 + e) * kWave + lane];
+    store_scaled((T *)p.out + (int64_t)m * p.out_stride, n0 + 16 * wave + lane / 16 * 4, p.n, s, p.a_scales[m],
+                 p.b_scales);
 }
 
-template <typename T, int MF> hx_status launch_skinny(const MatmulArgs &p, hipStream_t stream) {
-    const auto run = [&](auto nf) {
-        constexpr int NF = decltype(nf)::value;
-        hipLaunchKernelGGL((matmul_skinny_kernel<T, MF, NF>), dim3((uint32_t)ceil_div(p.n, 16 * NF)),
-                           dim3(kSkinnyWaves * kWave), 0, stream, p);
+template <typename T> hx_status launch_skinny(const MatmulArgs &p, hipStream_t stream) {
+    const auto run = [&](auto kernel, uint64_t channels) {
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)ceil_div(p.n, channels)), dim3(kSkinnyWaves * kWave), 0, stream, p);
     };
-    if (p.n >= 16 * 2 * 256) run(std::integral_constant<int, 2>{});
-    else run(std::integral_constant<int, 1>{});
+    // Two fragments of channels a block halve its reads of a, from the size
+    // on where there is a block for each CU all the same.
+    if (p.n >= 2 * 16 * 256) run(matmul_skinny_kernel<T, 2>, 32);
+    else run(matmul_skinny_kernel<T, 1>, 16);
     return check_launch("matmul_skinny_kernel");
 }
 
 // ------------------------------------------------------------------- tiles
-// BM tokens by BN channels a block of WM x WN waves.  A step's 128 bytes of k
-// of each row lie in LDS as eight chunks of 16, chunk c of row r at place
-// c ^ (r % 8), so that the 16 rows that a matrix instruction reads at one c
-// fall on all banks.  DIRECT loads go from memory to LDS without registers:
-// each wave's 64 chunks of an instruction land side by side, and the exchange
-// of places is made on the global side.  They need rows whose addresses and
-// lengths are multiples of 16; other rows pass through registers.
-template <typename T, int BM, int BN, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__(WM *WN *kWave) void matmul_tiles_kernel(MatmulArgs p, uint32_t tiles_m, uint32_t tiles_n) {
-    constexpr int kThreads = WM * WN * kWave, kRows = BM + BN, kStage = kRows * kDepth;
-    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    constexpr int kLoads = kRows * 8 / kThreads; // chunks of 16 bytes a thread and step
-    extern __shared__ __align__(16) int8_t lds[]; // two stages
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+// BM tokens by BN channels a block.  Its WM x WN waves each take a part of the
+// tile; with KG > 1 there are KG such groups, which take the steps of k in turn
+// and add their sums in LDS.  A step's 128 bytes of k of each row lie in LDS as
+// eight chunks of 16, chunk c of row r at place c ^ (r % 8), so that the 16 rows
+// that a matrix instruction reads at one c fall on all banks.
+//
+// Loads go from memory to LDS without registers, S - 1 steps ahead: each
+// wave's 64 chunks of an instruction land side by side, and the exchange of
+// places is made on the global side.  They need rows that begin on dwords;
+// others are copied to such rows first.
+//
+// The barrier between steps is written out: all of the wave's LDS reads and
+// writes and all but its last N loads have ended when it is passed.
+// __syncthreads would wait for every load.
+template <int N> __device__ __forceinline__ void step_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
+
+template <int BM, int BN, int WM, int WN, int KG, int S> struct Tile {
+    static constexpr int kWaves = WM * WN, kThreads = kWaves * KG * kWave;
+    static constexpr int kRows = BM + BN, kStage = kRows * kDepth, kLds = kStage * S * KG;
+    static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    static constexpr int kLoads = kRows * 8 / (kWaves * kWave); // chunks a thread and step
+    static_assert(kLds <= 160 * 1024 && kLoads * 8 * kWaves == kRows && (S - 2) * kLoads < 64);
+    static_assert(KG == 1 || BM * BN * 4 <= kLds);
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int KG, int S>
+__global__ __launch_bounds__(WM *WN *KG *kWave, 2) void matmul_tiles_kernel(MatmulArgs p, uint32_t tiles_m,
+                                                                        uint32_t tiles_n) {
+    using C = Tile<BM, BN, WM, WN, KG, S>;
+    constexpr int FM = C::FM, FN = C::FN, kLoads = C::kLoads;
+    extern __shared__ __align__(16) int8_t lds[];
+    const int lane = lane_id(), block_wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wave = block_wave % C::kWaves, group = block_wave / C::kWaves;
+    int8_t *stages = lds + group * (S * C::kStage);
 
     // Blocks go to the eight XCDs in turn: each XCD takes a run of tiles, in
     // strips of eight tiles of m so that its L2 serves both operands.
@@ -171,50 +192,19 @@ __global__ __launch_bounds__(WM *WN *kWave) void matmul_tiles_kernel(MatmulArgs 
     const uint32_t height = min(8u, tiles_m - 8 * strip);
     const uint64_t m0 = (uint64_t)(8 * strip + in_strip % height) * BM, n0 = (uint64_t)(in_strip / height) * BN;
 
-    const uint32_t k_end = (uint32_t)p.k;
-    // A thread's chunk of each row it loads: rows past the operands repeat the
-    // last one and are dropped at the end.
-    const uint32_t place = threadIdx.x % 8, row0 = DIRECT ? wave * (kLoads * 8) + lane / 8 : threadIdx.x / 8;
-    constexpr uint32_t kRowStep = DIRECT ? 8 : kThreads / 8;
-    const uint32_t chunk = (place ^ (row0 % 8)) * 16;
+    const uint32_t k_end = (uint32_t)p.k, steps = (k_end + kDepth - 1) / kDepth, whole = k_end / kDepth;
+    const uint32_t turns = (steps + KG - 1) / KG; // this group's step of turn t: t·KG + group
+    // A thread's chunk of each row that it loads: rows past the operands
+    // repeat the last one and are dropped at the end.
+    const uint32_t row0 = wave * (kLoads * 8) + lane / 8, place = lane % 8, chunk = (place ^ (row0 % 8)) * 16;
     const int8_t *src[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-        const uint32_t r = row0 + j * kRowStep;
-        src[j] = (r < BM ? p.a + (int64_t)min(m0 + r, p.m - 1) * p.a_stride
-                         : p.b + (int64_t)min(n0 + (r - BM), p.n - 1) * p.b_stride) + chunk;
+        const uint32_t r = row0 + j * 8;
+        src[j] = r < BM ? p.a + (int64_t)min(m0 + r, p.m - 1) * p.a_stride
+                        : p.b + (int64_t)min(n0 + (r - BM), p.n - 1) * p.b_stride;
     }
-    u32x4 held[DIRECT ? 1 : kLoads];
-
-    const auto fetch = [&](uint32_t k, int8_t *stage) {
-        if constexpr (DIRECT) {
-            if (k + kDepth <= k_end) {
-#pragma unroll
-                for (int j = 0; j < kLoads; ++j)
-                    __builtin_amdgcn_global_load_lds((const void *)(src[j] + k),
-                                                     (lds_void *)(stage + (wave * kLoads + j) * 1024), 16, 0, 0);
-            } else { // chunks past the end are zeros
-#pragma unroll
-                for (int j = 0; j < kLoads; ++j) {
-                    if (k + chunk < k_end)
-                        __builtin_amdgcn_global_load_lds((const void *)(src[j] + k),
-                                                         (lds_void *)(stage + (wave * kLoads + j) * 1024), 16, 0, 0);
-                    else *(u32x4 *)(stage + (wave * kLoads + j) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-                held[j] = __builtin_bit_cast(u32x4, load_bytes(src[j] - chunk, k + chunk, k_end));
-        }
-    };
-    const auto settle = [&](int8_t *stage) {
-        if constexpr (!DIRECT) {
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-                *(u32x4 *)(stage + (row0 + j * kRowStep) * kDepth + place * 16) = held[j];
-        }
-    };
+    const uint32_t to = wave * (kLoads * 1024); // this wave's first row in a stage
 
     const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
     const uint32_t swizzled = (lane / 16 ^ (lane % 8)) * 16; // of k bytes 0..63; 64..127: ^ 64
@@ -235,72 +225,167 @@ __global__ __launch_bounds__(WM *WN *kWave) void matmul_tiles_kernel(MatmulArgs 
         }
     };
 
-    // The barrier itself does not wait for direct loads.
-    const auto sync = [&] {
-        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(kWaitLoads);
-        __syncthreads();
+    // Whole steps: no branch in the loads.
+    const auto fetch = [&](uint32_t t) {
+        int8_t *stage = stages + t % S * C::kStage + to;
+        const uint32_t k = (t * KG + group) * kDepth + chunk;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j)
+            __builtin_amdgcn_global_load_lds((const void *)(src[j] + k), (lds_void *)(stage + j * 1024), 16, 0, 0);
     };
-    if (k_end) {
-        fetch(0, lds);
-        settle(lds);
-        sync();
-        uint32_t stage = 0;
-        for (uint32_t k = 0; k < k_end; k += kDepth, stage ^= 1) {
-            int8_t *next = lds + (stage ^ 1) * kStage;
-            const bool more = k + kDepth < k_end;
-            if (more) fetch(k + kDepth, next);
-            compute(lds + stage * kStage);
-            if (more) settle(next);
-            sync();
-        }
+    // The step of the last, partial 128 bytes: zeros past the end of k.
+    const auto fetch_rest = [&](uint32_t t) {
+        int8_t *stage = stages + t % S * C::kStage + to;
+        for (int j = 0; j < kLoads; ++j)
+            *(i32x4v *)(stage + j * 1024 + lane * 16) = load_bytes(src[j], whole * kDepth + chunk, k_end);
+    };
+    const auto fetch_any = [&](uint32_t t) {
+        const uint32_t q = t * KG + group;
+        if (q < whole) fetch(t);
+        else if (q < steps) fetch_rest(t);
+    };
+    for (int t = 0; t < S - 1; ++t) fetch_any(t);
+    // Step t has landed once no more loads are under way than those of the
+    // S - 2 steps behind it.
+    const uint32_t mine = whole > (uint32_t)group ? (whole - group + KG - 1) / KG : 0; // whole steps of this group
+    uint32_t t = 0;
+    for (; t + (S - 1) < mine; ++t) {
+        step_barrier<(S - 2) * kLoads>();
+        fetch(t + S - 1);
+        compute(stages + t % S * C::kStage);
     }
+    for (; t < turns; ++t) { // the last ones, not all of them direct loads
+        step_barrier<0>();
+        if (t + S - 1 < turns) fetch_any(t + S - 1);
+        if (t * KG + group < steps) compute(stages + t % S * C::kStage);
+    }
+
+    const uint32_t token = wm + lane % 16, channel = wn + lane / 16 * 4; // of the tile, and 16·i, 16·j on
+    if constexpr (KG > 1) {
+        int *sums = (int *)lds;
+        __syncthreads();
+        for (int i = threadIdx.x; i < BM * BN; i += C::kThreads) sums[i] = 0;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const uint64_t m = m0 + wm + 16 * i + lane % 16;
-        if (m >= p.m) continue;
-        const float sa = p.a_scales[m];
-        T *row = (T *)p.out + (int64_t)m * p.out_stride;
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-            store_scaled(row, n0 + wn + 16 * j + lane / 16 * 4, p.n, acc[i][j], sa, p.b_scales);
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    atomicAdd(&sums[((wave * FM * FN + i * FN + j) * 4 + e) * kWave + lane], acc[i][j][e]);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                if ((i * FN + j) % KG != group) continue; // the groups share the fragments
+                const uint64_t m = m0 + token + 16 * i;
+                if (m >= p.m) continue;
+                i32x4v v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = sums[((wave * FM * FN + i * FN + j) * 4 + e) * kWave + lane];
+                store_scaled((T *)p.out + (int64_t)m * p.out_stride, n0 + channel + 16 * j, p.n, v, p.a_scales[m],
+                             p.b_scales);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const uint64_t m = m0 + token + 16 * i;
+            if (m >= p.m) continue;
+            const float sa = p.a_scales[m];
+            T *row = (T *)p.out + (int64_t)m * p.out_stride;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) store_scaled(row, n0 + channel + 16 * j, p.n, acc[i][j], sa, p.b_scales);
+        }
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool DIRECT>
+template <typename T, int BM, int BN, int WM, int WN, int KG, int S>
 hx_status launch_tiles(const MatmulArgs &p, hipStream_t stream) {
-    constexpr uint32_t kLds = 2 * (BM + BN) * kDepth;
-    const auto kernel = matmul_tiles_kernel<T, BM, BN, WM, WN, DIRECT>;
-    if constexpr (kLds > 65536) {
+    using C = Tile<BM, BN, WM, WN, KG, S>;
+    const auto kernel = matmul_tiles_kernel<T, BM, BN, WM, WN, KG, S>;
+    if constexpr (C::kLds > 65536) {
         static const hipError_t allowed =
-            hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+            hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
         if (allowed != hipSuccess) return hip_fail(HX_ERR_DISPATCH_FAILED, allowed, "matmul LDS size");
     }
     const uint64_t tm = ceil_div(p.m, BM), tn = ceil_div(p.n, BN);
     if (tm * tn > 0x7FFFFFFFull)
         return fail(HX_ERR_DISPATCH_FAILED, "matmul of %llu tiles exceeds the grid range", (unsigned long long)(tm * tn));
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(WM * WN * kWave), kLds, stream, p, (uint32_t)tm,
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(C::kThreads), C::kLds, stream, p, (uint32_t)tm,
                        (uint32_t)tn);
     return check_launch("matmul_tiles_kernel");
 }
 
-template <typename T> hx_status launch(const MatmulArgs &p, hipStream_t stream) {
-    if (p.m <= 16) return launch_skinny<T, 1>(p, stream);
-    if (p.m <= 32) return launch_skinny<T, 2>(p, stream);
-    if (p.m <= 64) return launch_skinny<T, 4>(p, stream);
-    const bool direct = (((uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.a_stride | (uint64_t)p.b_stride | p.k) % 16) == 0;
-    if (!direct) return launch_tiles<T, 64, 64, 2, 2, false>(p, stream);
-    if (ceil_div(p.m, 256) * ceil_div(p.n, 256) >= 200) return launch_tiles<T, 256, 256, 2, 4, true>(p, stream);
-    if (ceil_div(p.m, 128) * ceil_div(p.n, 128) >= 200) return launch_tiles<T, 128, 128, 2, 2, true>(p, stream);
-    return launch_tiles<T, 64, 64, 2, 2, true>(p, stream);
+// The largest tile of which there are enough for the 256 CUs (from 160 on: a
+// smaller tile moves more bytes to the same CUs).  Where there are more tiles
+// than CUs two blocks share one, with LDS for half the steps in flight; the
+// smaller the tile, the more groups share a block's k.  Measured (us):
+//   1000 x 8192 x 8192   128 x 128 71.1    64 x 64 109     256 x 256 115
+//   2048 x 2048 x 2048   128 x 128 16.6    64 x 64 19.0    256 x 256 37.8
+//   300 x 2048 x 2048    64 x 64 6.5       64 x 32 8.0     128 x 128 12.7
+//   256 x 1024 x 8192    32 x 32 10.2      64 x 32 13.5    64 x 64 17.4
+//   20 x 4096 x 4096     32 x 16 6.0       32 x 32 7.0     64 x 32 8.3
+template <typename T> hx_status launch_tiled(const MatmulArgs &p, hipStream_t stream) {
+    const auto tiles = [&](uint64_t bm, uint64_t bn) { return ceil_div(p.m, bm) * ceil_div(p.n, bn); };
+    constexpr uint64_t kEnough = 160, kCus = 256;
+    if (tiles(256, 256) >= kEnough) return launch_tiles<T, 256, 256, 2, 4, 1, 2>(p, stream);
+    if (tiles(128, 128) > kCus) return launch_tiles<T, 128, 128, 2, 2, 1, 2>(p, stream);
+    if (tiles(128, 128) >= kEnough) return launch_tiles<T, 128, 128, 2, 4, 1, 4>(p, stream);
+    if (tiles(64, 64) > kCus) return launch_tiles<T, 64, 64, 2, 2, 2, 2>(p, stream);
+    if (tiles(64, 64) >= kEnough) return launch_tiles<T, 64, 64, 2, 2, 4, 2>(p, stream);
+    if (tiles(64, 32) > kCus) return launch_tiles<T, 64, 32, 2, 1, 3, 2>(p, stream);
+    if (tiles(64, 32) >= kEnough) return launch_tiles<T, 64, 32, 2, 1, 6, 2>(p, stream);
+    if (tiles(32, 32) > kCus) return launch_tiles<T, 32, 32, 1, 2, 4, 2>(p, stream);
+    if (tiles(32, 32) >= kEnough) return launch_tiles<T, 32, 32, 1, 2, 8, 2>(p, stream);
+    return launch_tiles<T, 32, 16, 1, 1, 8, 3>(p, stream);
+}
+
+// ----------------------------------------------------------- rows on dwords
+// Rows of a and b at any byte, copied to rows of whole 128 bytes with zeros
+// after their ends.  Loading such rows through registers in every tile took
+// 29 us for 1000 x 1027 x 4099; the copy and then direct loads take 23.
+__global__ __launch_bounds__(256) void matmul_align_kernel(MatmulArgs p, int8_t *rows, uint32_t pitch) {
+    const uint32_t chunk = (blockIdx.x * 256 + threadIdx.x) * 16;
+    if (chunk >= pitch) return;
+    for (uint64_t r = blockIdx.y; r < p.m + p.n; r += gridDim.y) {
+        const int8_t *from = r < p.m ? p.a + (int64_t)r * p.a_stride : p.b + (int64_t)(r - p.m) * p.b_stride;
+        *(i32x4v *)(rows + r * pitch + chunk) = load_bytes(from, chunk, (uint32_t)p.k);
+    }
+}
+
+constexpr uint64_t kSkinnyTokens = 16;
+
+bool needs_copy(const MatmulArgs &p) {
+    const uint64_t bits = (uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.a_stride | (uint64_t)p.b_stride;
+    return p.m > kSkinnyTokens && p.k > 0 && bits % 4 != 0;
+}
+uint64_t copy_pitch(const MatmulArgs &p) { return ceil_div(p.k, kDepth) * kDepth; }
+
+template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t stream) {
+    if (p.m <= kSkinnyTokens) return launch_skinny<T>(p, stream);
+    if (needs_copy(p)) {
+        const uint32_t pitch = (uint32_t)copy_pitch(p);
+        const dim3 grid((uint32_t)ceil_div(pitch, 256 * 16), (uint32_t)min(p.m + p.n, (uint64_t)65535));
+        hipLaunchKernelGGL(matmul_align_kernel, grid, dim3(256), 0, stream, p, (int8_t *)ws, pitch);
+        HX_TRY(check_launch("matmul_align_kernel"));
+        p.a = (const int8_t *)ws;
+        p.b = p.a + p.m * pitch;
+        p.a_stride = p.b_stride = pitch;
+        p.k = pitch;
+    }
+    return launch_tiled<T>(p, stream);
 }
 
 } // namespace
 
-uint64_t matmul_i8_workspace_bytes(const MatmulArgs &) { return 0; }
+uint64_t matmul_i8_workspace_bytes(const MatmulArgs &args) {
+    return args.m && args.n && needs_copy(args) ? (args.m + args.n) * copy_pitch(args) : 0;
+}
 
-hx_status launch_matmul_i8(const MatmulArgs &args, void *, hipStream_t stream) {
+hx_status launch_matmul_i8(const MatmulArgs &args, void *ws, hipStream_t stream) {
     if (args.m == 0 || args.n == 0) return HX_OK;
-    return args.dtype == HX_DTYPE_F32 ? launch<float>(args, stream) : launch<bf16>(args, stream);
+    return args.dtype == HX_DTYPE_F32 ? launch<float>(args, ws, stream) : launch<bf16>(args, ws, stream);
 }
 
 } // namespace hx
