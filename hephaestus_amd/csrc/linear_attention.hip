@@ -176,62 +176,175 @@ __device__ __forceinline__ void split(f32x4v v, bf16x4 (&to)[3]) {
 }
 __device__ __forceinline__ void split(f32x4v v, f32x4v (&to)[1]) { to[0] = v; }
 
-// Eight neighbours of a row in LDS as the two halves of a run of 32 terms.
-__device__ __forceinline__ void load_terms(const bf16 *p, bf16x4 (&f)[2]) {
-    const bf16x8 v = *(const bf16x8 *)p;
+// Whether an element is an infinity or no number: an exponent of ones, which
+// carries into the sign.
+template <int N> __device__ __forceinline__ bool not_finite(const bf16x4 (&v)[N]) {
+    uint32_t carry = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint2 two = __builtin_bit_cast(uint2, v[n]);
+        carry |= ((two.x & 0x7F807F80u) + 0x00800080u) | ((two.y & 0x7F807F80u) + 0x00800080u);
+    }
+    return (carry & 0x80008000u) != 0;
+}
+template <int N> __device__ __forceinline__ bool not_finite(const f32x4v (&v)[N]) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += v[n][e] * 0.0f;
+    return !(sum == 0.0f);
+}
+
+// A tile in LDS: rows of WIDTH elements (a power of two) as 16-byte slots.  Slot
+// c of row r lies at place c ^ turned(r), which puts on different banks both
+// what sixteen rows hold at one c and what rows 4·n..4·n+3 hold at c..c+3.
+template <typename T, int WIDTH> struct TileOf {
+    static constexpr int V = 16 / (int)sizeof(T), kSlots = WIDTH / V, kRow = WIDTH * (int)sizeof(T);
+    static_assert(kSlots >= 8 && (kSlots & (kSlots - 1)) == 0);
+    static __device__ __forceinline__ uint32_t turned(uint32_t row) {
+        if constexpr (kSlots == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3); // two rows share a line of banks
+        else return (row & 3) << 2 | (row >> 2 & 3);
+    }
+    static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t slot) { // bytes
+        return row * kRow + (slot ^ turned(row)) * 16;
+    }
+};
+
+// Terms 32·i + 8·(l / 16) on, eight neighbours of row l % 16 of the sixteen from
+// row `first` on, as the two halves of an operand.
+template <int WIDTH>
+__device__ __forceinline__ void load_terms(const char *tile, int first, int i, bf16x4 (&f)[2]) {
+    const int l = lane_id();
+    const bf16x8 v = *(const bf16x8 *)(tile + first * TileOf<bf16, WIDTH>::kRow +
+                                       TileOf<bf16, WIDTH>::place(l % 16, i * 4 + l / 16));
     f[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
     f[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
 }
-__device__ __forceinline__ void load_terms(const float *p, f32x4v (&f)[2]) {
-    f[0] = *(const f32x4v *)p;
-    f[1] = *(const f32x4v *)(p + 4);
-}
-// Four terms down a column: rows 4·(l / 16) + i of `tile`, and of its columns
-// the (l % 4)-th of the four that begin at `step`·(l % 16 / 4).
-__device__ __forceinline__ bf16x4 load_column(const bf16 *tile, int pitch, int step) {
-    // The transposing read: lane l names row 4·(l / 16) + l % 16 / 4 and four
-    // columns of it, and receives one column of its sixteen lanes' rows.
-    const int l = lane_id(), row = l / 16 * 4 + l % 16 / 4;
-    return __builtin_bit_cast(bf16x4,
-                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + row * pitch + l % 4 * step)));
-}
-__device__ __forceinline__ f32x4v load_column(const float *tile, int pitch, int step) {
+template <int WIDTH>
+__device__ __forceinline__ void load_terms(const char *tile, int first, int i, f32x4v (&f)[2]) {
     const int l = lane_id();
-    const float *p = tile + l / 16 * 4 * pitch + l % 16 / 4 * step + l % 4;
-    return f32x4v{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
+    const char *rows = tile + first * TileOf<float, WIDTH>::kRow;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+        f[n] = *(const f32x4v *)(rows + TileOf<float, WIDTH>::place(l % 16, i * 8 + l / 16 * 2 + n));
 }
 
-// One chunk of a head's rows on its way from memory to LDS: N vectors of 16
-// bytes a thread.  Rows from `rows` on and columns from `width` on are zeros.
-template <typename T, int ROWS, int COLS, int THREADS> struct Staged {
-    static constexpr int V = Pack16<T>::N, kRow = COLS / V, N = (ROWS * kRow + THREADS - 1) / THREADS;
+// Terms down columns: rows 4·(l / 16) + i of each of the BLOCKS sixteens of a
+// tile's rows, and of the columns the (l % 4)-th of the four that begin at
+// `column` + STEP·(l % 16 / 4).  With PAIR also the same four columns on.
+//
+// The transposing read: lane l names row 4·(l / 16) + l % 16 / 4 and four columns
+// of it, and receives one column of its sixteen lanes' rows.  It is written
+// out, with its wait, because the compiler puts a wait for all loads that write
+// LDS in front of the builtin, those of later chunks among them.
+template <int WIDTH, int STEP, int BLOCKS, bool PAIR>
+__device__ __forceinline__ void load_columns(const char *tile, int column, bf16x4 (&to)[BLOCKS * (PAIR ? 2 : 1)]) {
+    static_assert(BLOCKS == 4);
+    constexpr int kStep = 16 * TileOf<bf16, WIDTH>::kRow;
+    const int l = lane_id(), row = l / 16 * 4 + l % 16 / 4, c = column + l % 4 * STEP;
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)tile +
+                        TileOf<bf16, WIDTH>::place(row, c / 8) + c % 8 * 2;
+    if constexpr (PAIR)
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
+                     "ds_read_b64_tr_b16 %2, %8 offset:%10\n\tds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
+                     "ds_read_b64_tr_b16 %4, %8 offset:8\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %6, %8 offset:%13\n\tds_read_b64_tr_b16 %7, %8 offset:%14\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3]), "=&v"(to[4]), "=&v"(to[5]),
+                       "=&v"(to[6]), "=&v"(to[7])
+                     : "v"(at), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep), "i"(kStep + 8), "i"(2 * kStep + 8),
+                       "i"(3 * kStep + 8));
+    else
+        asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%5\n\t"
+                     "ds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %4 offset:%7\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3])
+                     : "v"(at), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep));
+}
+template <int WIDTH, int STEP, int BLOCKS, bool PAIR>
+__device__ __forceinline__ void load_columns(const char *tile, int column, f32x4v (&to)[BLOCKS * (PAIR ? 2 : 1)]) {
+    const int l = lane_id();
+#pragma unroll
+    for (int n = 0; n < BLOCKS * (PAIR ? 2 : 1); ++n) {
+        const char *rows = tile + n % BLOCKS * 16 * TileOf<float, WIDTH>::kRow;
+        const int at = column + n / BLOCKS * 4 + l % 16 / 4 * STEP + l % 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            to[n][e] = *(const float *)(rows + TileOf<float, WIDTH>::place(l / 16 * 4 + e, at / 4) + at % 4 * 4);
+    }
+}
+
+// ROWS rows of a head on their way from memory to a tile, by all threads of the
+// block.  Rows from `rows` on and columns from `width` on become zeros.
+//
+// DIRECT: loads that write LDS without registers, for rows that begin on dwords
+// and are whole 16-byte slots.  Every lane loads every time, so that a count of
+// loads under way says which have landed: lanes outside the rows load zeros.
+// Otherwise through registers.
+__device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+template <typename T, int ROWS, int WIDTH, int THREADS, bool DIRECT> struct Stager {
+    using Tile = TileOf<T, WIDTH>;
+    static constexpr int V = Tile::V, N = ROWS * Tile::kSlots / THREADS;
+    static_assert(N * THREADS == ROWS * Tile::kSlots);
     typedef typename std::conditional<sizeof(T) == 2, u32x4_a2, u32x4_a4>::type Vec;
-    u32x4 held[N];
-    __device__ __forceinline__ void load(const T *base, int64_t stride, uint32_t rows, uint32_t width) {
+    uint32_t offset[DIRECT ? N : 1]; // bytes from a chunk's first row
+    u32x4 held[DIRECT ? 1 : N];
+
+    // Thread t of a step fills place t % kSlots of row t / kSlots.
+    static __device__ __forceinline__ uint32_t row_of(int i) { return (threadIdx.x + i * THREADS) / Tile::kSlots; }
+    static __device__ __forceinline__ uint32_t slot_of(int i) {
+        return threadIdx.x % Tile::kSlots ^ Tile::turned(row_of(i));
+    }
+    __device__ __forceinline__ void begin(int64_t stride) {
+        if constexpr (DIRECT)
+#pragma unroll
+            for (int i = 0; i < N; ++i) offset[i] = (row_of(i) * (uint32_t)stride + slot_of(i) * V) * (uint32_t)sizeof(T);
+    }
+    __device__ __forceinline__ void load(const T *base, int64_t stride, uint32_t rows, uint32_t width, char *tile) {
+        if constexpr (DIRECT) {
+            char *wave = tile + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
+            const bool whole = rows >= ROWS && width == WIDTH;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const char *p = (const char *)base + offset[i];
+                if (!whole && !(row_of(i) < rows && slot_of(i) * V < width)) p = (const char *)kZeros;
+                __builtin_amdgcn_global_load_lds(
+                    (const void *)p, (__attribute__((address_space(3))) void *)(wave + i * THREADS * 16), 16, 0, 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t at = threadIdx.x + i * THREADS, row = at / kRow, col = at % kRow * V;
-            const T *p = base + (int64_t)row * stride + col;
-            held[i] = u32x4{0, 0, 0, 0};
-            if (row < rows && col + V <= width) {
-                held[i] = *(const Vec *)p;
-            } else if (row < rows) {
-                T part[V];
+            const uint32_t row = row_of(i), c = slot_of(i) * V;
+            const T *p = base + (int64_t)row * stride + c;
+            if constexpr (!DIRECT) {
+                held[i] = u32x4{0, 0, 0, 0};
+                if (row < rows && c + V <= width) {
+                    held[i] = *(const Vec *)p;
+                } else if (row < rows) {
+                    T part[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) part[e] = col + e < width ? p[e] : (T)0.0f;
-                __builtin_memcpy(&held[i], part, 16);
+                    for (int e = 0; e < V; ++e) part[e] = c + e < width ? p[e] : (T)0.0f;
+                    __builtin_memcpy(&held[i], part, 16);
+                }
             }
         }
     }
-    __device__ __forceinline__ void store(T *tile, int pitch) const {
+    __device__ __forceinline__ void store(char *tile) const {
+        if constexpr (!DIRECT)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t at = threadIdx.x + i * THREADS;
-            if (N * THREADS == ROWS * kRow || at < ROWS * kRow)
-                *(u32x4 *)(tile + at / kRow * pitch + at % kRow * V) = held[i];
-        }
+            for (int i = 0; i < N; ++i) *(u32x4 *)(tile + (threadIdx.x + i * THREADS) * 16) = held[i];
     }
 };
+
+// All of the wave's LDS reads and writes and all but its last N transfers of
+// memory have ended when it passes.
+template <int N> __device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
+__device__ __forceinline__ void meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A prompt cut into `parts` of `span` tokens each, a multiple of the chunk.
 struct Parts {
@@ -239,24 +352,28 @@ struct Parts {
     float *states; // [batch, heads, parts, dk, dv]: each part's own sum, then the state before it
 };
 
-template <typename T, int DK, int NW> struct Chunk {
-    static constexpr int C = sizeof(T) == 2 ? 64 : 32, B = C / 16, kThreads = NW * kWave, DV = NW * 16;
-    static constexpr int kPad = 16 / sizeof(T); // rows 16 bytes off each other's banks
-    static constexpr int kPitch = DK + kPad, kPitchV = DV + kPad;
-    static constexpr int kTiles = B * (B + 1) / 2; // of P, on and below the diagonal
-    static constexpr int kLds = (2 * C * kPitch + C * kPitchV + kTiles * 4 * kWave) * (int)sizeof(T);
+template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT> struct Chunk {
+    static constexpr int C = sizeof(T) == 2 ? 64 : 32, B = C / 16, // tokens, and sixteens of them
+                          kThreads = NW * kWave, DV = NW * 16;
+    static constexpr int WK = DK <= 64 ? 64 : DK <= 128 ? 128 : 256; // rows of q and k in LDS
+    static constexpr int kTileK = C * WK * (int)sizeof(T), kTileV = C * DV * (int)sizeof(T);
+    static constexpr int kStage = (OUTPUTS ? 2 : 1) * kTileK + kTileV;
+    static constexpr int kScores = OUTPUTS ? B * (B + 1) / 2 * 4 * kWave * (int)sizeof(T) : 0; // P, on and below the diagonal
+    // Chunks in LDS: one read, the others on their way.
+    static constexpr int S = DIRECT && 3 * kStage + kScores <= 160 * 1024 ? 3 : 2;
+    static constexpr int kLds = S * kStage + kScores;
+    static_assert(kLds <= 160 * 1024);
 };
 
 // OUTPUTS: the outputs of a part, from the state before it.  Otherwise only the
 // part's own sum, from nothing.
-template <typename T, int DK, int NW, bool OUTPUTS>
+template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT>
 __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArgs a, Parts parts) {
-    using G = Chunk<T, DK, NW>;
+    using G = Chunk<T, DK, NW, OUTPUTS, DIRECT>;
     using F = typename Fragment<T>::type;
-    constexpr int C = G::C, B = G::B, kPitch = G::kPitch, kPitchV = G::kPitchV;
+    constexpr int C = G::C, B = G::B, S = G::S, WK = G::WK, DV = G::DV;
     extern __shared__ __align__(16) char lds[];
-    T *ks = (T *)lds, *vs = ks + C * kPitch, *qs = vs + C * kPitchV;
-    F *ps = (F *)(qs + C * kPitch);
+    F *ps = (F *)(lds + S * G::kStage);
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane % 16, quad = lane / 16;
     const uint32_t part = blockIdx.x % parts.parts, block = blockIdx.x / parts.parts;
@@ -271,7 +388,7 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
     const uint32_t vcol = wave * 16 + col; // this lane's column of v and of the state
 
     // The decay as a power of two a token; minus infinity would make 0·log a NaN.
-    const float log2_decay = fmaxf(a.log_decay[h] * 1.44269504f, -1e30f);
+    const float log_decay = a.log_decay[h], log2_decay = fmaxf(log_decay * 1.44269504f, -1e30f);
     const auto power = [&](int n) { return __builtin_amdgcn_exp2f(log2_decay * (float)n); };
 
     // Row r of accumulator 2·i + j is dk 32·i + 8·(r / 4) + 4·j + r % 4: two
@@ -289,94 +406,161 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (from && state_row(i, e) < dk) s[i][e] = from[state_row(i, e) * stride];
+        // Here, or the compiler waits in every chunk, and for all its loads.
+        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
     }
 
-    Staged<T, C, DK, G::kThreads> next_q, next_k;
-    Staged<T, C, G::DV, G::kThreads> next_v;
-    const auto fetch = [&](uint32_t t0) {
-        const uint32_t rows = end - t0;
-        next_k.load(k + (int64_t)t0 * a.sk.token, a.sk.token, rows, dk);
-        next_v.load(v + (int64_t)t0 * a.sv.token, a.sv.token, rows, dv);
-        if constexpr (OUTPUTS) next_q.load(q + (int64_t)t0 * a.sq.token, a.sq.token, rows, dk);
+    // The decay over a chunk is rounded to a float; what that leaves out of the
+    // state is made good every kSettle chunks, so that the state keeps the
+    // precision of f32 however many there are.
+    constexpr uint32_t kSettle = 8;
+    float high, drift; // drift: the rounding's relative error
+    const auto decay_over = [&](int rows) {
+        const double d = exp((double)log_decay * rows);
+        high = (float)d;
+        drift = high > 0.0f ? (float)((d - high) / high) : 0.0f;
     };
-    if (begin < end) fetch(begin);
-    for (uint32_t t0 = begin; t0 < end; t0 += C) {
+    decay_over(C);
+    const auto make_good = [&](uint32_t chunks) {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][e] = fmaf(s[i][e], drift * (float)chunks, s[i][e]);
+    };
+    // Powers of the decay: over 16 tokens; in a whole chunk's last 16 rows, the
+    // weight of a row in the state; at a token of the first 16, of the state.
+    const float over16 = power(16), query_weight = power(col + 1) * a.scale;
+    f32x4v last_weight;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) last_weight[e] = power(15 - quad * 4 - e);
+
+    Stager<T, C, WK, G::kThreads, DIRECT> to_q, to_k;
+    Stager<T, C, DV, G::kThreads, DIRECT> to_v;
+    to_k.begin(a.sk.token);
+    to_v.begin(a.sv.token);
+    if constexpr (OUTPUTS) to_q.begin(a.sq.token);
+    constexpr int kLoads = to_k.N + to_v.N + (OUTPUTS ? to_q.N : 0); // instructions a chunk
+    const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;
+    const auto stage_of = [&](uint32_t n) { return lds + n % S * G::kStage; };
+    const auto fetch = [&](uint32_t n) {
+        const uint32_t t0 = begin + n * C, rows = end - t0;
+        char *stage = stage_of(n);
+        to_k.load(k + (int64_t)t0 * a.sk.token, a.sk.token, rows, dk, stage);
+        to_v.load(v + (int64_t)t0 * a.sv.token, a.sv.token, rows, dv, stage + G::kTileK);
+        if constexpr (OUTPUTS)
+            to_q.load(q + (int64_t)t0 * a.sq.token, a.sq.token, rows, dk, stage + G::kTileK + G::kTileV);
+    };
+    const auto settle = [&](uint32_t n) { // what went through registers
+        char *stage = stage_of(n);
+        to_k.store(stage);
+        to_v.store(stage + G::kTileK);
+        if constexpr (OUTPUTS) to_q.store(stage + G::kTileK + G::kTileV);
+    };
+    if constexpr (DIRECT) {
+        for (uint32_t n = 0; n < S - 1 && n < chunks; ++n) fetch(n);
+    } else if (chunks) {
+        fetch(0);
+        settle(0);
+    }
+    for (uint32_t n = 0; n < chunks; ++n) {
+        const uint32_t t0 = begin + n * C;
         const int rows = (int)min((uint32_t)C, end - t0);
-        __syncthreads(); // the last chunk has been read
-        next_k.store(ks, kPitch);
-        next_v.store(vs, kPitchV);
-        if constexpr (OUTPUTS) next_q.store(qs, kPitch);
-        __syncthreads();
-        if (t0 + C < end) fetch(t0 + C);
+        // Chunk n has landed once no more is under way than the chunks after it.
+        if (DIRECT && n + S - 2 < chunks) meet<(S - 2) * kLoads>();
+        else meet<0>();
+        const uint32_t ahead = DIRECT ? S - 1 : 1;
+        if (n + ahead < chunks) fetch(n + ahead);
+        const char *ks = stage_of(n), *vs = ks + G::kTileK, *qs = vs + G::kTileV;
 
         F vf[B]; // this lane's column of v
-#pragma unroll
-        for (int i = 0; i < B; ++i) vf[i] = load_column(vs + i * 16 * kPitchV + wave * 16, kPitchV, 4);
+        load_columns<DV, 4, B, false>(vs, wave * 16, vf);
 
         if constexpr (OUTPUTS) {
             // Pᵀ tiles (x: rows of k, y: rows of q), the waves in turn.
-            int tile = 0;
-#pragma unroll
-            for (int y = 0; y < B; ++y)
-#pragma unroll
-                for (int x = 0; x <= y; ++x, ++tile) {
-                    if (tile % NW != wave) continue;
-                    f32x4v p = {};
-#pragma unroll
-                    for (int i = 0; i < DK / 32; ++i) {
-                        F fk[2], fq[2];
-                        load_terms(ks + (x * 16 + col) * kPitch + i * 32 + quad * 8, fk);
-                        load_terms(qs + (y * 16 + col) * kPitch + i * 32 + quad * 8, fq);
-                        p = mma(fk, fq, p);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int far = (y * 16 + col) - (x * 16 + quad * 4 + e);
-                        p[e] = far >= 0 ? p[e] * (power(far) * a.scale) : 0.0f;
-                    }
-                    ps[tile * kWave + lane] = rounded(p, T{});
-                }
-            __syncthreads();
-            f32x4v o[B];
-            int first_bad = C; // the first token whose v is no number, in this lane's column
-            for (int again = 0;; ++again) {
-#pragma unroll
-                for (int y = 0; y < B; ++y) o[y] = f32x4v{};
+#pragma unroll 1
+            for (int tile = wave; tile < B * (B + 1) / 2; tile += NW) {
+                const int y = (tile >= 1) + (tile >= 3) + (tile >= 6), x = tile - y * (y + 1) / 2;
+                f32x4v p = {};
 #pragma unroll
                 for (int i = 0; i < DK / 32; ++i) {
-                    const F fs[2] = {rounded(s[2 * i], T{}), rounded(s[2 * i + 1], T{})};
-#pragma unroll
-                    for (int y = 0; y < B; ++y) {
-                        F fq[2];
-                        load_terms(qs + (y * 16 + col) * kPitch + i * 32 + quad * 8, fq);
-                        o[y] = mma(fs, fq, o[y]);
-                    }
+                    F fk[2], fq[2];
+                    load_terms<WK>(ks, x * 16, i, fk);
+                    load_terms<WK>(qs, y * 16, i, fq);
+                    p = mma(fk, fq, p);
                 }
-                float sick = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int far = (y * 16 + col) - (x * 16 + quad * 4 + e);
+                    p[e] = far >= 0 ? p[e] * (power(far) * a.scale) : 0.0f;
+                }
+                ps[tile * kWave + lane] = rounded(p, T{});
+            }
+        }
+        // The state's part of the outputs, before the state moves on.
+        f32x4v o[B] = {};
+        if constexpr (OUTPUTS) {
+#pragma unroll
+            for (int i = 0; i < DK / 32; ++i) {
+                const F fs[2] = {rounded(s[2 * i], T{}), rounded(s[2 * i + 1], T{})};
 #pragma unroll
                 for (int y = 0; y < B; ++y) {
-                    o[y] *= power(y * 16 + col + 1) * a.scale;
-#pragma unroll
-                    for (int x = 0; x <= y; x += 2) {
-                        const F fv[2] = {vf[x], vf[x + 1]};
-                        F fp[2] = {ps[(y * (y + 1) / 2 + x) * kWave + lane], F{}};
-                        if (x < y) fp[1] = ps[(y * (y + 1) / 2 + x + 1) * kWave + lane];
-                        o[y] = mma(fv, fp, o[y]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sick += o[y][e] * 0.0f;
+                    F fq[2];
+                    load_terms<WK>(qs, y * 16, i, fq);
+                    o[y] = mma(fs, fq, o[y]);
                 }
-                // A value that is no number also spoils the tokens before it,
-                // whose weights are 0: take it out, and put its mark where
-                // it belongs.
-                if (again || !__any(!(sick == 0.0f))) break;
+            }
+            float weight = query_weight;
+#pragma unroll
+            for (int y = 0; y < B; ++y, weight *= over16) o[y] *= weight;
+        }
+
+        // The state: decayed over the chunk, then the chunk's sum.
+        if (rows < C) { // the last one
+            make_good(n % kSettle);
+            decay_over(rows);
+        }
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) s[i] *= high;
+        F terms[B][kTerms<T>];
+        f32x4v weight = last_weight;
+#pragma unroll
+        for (int x = B - 1; x >= 0; --x, weight *= over16) {
+            if (rows < C)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) weight[e] = power(max(rows - 1 - (x * 16 + quad * 4 + e), 0));
+            split(widened(vf[x]) * weight, terms[x]);
+        }
+#pragma unroll
+        for (int i = 0; i < DK / 16; i += 2) {
+            F fk[2 * B];
+            load_columns<WK, 8, B, true>(ks, i * 16, fk);
+#pragma unroll
+            for (int m = kTerms<T> - 1; m >= 0; --m)
+#pragma unroll
+                for (int x = 0; x < B; x += 2) {
+                    const F fv[2] = {terms[x][m], terms[x + 1][m]};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const F f[2] = {fk[j * B + x], fk[j * B + x + 1]};
+                        s[i + j] = mma(f, fv, s[i + j]);
+                    }
+                }
+        }
+        if (rows < C || n % kSettle == kSettle - 1) make_good(rows < C ? 1 : kSettle);
+
+        if constexpr (OUTPUTS) {
+            // A value that is no number would also spoil the tokens before it,
+            // whose weights are 0: it is taken out, and its mark put where it
+            // belongs.
+            int first_bad = C; // the first token of one, in this lane's column
+            if (__any(not_finite(vf))) {
 #pragma unroll
                 for (int x = B - 1; x >= 0; --x) {
                     f32x4v w = widened(vf[x]);
 #pragma unroll
                     for (int e = 3; e >= 0; --e)
                         if (!(w[e] * 0.0f == 0.0f)) {
-                            first_bad = min(first_bad, x * 16 + quad * 4 + e);
+                            first_bad = x * 16 + quad * 4 + e;
                             w[e] = 0.0f;
                         }
                     vf[x] = rounded(w, T{});
@@ -384,6 +568,16 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
                 first_bad = min(first_bad, __shfl_xor(first_bad, 16));
                 first_bad = min(first_bad, __shfl_xor(first_bad, 32));
             }
+            meet_lds(); // P is whole
+#pragma unroll
+            for (int y = 0; y < B; ++y)
+#pragma unroll
+                for (int x = 0; x <= y; x += 2) {
+                    const F fv[2] = {vf[x], vf[x + 1]};
+                    F fp[2] = {ps[(y * (y + 1) / 2 + x) * kWave + lane], F{}};
+                    if (x < y) fp[1] = ps[(y * (y + 1) / 2 + x + 1) * kWave + lane];
+                    o[y] = mma(fv, fp, o[y]);
+                }
             if (__any(first_bad < C)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -392,8 +586,6 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
                     for (int y = 0; y < B; ++y)
                         if (y * 16 + col >= from) o[y][e] = __builtin_nanf("");
                 }
-#pragma unroll
-                for (int i = 0; i < B; ++i) vf[i] = load_column(vs + i * 16 * kPitchV + wave * 16, kPitchV, 4);
             }
             // Four neighbours of a token's row.
             const uint32_t c = wave * 16 + quad * 4;
@@ -412,36 +604,7 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
             }
         }
 
-        // The state: decayed over the chunk, to the last bit of f32 (the power
-        // in two floats), then the chunk's sum.
-        const double decayed = exp((double)a.log_decay[h] * rows);
-        const float high = (float)decayed, low = (float)(decayed - high);
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] = fmaf(s[i][e], high, s[i][e] * low);
-        F terms[B][kTerms<T>];
-#pragma unroll
-        for (int x = 0; x < B; ++x) {
-            f32x4v w = widened(vf[x]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] *= power(max(rows - 1 - (x * 16 + quad * 4 + e), 0));
-            split(w, terms[x]);
-        }
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int x = 0; x < B; x += 2) {
-                F fk[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    fk[j] = load_column(ks + (x + j) * 16 * kPitch + i / 2 * 32 + i % 2 * 4, kPitch, 8);
-#pragma unroll
-                for (int n = kTerms<T> - 1; n >= 0; --n) {
-                    const F fv[2] = {terms[x][n], terms[x + 1][n]};
-                    s[i] = mma(fk, fv, s[i]);
-                }
-            }
+        if (!DIRECT && n + 1 < chunks) settle(n + 1);
     }
 
     if constexpr (OUTPUTS) { // rows past the sequence's end
@@ -481,8 +644,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Pa
     if (a.state_out) a.state_out[b * a.st.batch + h * a.st.head + row * a.st.token + col] = s;
 }
 
-// Columns of v a block: up to 128, in whole waves of 16.
-uint32_t block_waves(const AttentionArgs &a) { return a.dv <= 64 ? 4 : 8; }
+// Waves a block, each with 16 columns of v: with wider keys than 128, two chunks
+// of q, k and 128 columns of v would not fit LDS.
+uint32_t block_waves(const AttentionArgs &a) { return a.dv <= 64 || a.dk > 128 ? 4 : 8; }
 
 constexpr uint64_t kStepTokens = 8; // up to here the recurrence
 constexpr uint64_t kFullCard = 256; // blocks
@@ -496,42 +660,58 @@ Parts parts_of(const AttentionArgs &a) {
     return Parts{(uint32_t)ceil_div(a.tokens, span), (uint32_t)span, nullptr};
 }
 
-template <typename T, int DK, int NW> hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    using G = Chunk<T, DK, NW>;
-    const auto run = [&](auto kernel, const Parts &parts) {
+template <typename T, int DK, int NW, bool DIRECT>
+hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
+    Parts parts = parts_of(a);
+    parts.states = (float *)ws;
+    const auto run = [&](auto outputs) {
+        using G = Chunk<T, DK, NW, decltype(outputs)::value, DIRECT>;
+        const auto kernel = attention_chunk_kernel<T, DK, NW, decltype(outputs)::value, DIRECT>;
         if constexpr (G::kLds > 65536) {
-            const hipError_t err =
+            static const hipError_t allowed =
                 hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-            if (err != hipSuccess) return hip_fail(HX_ERR_DISPATCH_FAILED, err, "attention LDS size");
+            if (allowed != hipSuccess) return hip_fail(HX_ERR_DISPATCH_FAILED, allowed, "attention LDS size");
         }
         const uint64_t x = ceil_div(a.dv, G::DV) * parts.parts;
         hipLaunchKernelGGL(kernel, dim3((uint32_t)x, (uint32_t)a.heads, (uint32_t)a.batch), dim3(G::kThreads), G::kLds,
                            stream, a, parts);
         return check_launch("attention_chunk_kernel");
     };
-    Parts parts = parts_of(a);
-    parts.states = (float *)ws;
     if (parts.parts > 1) {
-        HX_TRY(run(attention_chunk_kernel<T, DK, NW, false>, parts));
+        HX_TRY(run(std::false_type{}));
         hipLaunchKernelGGL(attention_join_kernel,
                            dim3((uint32_t)ceil_div(a.dk * a.dv, 256), (uint32_t)a.heads, (uint32_t)a.batch), dim3(256),
                            0, stream, a, parts);
         HX_TRY(check_launch("attention_join_kernel"));
     }
-    return run(attention_chunk_kernel<T, DK, NW, true>, parts);
+    return run(std::true_type{});
 }
 
-template <typename T, int NW> hx_status launch_width(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    if (a.dk <= 64) return launch_chunks<T, 64, NW>(a, ws, stream);
-    if (a.dk <= 128) return launch_chunks<T, 128, NW>(a, ws, stream);
-    return launch_chunks<T, 256, NW>(a, ws, stream);
+// Whether the rows of a chunk can be loaded without registers (Stager).
+template <typename T> bool direct_rows(const void *base, const AttentionView &s, uint64_t width) {
+    const uint64_t bits = (uintptr_t)base | (uint64_t)(s.token | s.head | s.batch) * sizeof(T);
+    return bits % 4 == 0 && width % (16 / sizeof(T)) == 0 && s.token >= 0 && s.token < 1 << 24;
+}
+
+template <typename T, int NW, bool DIRECT> hx_status launch_width(const AttentionArgs &a, void *ws, hipStream_t stream) {
+    if (a.dk <= 64) return launch_chunks<T, 64, NW, DIRECT>(a, ws, stream);
+    if (a.dk <= 96) return launch_chunks<T, 96, NW, DIRECT>(a, ws, stream);
+    if (a.dk <= 128) return launch_chunks<T, 128, NW, DIRECT>(a, ws, stream);
+    if constexpr (NW == 4) return launch_chunks<T, 256, NW, DIRECT>(a, ws, stream);
+    return fail(HX_ERR_DISPATCH_FAILED, "no attention block for keys of width %llu", (unsigned long long)a.dk);
+}
+template <typename T, bool DIRECT> hx_status launch_chunked(const AttentionArgs &a, void *ws, hipStream_t stream) {
+    return block_waves(a) == 4 ? launch_width<T, 4, DIRECT>(a, ws, stream) : launch_width<T, 8, DIRECT>(a, ws, stream);
 }
 
 bool by_chunks(const AttentionArgs &a) { return a.tokens > kStepTokens && a.dk > 0; }
 
 template <typename T> hx_status launch(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    if (by_chunks(a))
-        return block_waves(a) == 4 ? launch_width<T, 4>(a, ws, stream) : launch_width<T, 8>(a, ws, stream);
+    if (by_chunks(a)) {
+        const bool direct = direct_rows<T>(a.q, a.sq, a.dk) && direct_rows<T>(a.k, a.sk, a.dk) &&
+                            direct_rows<T>(a.v, a.sv, a.dv);
+        return direct ? launch_chunked<T, true>(a, ws, stream) : launch_chunked<T, false>(a, ws, stream);
+    }
     if (a.dk <= 32) return launch_step<T, 1>(a, stream);
     if (a.dk <= 64) return launch_step<T, 2>(a, stream);
     if (a.dk <= 128) return launch_step<T, 4>(a, stream);
