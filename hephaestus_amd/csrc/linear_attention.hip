@@ -176,6 +176,14 @@ __device__ __forceinline__ void split(f32x4v v, bf16x4 (&to)[3]) {
 }
 __device__ __forceinline__ void split(f32x4v v, f32x4v (&to)[1]) { to[0] = v; }
 
+// The same value, which the compiler cannot know: what is computed from it stays
+// where it is written, in a branch that is seldom taken, and takes up no
+// registers outside.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // Whether an element is an infinity or no number: an exponent of ones, which
 // carries into the sign.
 template <int N> __device__ __forceinline__ bool not_finite(const bf16x4 (&v)[N]) {
@@ -293,31 +301,38 @@ template <typename T, int ROWS, int WIDTH, int THREADS, bool DIRECT> struct Stag
     u32x4 held[DIRECT ? 1 : N];
 
     // Thread t of a step fills place t % kSlots of row t / kSlots.
-    static __device__ __forceinline__ uint32_t row_of(int i) { return (threadIdx.x + i * THREADS) / Tile::kSlots; }
-    static __device__ __forceinline__ uint32_t slot_of(int i) {
-        return threadIdx.x % Tile::kSlots ^ Tile::turned(row_of(i));
+    static __device__ __forceinline__ uint32_t row_of(uint32_t t, int i) { return (t + i * THREADS) / Tile::kSlots; }
+    static __device__ __forceinline__ uint32_t slot_of(uint32_t t, int i) {
+        return t % Tile::kSlots ^ Tile::turned(row_of(t, i));
     }
     __device__ __forceinline__ void begin(int64_t stride) {
         if constexpr (DIRECT)
 #pragma unroll
-            for (int i = 0; i < N; ++i) offset[i] = (row_of(i) * (uint32_t)stride + slot_of(i) * V) * (uint32_t)sizeof(T);
+            for (int i = 0; i < N; ++i)
+                offset[i] = (row_of(threadIdx.x, i) * (uint32_t)stride + slot_of(threadIdx.x, i) * V) * (uint32_t)sizeof(T);
     }
     __device__ __forceinline__ void load(const T *base, int64_t stride, uint32_t rows, uint32_t width, char *tile) {
         if constexpr (DIRECT) {
             char *wave = tile + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
-            const bool whole = rows >= ROWS && width == WIDTH;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const char *p = (const char *)base + offset[i];
-                if (!whole && !(row_of(i) < rows && slot_of(i) * V < width)) p = (const char *)kZeros;
+            const auto put = [&](int i, const void *p) {
                 __builtin_amdgcn_global_load_lds(
-                    (const void *)p, (__attribute__((address_space(3))) void *)(wave + i * THREADS * 16), 16, 0, 0);
+                    p, (__attribute__((address_space(3))) void *)(wave + i * THREADS * 16), 16, 0, 0);
+            };
+            if (rows >= ROWS && width == WIDTH) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) put(i, (const char *)base + offset[i]);
+            } else {
+                const uint32_t t = here(threadIdx.x);
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    put(i, row_of(t, i) < rows && slot_of(t, i) * V < width ? (const char *)base + offset[i]
+                                                                          : (const char *)kZeros);
             }
             return;
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t row = row_of(i), c = slot_of(i) * V;
+            const uint32_t row = row_of(threadIdx.x, i), c = slot_of(threadIdx.x, i) * V;
             const T *p = base + (int64_t)row * stride + c;
             if constexpr (!DIRECT) {
                 held[i] = u32x4{0, 0, 0, 0};
@@ -414,18 +429,22 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
     // state is made good every kSettle chunks, so that the state keeps the
     // precision of f32 however many there are.
     constexpr uint32_t kSettle = 8;
-    float high, drift; // drift: the rounding's relative error
-    const auto decay_over = [&](int rows) {
-        const double d = exp((double)log_decay * rows);
-        high = (float)d;
-        drift = high > 0.0f ? (float)((d - high) / high) : 0.0f;
+    struct Decay {
+        float by, drift; // the factor, and its rounding's relative error
     };
-    decay_over(C);
+    const auto decay_over = [&](uint32_t rows) {
+        const double d = exp((double)log_decay * rows);
+        const float by = (float)d;
+        return Decay{by, by > 0.0f ? (float)((d - by) / by) : 0.0f};
+    };
+    const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;
+    Decay decay = decay_over(C);
+    const Decay last_decay = decay_over(chunks ? end - begin - (chunks - 1) * C : 1);
     const auto make_good = [&](uint32_t chunks) {
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] = fmaf(s[i][e], drift * (float)chunks, s[i][e]);
+            for (int e = 0; e < 4; ++e) s[i][e] = fmaf(s[i][e], decay.drift * (float)chunks, s[i][e]);
     };
     // Powers of the decay: over 16 tokens; in a whole chunk's last 16 rows, the
     // weight of a row in the state; at a token of the first 16, of the state.
@@ -440,7 +459,6 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
     to_v.begin(a.sv.token);
     if constexpr (OUTPUTS) to_q.begin(a.sq.token);
     constexpr int kLoads = to_k.N + to_v.N + (OUTPUTS ? to_q.N : 0); // instructions a chunk
-    const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;
     const auto stage_of = [&](uint32_t n) { return lds + n % S * G::kStage; };
     const auto fetch = [&](uint32_t n) {
         const uint32_t t0 = begin + n * C, rows = end - t0;
@@ -475,7 +493,8 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
         F vf[B]; // this lane's column of v
         load_columns<DV, 4, B, false>(vs, wave * 16, vf);
 
-        if constexpr (OUTPUTS) {
+        f32x4v o[B] = {};
+        const auto outputs = [&] {
             // Pᵀ tiles (x: rows of k, y: rows of q), the waves in turn.
 #pragma unroll 1
             for (int tile = wave; tile < B * (B + 1) / 2; tile += NW) {
@@ -495,58 +514,60 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
                 }
                 ps[tile * kWave + lane] = rounded(p, T{});
             }
-        }
-        // The state's part of the outputs, before the state moves on.
-        f32x4v o[B] = {};
-        if constexpr (OUTPUTS) {
+            // The state's part of the outputs.
 #pragma unroll
             for (int i = 0; i < DK / 32; ++i) {
-                const F fs[2] = {rounded(s[2 * i], T{}), rounded(s[2 * i + 1], T{})};
+                const F state[2] = {rounded(s[2 * i], T{}), rounded(s[2 * i + 1], T{})};
 #pragma unroll
                 for (int y = 0; y < B; ++y) {
                     F fq[2];
                     load_terms<WK>(qs, y * 16, i, fq);
-                    o[y] = mma(fs, fq, o[y]);
+                    o[y] = mma(state, fq, o[y]);
                 }
             }
             float weight = query_weight;
 #pragma unroll
             for (int y = 0; y < B; ++y, weight *= over16) o[y] *= weight;
-        }
-
-        // The state: decayed over the chunk, then the chunk's sum.
-        if (rows < C) { // the last one
-            make_good(n % kSettle);
-            decay_over(rows);
-        }
+        };
+        const auto advance = [&] {
+            // The state: decayed over the chunk, then the chunk's sum.
+            if (rows < C) { // the last one
+                make_good(n % kSettle);
+                decay = last_decay;
+            }
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i) s[i] *= high;
-        F terms[B][kTerms<T>];
-        f32x4v weight = last_weight;
+            for (int i = 0; i < DK / 16; ++i) s[i] *= decay.by;
+            F terms[B][kTerms<T>];
+            f32x4v weight = last_weight;
 #pragma unroll
-        for (int x = B - 1; x >= 0; --x, weight *= over16) {
-            if (rows < C)
+            for (int x = B - 1; x >= 0; --x, weight *= over16) {
+                if (rows < C) {
+                    const int left = rows - 1 - x * 16 - (int)here(quad * 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) weight[e] = power(max(rows - 1 - (x * 16 + quad * 4 + e), 0));
-            split(widened(vf[x]) * weight, terms[x]);
-        }
-#pragma unroll
-        for (int i = 0; i < DK / 16; i += 2) {
-            F fk[2 * B];
-            load_columns<WK, 8, B, true>(ks, i * 16, fk);
-#pragma unroll
-            for (int m = kTerms<T> - 1; m >= 0; --m)
-#pragma unroll
-                for (int x = 0; x < B; x += 2) {
-                    const F fv[2] = {terms[x][m], terms[x + 1][m]};
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const F f[2] = {fk[j * B + x], fk[j * B + x + 1]};
-                        s[i + j] = mma(f, fv, s[i + j]);
-                    }
+                    for (int e = 0; e < 4; ++e) weight[e] = power(max(left - e, 0));
                 }
-        }
-        if (rows < C || n % kSettle == kSettle - 1) make_good(rows < C ? 1 : kSettle);
+                split(widened(vf[x]) * weight, terms[x]);
+            }
+#pragma unroll
+            for (int i = 0; i < DK / 16; i += 2) {
+                F fk[2 * B];
+                load_columns<WK, 8, B, true>(ks, i * 16, fk);
+#pragma unroll
+                for (int m = kTerms<T> - 1; m >= 0; --m)
+#pragma unroll
+                    for (int x = 0; x < B; x += 2) {
+                        const F fv[2] = {terms[x][m], terms[x + 1][m]};
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const F f[2] = {fk[j * B + x], fk[j * B + x + 1]};
+                            s[i + j] = mma(f, fv, s[i + j]);
+                        }
+                    }
+            }
+            if (rows < C || n % kSettle == kSettle - 1) make_good(rows < C ? 1 : kSettle);
+        };
+        if constexpr (OUTPUTS) outputs();
+        advance();
 
         if constexpr (OUTPUTS) {
             // A value that is no number would also spoil the tokens before it,
@@ -588,19 +609,19 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
                 }
             }
             // Four neighbours of a token's row.
-            const uint32_t c = wave * 16 + quad * 4;
+            T *to = out + (int64_t)(t0 + col) * a.so.token + wave * 16 + quad * 4;
+            if (rows == C && dv >= (wave + 1) * 16u) {
 #pragma unroll
-            for (int y = 0; y < B; ++y) {
-                if (y * 16 + col >= rows) continue;
-                T *to = out + (int64_t)(t0 + y * 16 + col) * a.so.token + c;
-                if (c + 4 <= dv) {
+                for (int y = 0; y < B; ++y, to += 16 * a.so.token) {
                     const F r = rounded(o[y], T{});
                     __builtin_memcpy(to, &r, sizeof(r));
-                } else {
+                }
+            } else {
+                const uint32_t c = wave * 16 + here(quad * 4);
+                for (int y = 0; y < B; ++y, to += 16 * a.so.token)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (c + e < dv) to[e] = (T)o[y][e];
-                }
+                        if (y * 16 + col < rows && c + e < dv) to[e] = (T)o[y][e];
             }
         }
 
@@ -625,21 +646,32 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
 }
 
 // The state before each part, from the parts' own sums: one element of the
-// state a thread, the parts in order.
+// state a thread, the parts in order, eight of them loaded together.
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Parts parts) {
     const uint32_t n = (uint32_t)(a.dk * a.dv), i = blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const uint32_t h = blockIdx.y, b = blockIdx.z, row = i / (uint32_t)a.dv, col = i % (uint32_t)a.dv;
     const uint32_t tokens = (uint32_t)a.tokens, length = a.lengths ? min(a.lengths[b], tokens) : tokens;
     const double log_decay = a.log_decay[h];
+    // Every part but the last with tokens is whole, and those behind it have none.
+    const uint32_t whole = length / parts.span, rest = length % parts.span;
+    const double of_whole = exp(log_decay * parts.span), of_rest = rest ? exp(log_decay * rest) : 1.0;
+    const float whole_high = (float)of_whole, whole_low = (float)(of_whole - whole_high);
+    const float rest_high = (float)of_rest, rest_low = (float)(of_rest - rest_high);
     float s = a.state_in ? a.state_in[b * a.si.batch + h * a.si.head + row * a.si.token + col] : 0.0f;
     float *at = parts.states + ((uint64_t)b * a.heads + h) * parts.parts * n + i;
-    for (uint32_t p = 0; p < parts.parts; ++p, at += n) {
-        const int64_t left = (int64_t)length - (int64_t)p * parts.span, count = min(left, (int64_t)parts.span);
-        const double decayed = count > 0 ? exp(log_decay * (double)count) : 1.0; // infinite logs among them
-        const float high = (float)decayed, low = (float)(decayed - high), own = *at;
-        *at = s;
-        s = fmaf(s, high, s * low) + own;
+    constexpr uint32_t kBatch = 8;
+    for (uint32_t p = 0; p < parts.parts; p += kBatch, at += (uint64_t)kBatch * n) {
+        float own[kBatch];
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k) own[k] = p + k < parts.parts ? at[(uint64_t)k * n] : 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k) {
+            if (p + k >= parts.parts) break;
+            at[(uint64_t)k * n] = s;
+            if (p + k < whole) s = fmaf(s, whole_high, s * whole_low) + own[k];
+            else if (p + k == whole) s = fmaf(s, rest_high, s * rest_low) + own[k];
+        }
     }
     if (a.state_out) a.state_out[b * a.st.batch + h * a.st.head + row * a.st.token + col] = s;
 }
