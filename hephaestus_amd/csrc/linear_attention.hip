@@ -205,14 +205,18 @@ template <int N> __device__ __forceinline__ bool not_finite(const f32x4v (&v)[N]
 }
 
 // A tile in LDS: rows of WIDTH elements (a power of two) as 16-byte slots.  Slot
-// c of row r lies at place c ^ turned(r), which puts on different banks both
-// what sixteen rows hold at one c and what rows 4·n..4·n+3 hold at c..c+3.
-template <typename T, int WIDTH> struct TileOf {
+// c of row r lies at place c ^ turned(r), so that what is read at once lies on
+// different banks: sixteen rows at one slot, and of bf16 tiles that are read
+// down columns too, of rows 4·q..4·q + 3 the halves of four slots.  Cycles of a
+// wave's instruction with eight waves reading: 16 bytes a lane 6.7 (ROWS, row & 15)
+// and 8.2 (else), down columns 8.1 and 6.5; without turning 32 and 16.
+template <typename T, int WIDTH, bool ROWS> struct TileOf {
     static constexpr int V = 16 / (int)sizeof(T), kSlots = WIDTH / V, kRow = WIDTH * (int)sizeof(T);
     static_assert(kSlots >= 8 && (kSlots & (kSlots - 1)) == 0);
     static __device__ __forceinline__ uint32_t turned(uint32_t row) {
-        if constexpr (kSlots == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3); // two rows share a line of banks
-        else return (row & 3) << 2 | (row >> 2 & 3);
+        if constexpr (kSlots == 8) return (row & 1) << 2 | (row >> 2 & 1) << 1 | (row >> 1 & 1);
+        if constexpr (ROWS || sizeof(T) == 4) return row & 15;
+        return (row & 3) << 2 | (row >> 2 & 3);
     }
     static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t slot) { // bytes
         return row * kRow + (slot ^ turned(row)) * 16;
@@ -221,65 +225,106 @@ template <typename T, int WIDTH> struct TileOf {
 
 // Terms 32·i + 8·(l / 16) on, eight neighbours of row l % 16 of the sixteen from
 // row `first` on, as the two halves of an operand.
-template <int WIDTH>
+template <int WIDTH, bool ROWS>
 __device__ __forceinline__ void load_terms(const char *tile, int first, int i, bf16x4 (&f)[2]) {
+    using Tile = TileOf<bf16, WIDTH, ROWS>;
     const int l = lane_id();
-    const bf16x8 v = *(const bf16x8 *)(tile + first * TileOf<bf16, WIDTH>::kRow +
-                                       TileOf<bf16, WIDTH>::place(l % 16, i * 4 + l / 16));
+    const bf16x8 v = *(const bf16x8 *)(tile + first * Tile::kRow + Tile::place(l % 16, i * 4 + l / 16));
     f[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
     f[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
 }
-template <int WIDTH>
+template <int WIDTH, bool ROWS>
 __device__ __forceinline__ void load_terms(const char *tile, int first, int i, f32x4v (&f)[2]) {
+    using Tile = TileOf<float, WIDTH, ROWS>;
     const int l = lane_id();
-    const char *rows = tile + first * TileOf<float, WIDTH>::kRow;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
-        f[n] = *(const f32x4v *)(rows + TileOf<float, WIDTH>::place(l % 16, i * 8 + l / 16 * 2 + n));
+        f[n] = *(const f32x4v *)(tile + first * Tile::kRow + Tile::place(l % 16, i * 8 + l / 16 * 2 + n));
 }
 
-// Terms down columns: rows 4·(l / 16) + i of each of the BLOCKS sixteens of a
-// tile's rows, and of the columns the (l % 4)-th of the four that begin at
-// `column` + STEP·(l % 16 / 4).  With PAIR also the same four columns on.
+// A state S, [dk, columns of v], lies in accumulators of 16 rows each.  Row
+// 4·(l / 16) + e of accumulator i is row state_row(i, e) of S; the rows of two
+// accumulators, 32·(i / 2) on, are ordered as suits the reads below.
 //
+// load_state_terms: of row l % 16 of the sixteen from row `first` on, the terms
+// that accumulators 2·i and 2·i + 1 hold in this lane.
+// load_columns: terms down column l % 16 of the sixteen that accumulator 2·i holds:
+// rows 4·(l / 16) + e of each of the BLOCKS sixteens of the tile's rows, then the
+// same for accumulator 2·i + 1.
+// load_column: the same down column `column` + l % 16.
+template <typename T> __device__ __forceinline__ uint32_t state_row(int i, int e) {
+    const int q = lane_id() / 16;
+    if constexpr (sizeof(T) == 4) return i * 16 + q * 4 + e;
+    return i / 2 * 32 + q * 8 + i % 2 * 4 + e;
+}
+template <int WIDTH>
+__device__ __forceinline__ void load_state_terms(const char *tile, int first, int i, bf16x4 (&f)[2]) {
+    load_terms<WIDTH, true>(tile, first, i, f);
+}
+template <int WIDTH>
+__device__ __forceinline__ void load_state_terms(const char *tile, int first, int i, f32x4v (&f)[2]) {
+    using Tile = TileOf<float, WIDTH, true>;
+    const int l = lane_id();
+    const uint32_t at = Tile::place(l % 16, i * 8 + l / 16);
+    f[0] = *(const f32x4v *)(tile + first * Tile::kRow + at);
+    f[1] = *(const f32x4v *)(tile + first * Tile::kRow + (at ^ 64)); // four slots on
+}
+
 // The transposing read: lane l names row 4·(l / 16) + l % 16 / 4 and four columns
 // of it, and receives one column of its sixteen lanes' rows.  It is written
 // out, with its wait, because the compiler puts a wait for all loads that write
 // LDS in front of the builtin, those of later chunks among them.
-template <int WIDTH, int STEP, int BLOCKS, bool PAIR>
-__device__ __forceinline__ void load_columns(const char *tile, int column, bf16x4 (&to)[BLOCKS * (PAIR ? 2 : 1)]) {
-    static_assert(BLOCKS == 4);
-    constexpr int kStep = 16 * TileOf<bf16, WIDTH>::kRow;
-    const int l = lane_id(), row = l / 16 * 4 + l % 16 / 4, c = column + l % 4 * STEP;
-    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)tile +
-                        TileOf<bf16, WIDTH>::place(row, c / 8) + c % 8 * 2;
-    if constexpr (PAIR)
-        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
-                     "ds_read_b64_tr_b16 %2, %8 offset:%10\n\tds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
-                     "ds_read_b64_tr_b16 %4, %8 offset:8\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
-                     "ds_read_b64_tr_b16 %6, %8 offset:%13\n\tds_read_b64_tr_b16 %7, %8 offset:%14\n\t"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3]), "=&v"(to[4]), "=&v"(to[5]),
-                       "=&v"(to[6]), "=&v"(to[7])
-                     : "v"(at), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep), "i"(kStep + 8), "i"(2 * kStep + 8),
-                       "i"(3 * kStep + 8));
-    else
-        asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%5\n\t"
-                     "ds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %4 offset:%7\n\t"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3])
-                     : "v"(at), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep));
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
 }
-template <int WIDTH, int STEP, int BLOCKS, bool PAIR>
-__device__ __forceinline__ void load_columns(const char *tile, int column, f32x4v (&to)[BLOCKS * (PAIR ? 2 : 1)]) {
+template <int WIDTH, int BLOCKS>
+__device__ __forceinline__ void load_columns(const char *tile, int i, bf16x4 (&to)[2 * BLOCKS]) {
+    static_assert(BLOCKS == 4);
+    using Tile = TileOf<bf16, WIDTH, false>;
+    constexpr int kStep = 16 * Tile::kRow;
     const int l = lane_id();
+    const uint32_t at = lds_address(tile) + Tile::place(l / 16 * 4 + l % 16 / 4, i * 4 + l % 4);
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%9\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%10\n\tds_read_b64_tr_b16 %3, %8 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %4, %8 offset:8\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %8 offset:%13\n\tds_read_b64_tr_b16 %7, %8 offset:%14\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3]), "=&v"(to[4]), "=&v"(to[5]), "=&v"(to[6]),
+                   "=&v"(to[7])
+                 : "v"(at), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep), "i"(kStep + 8), "i"(2 * kStep + 8),
+                   "i"(3 * kStep + 8));
+}
+template <int WIDTH, int BLOCKS>
+__device__ __forceinline__ void load_column(const char *tile, int column, bf16x4 (&to)[BLOCKS]) {
+    static_assert(BLOCKS == 4);
+    using Tile = TileOf<bf16, WIDTH, false>;
+    constexpr int kStep = 16 * Tile::kRow;
+    const int l = lane_id(), c = column + l % 4 * 4;
+    const uint32_t at = lds_address(tile) + Tile::place(l / 16 * 4 + l % 16 / 4, c / 8) + c % 8 * 2;
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%5\n\t"
+                 "ds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %4 offset:%7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(to[0]), "=&v"(to[1]), "=&v"(to[2]), "=&v"(to[3])
+                 : "v"(at), "i"(kStep), "i"(2 * kStep), "i"(3 * kStep));
+}
+template <int WIDTH, int BLOCKS>
+__device__ __forceinline__ void load_column(const char *tile, int column, f32x4v (&to)[BLOCKS]) {
+    using Tile = TileOf<float, WIDTH, false>;
+    const int l = lane_id(), at = column + l % 16;
 #pragma unroll
-    for (int n = 0; n < BLOCKS * (PAIR ? 2 : 1); ++n) {
-        const char *rows = tile + n % BLOCKS * 16 * TileOf<float, WIDTH>::kRow;
-        const int at = column + n / BLOCKS * 4 + l % 16 / 4 * STEP + l % 4;
+    for (int n = 0; n < BLOCKS; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            to[n][e] = *(const float *)(rows + TileOf<float, WIDTH>::place(l / 16 * 4 + e, at / 4) + at % 4 * 4);
+            to[n][e] = *(const float *)(tile + n * 16 * Tile::kRow + Tile::place(l / 16 * 4 + e, at / 4) + at % 4 * 4);
+}
+template <int WIDTH, int BLOCKS>
+__device__ __forceinline__ void load_columns(const char *tile, int i, f32x4v (&to)[2 * BLOCKS]) {
+    f32x4v part[2][BLOCKS];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        load_column<WIDTH, BLOCKS>(tile, i * 32 + j * 16, part[j]);
+#pragma unroll
+        for (int n = 0; n < BLOCKS; ++n) to[j * BLOCKS + n] = part[j][n];
     }
 }
 
@@ -292,8 +337,8 @@ __device__ __forceinline__ void load_columns(const char *tile, int column, f32x4
 // Otherwise through registers.
 __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-template <typename T, int ROWS, int WIDTH, int THREADS, bool DIRECT> struct Stager {
-    using Tile = TileOf<T, WIDTH>;
+template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIRECT> struct Stager {
+    using Tile = TileOf<T, WIDTH, BY_ROWS>;
     static constexpr int V = Tile::V, N = ROWS * Tile::kSlots / THREADS;
     static_assert(N * THREADS == ROWS * Tile::kSlots);
     typedef typename std::conditional<sizeof(T) == 2, u32x4_a2, u32x4_a4>::type Vec;
@@ -406,10 +451,65 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
     const float log_decay = a.log_decay[h], log2_decay = fmaxf(log_decay * 1.44269504f, -1e30f);
     const auto power = [&](int n) { return __builtin_amdgcn_exp2f(log2_decay * (float)n); };
 
-    // Row r of accumulator 2·i + j is dk 32·i + 8·(r / 4) + 4·j + r % 4: two
-    // accumulators hold the eight neighbours that a query's lane reads at once.
+    const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;
+    Stager<T, C, WK, true, G::kThreads, DIRECT> to_q;
+    Stager<T, C, WK, false, G::kThreads, DIRECT> to_k;
+    Stager<T, C, DV, false, G::kThreads, DIRECT> to_v;
+    to_k.begin(a.sk.token);
+    to_v.begin(a.sv.token);
+    if constexpr (OUTPUTS) to_q.begin(a.sq.token);
+    constexpr int kLoads = to_k.N + to_v.N + (OUTPUTS ? to_q.N : 0); // instructions a chunk
+    const auto stage_of = [&](uint32_t n) { return lds + n % S * G::kStage; };
+    const auto fetch = [&](uint32_t n) {
+        const uint32_t t0 = begin + n * C, rows = end - t0;
+        char *stage = stage_of(n);
+        to_k.load(k + (int64_t)t0 * a.sk.token, a.sk.token, rows, dk, stage);
+        to_v.load(v + (int64_t)t0 * a.sv.token, a.sv.token, rows, dv, stage + G::kTileK);
+        if constexpr (OUTPUTS)
+            to_q.load(q + (int64_t)t0 * a.sq.token, a.sq.token, rows, dk, stage + G::kTileK + G::kTileV);
+    };
+    const auto fetch_ahead = [&](uint32_t n) {
+        const uint32_t ahead = n + (DIRECT ? S - 1 : 1);
+        if (ahead < chunks) fetch(ahead);
+    };
+    // A chunk's outputs, from their place in LDS as whole rows.
+    const auto write_out = [&](uint32_t n) {
+        const char *tile = stage_of(n) + G::kTileK;
+        const uint32_t t0 = begin + n * C;
+        T *rows = out + (int64_t)t0 * a.so.token;
+        using ToOut = Stager<T, C, DV, false, G::kThreads, false>;
+        u32x4 held[ToOut::N];
+#pragma unroll
+        for (int i = 0; i < ToOut::N; ++i) held[i] = *(const u32x4 *)(tile + (threadIdx.x + i * G::kThreads) * 16);
+#pragma unroll
+        for (int i = 0; i < ToOut::N; ++i) {
+            const uint32_t row = ToOut::row_of(threadIdx.x, i), c = ToOut::slot_of(threadIdx.x, i) * ToOut::V;
+            T *to = rows + (int64_t)row * a.so.token + c;
+            if (row >= end - t0) continue;
+            if (c + ToOut::V <= dv) {
+                *(typename ToOut::Vec *)to = held[i];
+            } else {
+                T part[ToOut::V];
+                __builtin_memcpy(part, &held[i], 16);
+#pragma unroll
+                for (int e = 0; e < ToOut::V; ++e)
+                    if (c + e < dv) to[e] = part[e];
+            }
+        }
+    };
+    const auto settle = [&](uint32_t n) { // what went through registers
+        char *stage = stage_of(n);
+        to_k.store(stage);
+        to_v.store(stage + G::kTileK);
+        if constexpr (OUTPUTS) to_q.store(stage + G::kTileK + G::kTileV);
+    };
+    if constexpr (DIRECT) {
+        for (uint32_t n = 0; n < S - 1 && n < chunks; ++n) fetch(n);
+    } else if (chunks) {
+        fetch(0);
+        settle(0);
+    }
     f32x4v s[DK / 16] = {};
-    const auto state_row = [&](int i, int e) { return (uint32_t)(i / 2 * 32 + quad * 8 + i % 2 * 4 + e); };
     float *saved = parts.states + (((uint64_t)b * a.heads + h) * parts.parts + part) * dk * a.dv + dv0 + vcol;
     if (OUTPUTS && vcol < dv) {
         const float *from = parts.parts > 1 ? saved
@@ -420,9 +520,7 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (from && state_row(i, e) < dk) s[i][e] = from[state_row(i, e) * stride];
-        // Here, or the compiler waits in every chunk, and for all its loads.
-        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
+                if (from && state_row<T>(i, e) < dk) s[i][e] = from[state_row<T>(i, e) * stride];
     }
 
     // The decay over a chunk is rounded to a float; what that leaves out of the
@@ -437,7 +535,6 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
         const float by = (float)d;
         return Decay{by, by > 0.0f ? (float)((d - by) / by) : 0.0f};
     };
-    const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;
     Decay decay = decay_over(C);
     const Decay last_decay = decay_over(chunks ? end - begin - (chunks - 1) * C : 1);
     const auto make_good = [&](uint32_t chunks) {
@@ -453,45 +550,24 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
 #pragma unroll
     for (int e = 0; e < 4; ++e) last_weight[e] = power(15 - quad * 4 - e);
 
-    Stager<T, C, WK, G::kThreads, DIRECT> to_q, to_k;
-    Stager<T, C, DV, G::kThreads, DIRECT> to_v;
-    to_k.begin(a.sk.token);
-    to_v.begin(a.sv.token);
-    if constexpr (OUTPUTS) to_q.begin(a.sq.token);
-    constexpr int kLoads = to_k.N + to_v.N + (OUTPUTS ? to_q.N : 0); // instructions a chunk
-    const auto stage_of = [&](uint32_t n) { return lds + n % S * G::kStage; };
-    const auto fetch = [&](uint32_t n) {
-        const uint32_t t0 = begin + n * C, rows = end - t0;
-        char *stage = stage_of(n);
-        to_k.load(k + (int64_t)t0 * a.sk.token, a.sk.token, rows, dk, stage);
-        to_v.load(v + (int64_t)t0 * a.sv.token, a.sv.token, rows, dv, stage + G::kTileK);
-        if constexpr (OUTPUTS)
-            to_q.load(q + (int64_t)t0 * a.sq.token, a.sq.token, rows, dk, stage + G::kTileK + G::kTileV);
-    };
-    const auto settle = [&](uint32_t n) { // what went through registers
-        char *stage = stage_of(n);
-        to_k.store(stage);
-        to_v.store(stage + G::kTileK);
-        if constexpr (OUTPUTS) to_q.store(stage + G::kTileK + G::kTileV);
-    };
-    if constexpr (DIRECT) {
-        for (uint32_t n = 0; n < S - 1 && n < chunks; ++n) fetch(n);
-    } else if (chunks) {
-        fetch(0);
-        settle(0);
-    }
+    // The state has come: or the compiler waits for it in every chunk, and there
+    // for all loads under way.
+    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
     for (uint32_t n = 0; n < chunks; ++n) {
         const uint32_t t0 = begin + n * C;
         const int rows = (int)min((uint32_t)C, end - t0);
         // Chunk n has landed once no more is under way than the chunks after it.
         if (DIRECT && n + S - 2 < chunks) meet<(S - 2) * kLoads>();
         else meet<0>();
-        const uint32_t ahead = DIRECT ? S - 1 : 1;
-        if (n + ahead < chunks) fetch(n + ahead);
-        const char *ks = stage_of(n), *vs = ks + G::kTileK, *qs = vs + G::kTileV;
+        if constexpr (OUTPUTS) {
+            if (n) write_out(n - 1);
+        } else {
+            fetch_ahead(n);
+        }
+        char *ks = stage_of(n), *vs = ks + G::kTileK, *qs = vs + G::kTileV;
 
         F vf[B]; // this lane's column of v
-        load_columns<DV, 4, B, false>(vs, wave * 16, vf);
+        load_column<DV, B>(vs, wave * 16, vf);
 
         f32x4v o[B] = {};
         const auto outputs = [&] {
@@ -503,8 +579,8 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
 #pragma unroll
                 for (int i = 0; i < DK / 32; ++i) {
                     F fk[2], fq[2];
-                    load_terms<WK>(ks, x * 16, i, fk);
-                    load_terms<WK>(qs, y * 16, i, fq);
+                    load_terms<WK, false>(ks, x * 16, i, fk);
+                    load_terms<WK, true>(qs, y * 16, i, fq);
                     p = mma(fk, fq, p);
                 }
 #pragma unroll
@@ -521,7 +597,7 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
 #pragma unroll
                 for (int y = 0; y < B; ++y) {
                     F fq[2];
-                    load_terms<WK>(qs, y * 16, i, fq);
+                    load_state_terms<WK>(qs, y * 16, i, fq);
                     o[y] = mma(state, fq, o[y]);
                 }
             }
@@ -551,7 +627,7 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
 #pragma unroll
             for (int i = 0; i < DK / 16; i += 2) {
                 F fk[2 * B];
-                load_columns<WK, 8, B, true>(ks, i * 16, fk);
+                load_columns<WK, B>(ks, i / 2, fk);
 #pragma unroll
                 for (int m = kTerms<T> - 1; m >= 0; --m)
 #pragma unroll
@@ -589,7 +665,8 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
                 first_bad = min(first_bad, __shfl_xor(first_bad, 16));
                 first_bad = min(first_bad, __shfl_xor(first_bad, 32));
             }
-            meet_lds(); // P is whole
+            meet_lds(); // P is whole, the last chunk's outputs have left LDS
+            fetch_ahead(n);
 #pragma unroll
             for (int y = 0; y < B; ++y)
 #pragma unroll
@@ -608,27 +685,25 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
                         if (y * 16 + col >= from) o[y][e] = __builtin_nanf("");
                 }
             }
-            // Four neighbours of a token's row.
-            T *to = out + (int64_t)(t0 + col) * a.so.token + wave * 16 + quad * 4;
-            if (rows == C && dv >= (wave + 1) * 16u) {
+            // The outputs take the place of v, which all waves have read.
 #pragma unroll
-                for (int y = 0; y < B; ++y, to += 16 * a.so.token) {
-                    const F r = rounded(o[y], T{});
-                    __builtin_memcpy(to, &r, sizeof(r));
-                }
-            } else {
-                const uint32_t c = wave * 16 + here(quad * 4);
-                for (int y = 0; y < B; ++y, to += 16 * a.so.token)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (y * 16 + col < rows && c + e < dv) to[e] = (T)o[y][e];
+            for (int y = 0; y < B; ++y) {
+                const F r = rounded(o[y], T{});
+                const int c = wave * 16 + quad * 4;
+                using Tile = TileOf<T, DV, false>;
+                *(F *)(vs + Tile::place(y * 16 + col, c / Tile::V) + c % Tile::V * sizeof(T)) = r;
             }
         }
 
         if (!DIRECT && n + 1 < chunks) settle(n + 1);
     }
 
-    if constexpr (OUTPUTS) { // rows past the sequence's end
+    if constexpr (OUTPUTS) {
+        if (chunks) {
+            meet_lds();
+            write_out(chunks - 1);
+        }
+        // Rows past the sequence's end.
         const uint32_t until = min(begin + parts.span, tokens);
         for (uint32_t t = max(begin, length) + threadIdx.x / 16; t < until; t += G::kThreads / 16)
             for (uint32_t c = threadIdx.x % 16; c < dv; c += 16) out[(int64_t)t * a.so.token + c] = (T)0.0f;
@@ -642,7 +717,7 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
     for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (to && state_row(i, e) < dk) to[state_row(i, e) * stride] = s[i][e];
+            if (to && state_row<T>(i, e) < dk) to[state_row<T>(i, e) * stride] = s[i][e];
 }
 
 // The state before each part, from the parts' own sums: one element of the
