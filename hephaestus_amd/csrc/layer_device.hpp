@@ -17,19 +17,22 @@ template <typename T> struct Pack16;
 template <> struct Pack16<float> { static constexpr int N = 4; };
 template <> struct Pack16<bf16> { static constexpr int N = 8; };
 
-// f32 values of the 16 bytes at p.
-__device__ __forceinline__ void load_pack(const float *p, float (&x)[4]) {
-    const f32x4 r = *(const f32x4_a4 *)p;
+__device__ __forceinline__ u32x4 load_raw(const float *p) { return *(const u32x4_a4 *)p; }
+__device__ __forceinline__ u32x4 load_raw(const bf16 *p) { return *(const u32x4_a2 *)p; }
+// f32 values of 16 bytes of elements.
+template <typename T, int N> __device__ __forceinline__ void unpack(u32x4 v, float (&x)[N]) {
+    static_assert(N == Pack16<T>::N);
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 f = __builtin_bit_cast(f32x4, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = r[i];
-}
-__device__ __forceinline__ void load_pack(const bf16 *p, float (&x)[8]) {
-    const u32x4 r = *(const u32x4_a2 *)p;
+        for (int i = 0; i < 4; ++i) x[i] = f[i];
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t two = r[i];
-        x[2 * i] = __builtin_bit_cast(float, two << 16);
-        x[2 * i + 1] = __builtin_bit_cast(float, two & 0xFFFF0000u);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t two = v[i];
+            x[2 * i] = __builtin_bit_cast(float, two << 16);
+            x[2 * i + 1] = __builtin_bit_cast(float, two & 0xFFFF0000u);
+        }
     }
 }
 __device__ __forceinline__ void store_pack(float *p, const float (&x)[4]) {
@@ -41,17 +44,6 @@ __device__ __forceinline__ void store_pack(bf16 *p, const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = (bf16)x[i];
     *(u32x4_a2 *)p = __builtin_bit_cast(u32x4, r);
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-    return v;
 }
 
 } // namespace hx

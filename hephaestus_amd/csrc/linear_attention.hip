@@ -2,11 +2,17 @@
 // gfx950:
 //   S_t = e^g·S_{t-1} + k_tᵀ·v_t,   o_t = scale·q_t·S_t.
 //
-// Two forms.  The recurrence, for single tokens: a block holds 32 columns of one head's state in registers,
-// eight lanes of four columns by 32 groups of rows, and steps through the
-// tokens.  Each step is a rank-1 update of the lane's own elements and a sum
-// over the rows: within the wave by lane exchange, across the four waves
-// through LDS (two buffers in turn, so one barrier a token).
+// Two forms.  The recurrence, for a few tokens: a block holds 32 columns of one
+// head's state in registers, eight lanes of four columns by 32 groups of rows,
+// and steps through the tokens.  Each step is a rank-1 update of the lane's own
+// elements and a sum over the rows: within the wave by lane exchange, across the
+// four waves through LDS (two buffers in turn, so one barrier a token).  The
+// state's bytes, in and out, bound it: 128 sequences of 32 heads of 128 x 128
+// take 97 us, 5.5 TB/s.  Blocks of 64 or 128 columns, with whole rows of the
+// state side by side but more registers, took 154 and 95 us, and for one
+// sequence of 16 heads 6.3 and 6.8 us against 4.7.
+//
+// Chunks, for prompts: below.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 
@@ -16,36 +22,49 @@
 namespace hx {
 namespace {
 
-constexpr int kColumns = 32; // of a state, a block
-constexpr int kRowGroups = 32;
-
 // Four columns of a row from column c on.  VEC: the rows are 16-byte aligned
-// and the width a multiple of four.
-template <bool VEC> __device__ __forceinline__ f32x4 load4(const float *row, uint32_t c, uint32_t width) {
-    if constexpr (VEC) return c < width ? *(const f32x4 *)(row + c) : f32x4{0, 0, 0, 0};
+// and the width a multiple of four.  NT: streamed, not kept in the caches.
+template <bool VEC, bool NT> __device__ __forceinline__ f32x4 load4(const float *row, uint32_t c, uint32_t width) {
+    if constexpr (VEC) return c < width ? load_vec<NT>((const f32x4 *)(row + c)) : f32x4{0, 0, 0, 0};
     f32x4 v = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (c + i < width) v[i] = row[c + i];
     return v;
 }
-template <bool VEC> __device__ __forceinline__ void store4(float *row, uint32_t c, uint32_t width, f32x4 v) {
+template <bool VEC, bool NT> __device__ __forceinline__ void store4(float *row, uint32_t c, uint32_t width, f32x4 v) {
     if constexpr (VEC) {
-        if (c < width) *(f32x4 *)(row + c) = v;
+        if (c < width) store_vec<NT>(v, (f32x4 *)(row + c));
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (c + i < width) row[c + i] = v[i];
 }
+// N neighbours of a row of T in f32, zeros past its end.
+template <int N, typename T> __device__ __forceinline__ void load_run(const T *p, uint32_t from, uint32_t end, float (&x)[N]) {
+    if (from + N <= end) {
+        typedef T Run __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+        const Run v = *(const Run *)(p + from);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = from + i < end ? (float)p[from + i] : 0.0f;
+    }
+}
 
-// Rows of the state a lane: dk at most 32·ROWS.
-template <typename T, int ROWS, bool VEC>
+constexpr uint64_t kStreamedBytes = 64ull << 20;
+
+// A block takes COLUMNS columns of a state, four a lane, and all its rows, ROWS
+// neighbours a lane: dk at most ROWS·1024 / COLUMNS.
+template <typename T, int COLUMNS, int ROWS, bool VEC, bool NT>
 __global__ __launch_bounds__(256) void attention_step_kernel(AttentionArgs a) {
-    __shared__ f32x4 part[2][4][8];
+    constexpr int kLanes = COLUMNS / 4; // of a row
+    __shared__ f32x4 part[2][4][kLanes];
     const uint32_t h = blockIdx.y, b = blockIdx.z, hk = (uint32_t)(h / (a.heads / a.kv_heads));
     const uint32_t dk = (uint32_t)a.dk, dv = (uint32_t)a.dv;
-    const uint32_t c = blockIdx.x * kColumns + threadIdx.x % 8 * 4, group = threadIdx.x / 8;
+    const uint32_t c = blockIdx.x * COLUMNS + threadIdx.x % kLanes * 4, row0 = threadIdx.x / kLanes * ROWS;
     const int wave = threadIdx.x / kWave;
     const uint64_t length = a.lengths ? min((uint64_t)a.lengths[b], a.tokens) : a.tokens;
     const T *q = (const T *)a.q + b * a.sq.batch + h * a.sq.head;
@@ -56,48 +75,46 @@ __global__ __launch_bounds__(256) void attention_step_kernel(AttentionArgs a) {
     f32x4 s[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        const uint32_t row = group + kRowGroups * r;
         s[r] = f32x4{0, 0, 0, 0};
-        if (a.state_in && row < dk)
-            s[r] = load4<VEC>(a.state_in + b * a.si.batch + h * a.si.head + row * a.si.token, c, dv);
+        if (a.state_in && row0 + r < dk)
+            s[r] = load4<VEC, NT>(a.state_in + b * a.si.batch + h * a.si.head + (row0 + r) * a.si.token, c, dv);
     }
     for (uint64_t t = 0; t < length; ++t) {
-        f32x4 vt = {0, 0, 0, 0}, o = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < dv) vt[i] = (float)v[(int64_t)t * a.sv.token + c + i];
+        float vt[4], kt[ROWS], qt[ROWS];
+        load_run<4>(v + (int64_t)t * a.sv.token, c, dv, vt);
+        load_run<ROWS>(k + (int64_t)t * a.sk.token, row0, dk, kt);
+        load_run<ROWS>(q + (int64_t)t * a.sq.token, row0, dk, qt);
+        const f32x4 values = {vt[0], vt[1], vt[2], vt[3]};
+        f32x4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const uint32_t row = group + kRowGroups * r;
-            if (row >= dk) continue;
-            const float kt = (float)k[(int64_t)t * a.sk.token + row], qt = (float)q[(int64_t)t * a.sq.token + row];
-            s[r] = decay * s[r] + kt * vt;
-            o += qt * s[r];
+            s[r] = decay * s[r] + kt[r] * values;
+            // A row past dk adds nothing, whatever the value.
+            if (row0 + r < dk) o += qt[r] * s[r];
         }
 #pragma unroll
-        for (int d = 8; d < kWave; d *= 2)
+        for (int d = kLanes; d < kWave; d *= 2)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d);
-        f32x4(*buffer)[8] = part[t & 1];
-        if (lane_id() < 8) buffer[wave][lane_id()] = o;
+        f32x4(*buffer)[kLanes] = part[t & 1];
+        if (lane_id() < kLanes) buffer[wave][lane_id()] = o;
         __syncthreads();
-        if (threadIdx.x < 8) {
+        if (threadIdx.x < kLanes) {
             o = (buffer[0][threadIdx.x] + buffer[1][threadIdx.x]) + (buffer[2][threadIdx.x] + buffer[3][threadIdx.x]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (c + i < dv) out[(int64_t)t * a.so.token + c + i] = (T)(o[i] * a.scale);
         }
     }
-    for (uint64_t t = length + group; t < a.tokens; t += kRowGroups)
+    for (uint64_t t = length + threadIdx.x / kLanes; t < a.tokens; t += 256 / kLanes)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (c + i < dv) out[(int64_t)t * a.so.token + c + i] = (T)0.0f;
     if (!a.state_out) return;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        const uint32_t row = group + kRowGroups * r;
-        if (row < dk) store4<VEC>(a.state_out + b * a.st.batch + h * a.st.head + row * a.st.token, c, dv, s[r]);
-    }
+    for (int r = 0; r < ROWS; ++r)
+        if (row0 + r < dk)
+            store4<VEC, NT>(a.state_out + b * a.st.batch + h * a.st.head + (row0 + r) * a.st.token, c, dv, s[r]);
 }
 
 bool vector_rows(const float *base, const AttentionView &s, uint64_t dv) {
@@ -105,12 +122,22 @@ bool vector_rows(const float *base, const AttentionView &s, uint64_t dv) {
                                s.token % 4 == 0);
 }
 
-template <typename T, int ROWS> hx_status launch_step(const AttentionArgs &a, hipStream_t stream) {
-    const dim3 grid((uint32_t)ceil_div(a.dv, kColumns), (uint32_t)a.heads, (uint32_t)a.batch);
-    if (vector_rows(a.state_in, a.si, a.dv) && vector_rows(a.state_out, a.st, a.dv))
-        hipLaunchKernelGGL((attention_step_kernel<T, ROWS, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attention_step_kernel<T, ROWS, false>), grid, dim3(256), 0, stream, a);
+template <typename T, int COLUMNS, int ROWS> hx_status launch_step(const AttentionArgs &a, hipStream_t stream) {
+    const dim3 grid((uint32_t)ceil_div(a.dv, COLUMNS), (uint32_t)a.heads, (uint32_t)a.batch);
+    const bool vec = vector_rows(a.state_in, a.si, a.dv) && vector_rows(a.state_out, a.st, a.dv);
+    // States that the caches cannot hold until the next token are streamed.
+    const bool nt = a.batch * a.heads * a.dk * a.dv * sizeof(float) > kStreamedBytes;
+    if (vec && nt) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true, true>), grid, dim3(256), 0, stream, a);
+    else if (vec) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true, false>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, false, false>), grid, dim3(256), 0, stream, a);
     return check_launch("attention_step_kernel");
+}
+
+template <typename T> hx_status launch_steps(const AttentionArgs &a, hipStream_t stream) {
+    if (a.dk <= 32) return launch_step<T, 32, 1>(a, stream);
+    if (a.dk <= 64) return launch_step<T, 32, 2>(a, stream);
+    if (a.dk <= 128) return launch_step<T, 32, 4>(a, stream);
+    return launch_step<T, 32, 8>(a, stream);
 }
 
 // ------------------------------------------------------------------ chunks
@@ -755,7 +782,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Pa
 // of q, k and 128 columns of v would not fit LDS.
 uint32_t block_waves(const AttentionArgs &a) { return a.dv <= 64 || a.dk > 128 ? 4 : 8; }
 
-constexpr uint64_t kStepTokens = 8; // up to here the recurrence
 constexpr uint64_t kFullCard = 256; // blocks
 
 Parts parts_of(const AttentionArgs &a) {
@@ -811,7 +837,11 @@ template <typename T, bool DIRECT> hx_status launch_chunked(const AttentionArgs 
     return block_waves(a) == 4 ? launch_width<T, 4, DIRECT>(a, ws, stream) : launch_width<T, 8, DIRECT>(a, ws, stream);
 }
 
-bool by_chunks(const AttentionArgs &a) { return a.tokens > kStepTokens && a.dk > 0; }
+// Up to 4 tokens (10 in f32, whose matrix instructions are slower) the recurrence
+// is faster: 32 heads of one sequence take 4.9 us for one token and 1.1 us for
+// each more (0.8 in f32), chunks 11 us (14) however few the tokens; 32 sequences
+// 32 us and 5.2 (3.4), chunks 50 (70).
+bool by_chunks(const AttentionArgs &a) { return a.tokens > (a.dtype == HX_DTYPE_F32 ? 10 : 4) && a.dk > 0; }
 
 template <typename T> hx_status launch(const AttentionArgs &a, void *ws, hipStream_t stream) {
     if (by_chunks(a)) {
@@ -819,10 +849,7 @@ template <typename T> hx_status launch(const AttentionArgs &a, void *ws, hipStre
                             direct_rows<T>(a.v, a.sv, a.dv);
         return direct ? launch_chunked<T, true>(a, ws, stream) : launch_chunked<T, false>(a, ws, stream);
     }
-    if (a.dk <= 32) return launch_step<T, 1>(a, stream);
-    if (a.dk <= 64) return launch_step<T, 2>(a, stream);
-    if (a.dk <= 128) return launch_step<T, 4>(a, stream);
-    return launch_step<T, 8>(a, stream);
+    return launch_steps<T>(a, stream);
 }
 
 } // namespace

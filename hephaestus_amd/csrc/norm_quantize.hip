@@ -36,37 +36,46 @@ __device__ __forceinline__ int quantize(float hw, const RowScale &r) {
     return r.inv > 0.0f ? (int)fminf(fmaxf(rintf(hw * r.up * r.inv), -127.0f), 127.0f) : 0;
 }
 
-// Σ and max over the WAVES waves of a row; every wave of the block calls it.
-template <int WAVES> __device__ __forceinline__ void combine(float &sum, uint32_t &top) {
-    sum = wave_sum(sum);
-    top = wave_max(top);
-    if constexpr (WAVES > 1) {
-        __shared__ float sums[WAVES];
-        __shared__ uint32_t tops[WAVES];
-        const int wave = threadIdx.x / kWave;
-        if (lane_id() == 0) {
-            sums[wave] = sum;
-            tops[wave] = top;
-        }
-        __syncthreads();
-        sum = 0.0f;
-        top = 0;
+// Σ and max over a row's lanes: LANES of one wave, or WAVES waves of a block.
+template <int LANES> __device__ __forceinline__ void combine_lanes(float &sum, uint32_t &top) {
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            sum += sums[i];
-            top = max(top, tops[i]);
-        }
+    for (int d = 1; d < LANES; d *= 2) {
+        sum += __shfl_xor(sum, d);
+        top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    }
+}
+template <int WAVES> __device__ __forceinline__ void combine_waves(float &sum, uint32_t &top) {
+    combine_lanes<kWave>(sum, top);
+    __shared__ float sums[WAVES];
+    __shared__ uint32_t tops[WAVES];
+    const int wave = threadIdx.x / kWave;
+    if (lane_id() == 0) {
+        sums[wave] = sum;
+        tops[wave] = top;
+    }
+    __syncthreads();
+    sum = 0.0f;
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        sum += sums[i];
+        top = max(top, tops[i]);
     }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T *p, uint32_t c, uint32_t cols, float (&x)[N]) {
-    if (c + N <= cols) {
-        load_pack(p + c, x);
-    } else {
+// The 16 bytes at column c, zeros past the row's end: as loaded, so that nothing
+// waits for them before all of a row's loads are under way.
+template <typename T> __device__ __forceinline__ u32x4 load_row(const T *p, uint32_t c, uint32_t cols) {
+    constexpr uint32_t N = Pack16<T>::N;
+    if (c + N <= cols) return load_raw(p + c);
+    u32x4 v = {0, 0, 0, 0};
+    if (c < cols) {
+        T part[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = c + i < cols ? (float)p[c + i] : 0.0f;
+        for (uint32_t i = 0; i < N; ++i) part[i] = c + i < cols ? p[c + i] : (T)0.0f;
+        __builtin_memcpy(&v, part, 16);
     }
+    return v;
 }
 
 template <typename T, int N>
@@ -99,47 +108,66 @@ __device__ __forceinline__ void store_bytes(int8_t *p, uint32_t c, uint32_t cols
     }
 }
 
-// WAVES waves a row, STEPS vectors a lane; rows of up to WAVES·64·STEPS·N.
-template <typename T, int WAVES, int STEPS>
-__global__ __launch_bounds__(WAVES *kWave) void norm_rows_kernel(NormArgs a) {
-    constexpr int N = Pack16<T>::N;
-    const uint64_t row = blockIdx.x;
+// Rows of up to LANES·STEPS vectors, LANES threads a row.  A block has one row,
+// or, where a row has less than four waves, as many as fill four.
+template <typename T, int LANES, int STEPS>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows_kernel(NormArgs a) {
+    constexpr int N = Pack16<T>::N, kRows = LANES <= kWave ? 256 / LANES : 1;
+    static_assert(LANES <= kWave || LANES >= 256);
+    const uint64_t row = kRows > 1 ? (uint64_t)blockIdx.x * kRows + threadIdx.x / LANES : blockIdx.x;
+    const uint32_t lane = kRows > 1 ? threadIdx.x % LANES : threadIdx.x;
+    if (kRows > 1 && row >= a.rows) return; // a row's lanes leave together
     const uint32_t cols = (uint32_t)a.cols;
     const T *x = (const T *)a.x + (int64_t)row * a.x_stride;
     const T *res = (const T *)a.residual + (int64_t)row * a.residual_stride;
     const T *w = (const T *)a.weight;
-    float h[STEPS][N], hw[STEPS][N];
+    u32x4 vx[STEPS], vr[STEPS], vw[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const uint32_t c = ((uint32_t)s * LANES + lane) * N;
+        vx[s] = load_row(x, c, cols);
+        vr[s] = u32x4{0, 0, 0, 0};
+        if (a.residual) vr[s] = load_row(res, c, cols);
+        vw[s] = load_row(w, c, cols);
+    }
+    // h and h·w of a vector, from the registers it was loaded into.
+    const auto values = [&](int s, float(&h)[N], float(&hw)[N]) {
+        float r[N];
+        unpack<T>(vx[s], h);
+        unpack<T>(vr[s], r);
+        unpack<T>(vw[s], hw);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (a.residual) h[i] += r[i];
+            hw[i] *= h[i];
+        }
+    };
     float sum = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const uint32_t c = ((uint32_t)s * WAVES * kWave + threadIdx.x) * N;
-        load_row(x, c, cols, h[s]);
-        if (a.residual) {
-            float r[N];
-            load_row(res, c, cols, r);
-#pragma unroll
-            for (int i = 0; i < N; ++i) h[s][i] += r[i];
-        }
-        load_row(w, c, cols, hw[s]);
+        float h[N], hw[N];
+        values(s, h, hw);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            sum += h[s][i] * h[s][i];
-            hw[s][i] *= h[s][i];
-            top = max(top, magnitude(hw[s][i]));
+            sum += h[i] * h[i];
+            top = max(top, magnitude(hw[i]));
         }
     }
-    combine<WAVES>(sum, top);
+    if constexpr (LANES <= kWave) combine_lanes<LANES>(sum, top);
+    else combine_waves<LANES / kWave>(sum, top);
     const RowScale r = row_scale(sum, top, (float)a.cols, a.epsilon);
-    if (threadIdx.x == 0) a.scales[row] = r.scale;
+    if (lane == 0) a.scales[row] = r.scale;
     T *ho = (T *)a.residual_out + (int64_t)row * a.residual_out_stride;
     int8_t *q = a.quantized + (int64_t)row * a.quantized_stride;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const uint32_t c = ((uint32_t)s * WAVES * kWave + threadIdx.x) * N;
+        const uint32_t c = ((uint32_t)s * LANES + lane) * N;
         if (c >= cols) continue;
-        if (a.residual_out) store_row(ho, c, cols, h[s]);
-        store_bytes(q, c, cols, hw[s], r);
+        float h[N], hw[N];
+        values(s, h, hw);
+        if (a.residual_out) store_row(ho, c, cols, h);
+        store_bytes(q, c, cols, hw, r);
     }
 }
 
@@ -155,14 +183,14 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_long_rows_ker
     T *ho = (T *)a.residual_out + (int64_t)row * a.residual_out_stride;
     int8_t *q = a.quantized + (int64_t)row * a.quantized_stride;
     const auto sweep = [&](uint32_t c, float (&h)[N], float (&hw)[N]) {
-        load_row(x, c, cols, h);
+        unpack<T>(load_row(x, c, cols), h);
         if (a.residual) {
             float r[N];
-            load_row(res, c, cols, r);
+            unpack<T>(load_row(res, c, cols), r);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] += r[i];
         }
-        load_row(w, c, cols, hw);
+        unpack<T>(load_row(w, c, cols), hw);
 #pragma unroll
         for (int i = 0; i < N; ++i) hw[i] *= h[i];
     };
@@ -177,7 +205,7 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_long_rows_ker
             top = max(top, magnitude(hw[i]));
         }
     }
-    combine<16>(sum, top);
+    combine_waves<16>(sum, top);
     const RowScale r = row_scale(sum, top, (float)a.cols, a.epsilon);
     if (threadIdx.x == 0) a.scales[row] = r.scale;
     for (uint32_t c = threadIdx.x * N; c < cols; c += 1024 * N) {
@@ -189,15 +217,25 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_long_rows_ker
 }
 
 template <typename T> hx_status launch(const NormArgs &a, hipStream_t stream) {
-    constexpr uint64_t N = Pack16<T>::N;
-    const uint64_t vectors = ceil_div(a.cols, N);
-    const dim3 grid((uint32_t)a.rows);
-    if (vectors <= 4 * kWave) hipLaunchKernelGGL((norm_rows_kernel<T, 1, 4>), grid, dim3(kWave), 0, stream, a);
-    else if (vectors <= 16 * kWave)
-        hipLaunchKernelGGL((norm_rows_kernel<T, 4, 4>), grid, dim3(4 * kWave), 0, stream, a);
-    else if (vectors <= 64 * kWave)
-        hipLaunchKernelGGL((norm_rows_kernel<T, 16, 4>), grid, dim3(16 * kWave), 0, stream, a);
-    else hipLaunchKernelGGL((norm_long_rows_kernel<T>), grid, dim3(1024), 0, stream, a);
+    const uint64_t vectors = ceil_div(a.cols, Pack16<T>::N);
+    const auto run = [&](auto kernel, uint64_t lanes) {
+        const uint64_t rows = lanes <= kWave ? 256 / lanes : 1;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)ceil_div(a.rows, rows)), dim3((uint32_t)(lanes < 256 ? 256 : lanes)), 0,
+                           stream, a);
+    };
+    // One or two vectors a thread as long as rows allow: a thread that holds
+    // more keeps fewer waves on a CU.  Measured (us): 16384 x 128 16 lanes 5.5, 64
+    // lanes 10.8; 16384 x 1024 64 lanes 23.5, 256 30.0; 16384 x 4096 512 lanes
+    // 77.8, 64 88.8, 1024 100.6; 1 x 4096 512 lanes 2.7, 64 6.1.
+    if (vectors <= 16) run(norm_rows_kernel<T, 16, 1>, 16);
+    else if (vectors <= 64) run(norm_rows_kernel<T, 64, 1>, 64);
+    else if (vectors <= 128) run(norm_rows_kernel<T, 64, 2>, 64);
+    else if (vectors <= 256) run(norm_rows_kernel<T, 256, 1>, 256);
+    else if (vectors <= 512) run(norm_rows_kernel<T, 512, 1>, 512);
+    else if (vectors <= 1024) run(norm_rows_kernel<T, 512, 2>, 512);
+    else if (vectors <= 2048) run(norm_rows_kernel<T, 512, 4>, 512);
+    else if (vectors <= 4096) run(norm_rows_kernel<T, 1024, 4>, 1024);
+    else run(norm_long_rows_kernel<T>, 1024);
     return check_launch("norm_rows_kernel");
 }
 
