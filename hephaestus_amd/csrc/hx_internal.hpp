@@ -378,6 +378,10 @@ hx_status launch_map_reduce(const MapReduceArgs &args, void *ws, uint64_t ws_byt
 hx_status launch_vector_op(hx_vector_op op, const float *t, const float *s, float *out, uint64_t n,
                            float factor, hipStream_t stream);
 
+// Let `kernel` take `bytes` of dynamic LDS, beyond 64 KiB if need be, on the
+// current device.  `allowed` remembers the devices, a bit each.
+hx_status allow_lds(const void *kernel, uint32_t bytes, std::atomic<uint64_t> &allowed);
+
 // Layer operators (layer_ops.cpp checks, then launches).  Pointers are to the
 // first element of each view, strides count elements; the last dimension of
 // every view has stride 1.

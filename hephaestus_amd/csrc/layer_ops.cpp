@@ -366,6 +366,22 @@ hx_status make_plan(hx_device *dev, const Args &args, uint64_t bytes, hx_plan **
 
 } // namespace
 
+namespace hx {
+
+hx_status allow_lds(const void *kernel, uint32_t bytes, std::atomic<uint64_t> &allowed) {
+    if (bytes <= 65536) return HX_OK;
+    int device = 0;
+    HX_HIP(hipGetDevice(&device), HX_ERR_DISPATCH_FAILED, "hipGetDevice");
+    const uint64_t bit = device < 64 ? 1ull << device : 0; // asked for anew where there is no bit
+    if (allowed.load(std::memory_order_relaxed) & bit) return HX_OK;
+    HX_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), HX_ERR_DISPATCH_FAILED,
+           "LDS size");
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+    return HX_OK;
+}
+
+} // namespace hx
+
 extern "C" {
 
 hx_status hx_rms_norm_quantize(hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,

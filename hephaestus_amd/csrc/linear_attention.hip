@@ -17,6 +17,7 @@
 #include "layer_device.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace hx {
@@ -800,11 +801,8 @@ hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
     const auto run = [&](auto outputs) {
         using G = Chunk<T, DK, NW, decltype(outputs)::value, DIRECT>;
         const auto kernel = attention_chunk_kernel<T, DK, NW, decltype(outputs)::value, DIRECT>;
-        if constexpr (G::kLds > 65536) {
-            static const hipError_t allowed =
-                hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-            if (allowed != hipSuccess) return hip_fail(HX_ERR_DISPATCH_FAILED, allowed, "attention LDS size");
-        }
+        static std::atomic<uint64_t> allowed{0};
+        HX_TRY(allow_lds((const void *)kernel, G::kLds, allowed));
         const uint64_t x = ceil_div(a.dv, G::DV) * parts.parts;
         hipLaunchKernelGGL(kernel, dim3((uint32_t)x, (uint32_t)a.heads, (uint32_t)a.batch), dim3(G::kThreads), G::kLds,
                            stream, a, parts);

@@ -14,6 +14,8 @@
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 
+#include <atomic>
+
 namespace hx {
 namespace {
 
@@ -304,11 +306,8 @@ template <typename T, int BM, int BN, int WM, int WN, int KG, int S>
 hx_status launch_tiles(const MatmulArgs &p, hipStream_t stream) {
     using C = Tile<BM, BN, WM, WN, KG, S>;
     const auto kernel = matmul_tiles_kernel<T, BM, BN, WM, WN, KG, S>;
-    if constexpr (C::kLds > 65536) {
-        static const hipError_t allowed =
-            hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds);
-        if (allowed != hipSuccess) return hip_fail(HX_ERR_DISPATCH_FAILED, allowed, "matmul LDS size");
-    }
+    static std::atomic<uint64_t> allowed{0};
+    HX_TRY(allow_lds((const void *)kernel, C::kLds, allowed));
     const uint64_t tm = ceil_div(p.m, BM), tn = ceil_div(p.n, BN);
     if (tm * tn > 0x7FFFFFFFull)
         return fail(HX_ERR_DISPATCH_FAILED, "matmul of %llu tiles exceeds the grid range", (unsigned long long)(tm * tn));
@@ -317,23 +316,31 @@ hx_status launch_tiles(const MatmulArgs &p, hipStream_t stream) {
     return check_launch("matmul_tiles_kernel");
 }
 
-// The largest tile of which there are enough for the 256 CUs (from 160 on: a
-// smaller tile moves more bytes to the same CUs).  Where there are more tiles
-// than CUs two blocks share one, with LDS for half the steps in flight; the
-// smaller the tile, the more groups share a block's k.  Measured (us):
+// The largest tile of which there are enough for the 256 CUs: a smaller tile
+// moves more bytes to the same CUs.  Where there are more tiles than CUs two
+// blocks share one, with LDS for half the steps in flight.  Groups that share a
+// block's k keep more loads under way in a block, for about 2 us to add their
+// sums: worth it for long rows, or where tiles are too few to fill the card.
+// Measured (us):
 //   1000 x 8192 x 8192   128 x 128 71.1    64 x 64 109     256 x 256 115
 //   2048 x 2048 x 2048   128 x 128 16.6    64 x 64 19.0    256 x 256 37.8
-//   300 x 2048 x 2048    64 x 64 6.5       64 x 32 8.0     128 x 128 12.7
-//   256 x 1024 x 8192    32 x 32 10.2      64 x 32 13.5    64 x 64 17.4
-//   20 x 4096 x 4096     32 x 16 6.0       32 x 32 7.0     64 x 32 8.3
+//   1500 x 1500 x 8192    96 x  96 28.6    64 x 64 39.2
+//   128 x 8192 x 4096     64 x  64 10.9 in three groups, 11.8 in one
+//   700 x 1500 x 1500     64 x  64 22.5 in three groups, 12.6 in one
+//   256 x 1024 x 8192     32 x  32 10.2    64 x 32 13.5    64 x 64 17.4
+//   20 x 4096 x 4096      32 x  16 6.0     32 x 32 7.0     64 x 32 8.3
 template <typename T> hx_status launch_tiled(const MatmulArgs &p, hipStream_t stream) {
     const auto tiles = [&](uint64_t bm, uint64_t bn) { return ceil_div(p.m, bm) * ceil_div(p.n, bn); };
-    constexpr uint64_t kEnough = 160, kCus = 256;
+    constexpr uint64_t kCus = 256, kEnough = 160, kFull = 192;
+    const bool long_rows = p.k >= 4096;
     if (tiles(256, 256) >= kEnough) return launch_tiles<T, 256, 256, 2, 4, 1, 2>(p, stream);
     if (tiles(128, 128) > kCus) return launch_tiles<T, 128, 128, 2, 2, 1, 2>(p, stream);
-    if (tiles(128, 128) >= kEnough) return launch_tiles<T, 128, 128, 2, 4, 1, 4>(p, stream);
-    if (tiles(64, 64) > kCus) return launch_tiles<T, 64, 64, 2, 2, 2, 2>(p, stream);
-    if (tiles(64, 64) >= kEnough) return launch_tiles<T, 64, 64, 2, 2, 4, 2>(p, stream);
+    if (tiles(128, 128) >= kFull) return launch_tiles<T, 128, 128, 2, 4, 1, 4>(p, stream);
+    if (long_rows && tiles(96, 96) >= kFull && tiles(96, 96) <= kCus)
+        return launch_tiles<T, 96, 96, 2, 2, 2, 3>(p, stream);
+    if (long_rows && tiles(64, 64) >= kEnough && tiles(64, 64) <= kCus)
+        return launch_tiles<T, 64, 64, 2, 2, 3, 3>(p, stream);
+    if (tiles(64, 64) >= kEnough) return launch_tiles<T, 64, 64, 4, 2, 1, 4>(p, stream);
     if (tiles(64, 32) > kCus) return launch_tiles<T, 64, 32, 2, 1, 3, 2>(p, stream);
     if (tiles(64, 32) >= kEnough) return launch_tiles<T, 64, 32, 2, 1, 6, 2>(p, stream);
     if (tiles(32, 32) > kCus) return launch_tiles<T, 32, 32, 1, 2, 4, 2>(p, stream);
