@@ -783,14 +783,33 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Pa
 // of q, k and 128 columns of v would not fit LDS.
 uint32_t block_waves(const AttentionArgs &a) { return a.dv <= 64 || a.dk > 128 ? 4 : 8; }
 
-constexpr uint64_t kFullCard = 256; // blocks
-
+// How many parts a prompt is cut into where there are fewer heads than the card
+// takes blocks.  The parts run side by side, but their own sums have to be taken
+// first, in half the time of the outputs, and their states written, joined and
+// read.  Times in us as measured: a chunk 4.7 for heads of 128 x 128 (6.2 in f32,
+// of 32 tokens), 3.0 for 64 x 64; two more launches 12; the states 5 TB/s.
+//   1 x 16 x 16384 tokens, 16 parts  121, uncut 860
+//   1 x  8 x 512,           8 parts   21, uncut  32
+//   4 x 16 x 512,           4 parts   39, uncut  35
+//   2 x 64 x 4096 of 64 x 64, 4 parts 115, 2 parts 148, uncut 184
 Parts parts_of(const AttentionArgs &a) {
-    const uint64_t chunk = a.dtype == HX_DTYPE_F32 ? 32 : 64, chunks = ceil_div(a.tokens, chunk);
+    const bool f32 = a.dtype == HX_DTYPE_F32;
+    const uint64_t chunk = f32 ? 32 : 64, chunks = ceil_div(a.tokens, chunk);
     const uint64_t blocks = a.batch * a.heads * ceil_div(a.dv, 16 * block_waves(a));
-    uint64_t parts = blocks < kFullCard / 2 ? kFullCard / blocks : 1;
-    parts = std::min(parts, std::max<uint64_t>(chunks / 4, 1));
-    const uint64_t span = ceil_div(chunks, parts) * chunk;
+    // Blocks of the narrowest heads take half a CU's LDS.
+    const uint64_t card = a.dk <= 64 && a.dv <= 64 && !f32 ? 512 : 256;
+    const double area = (double)(a.dk * a.dv) / (128 * 128), chunk_us = 2.4 + (f32 ? 3.8 : 2.3) * area;
+    uint64_t best = 1;
+    double best_us = chunks * chunk_us;
+    for (uint64_t parts = 2; parts <= std::min(chunks, card / blocks); ++parts) {
+        const double states_us = (double)(a.batch * a.heads * parts) * area * (128 * 128 * 16) / 5e6;
+        const double us = ceil_div(chunks, parts) * 1.5 * chunk_us + 12 + states_us;
+        if (us < best_us) {
+            best_us = us;
+            best = parts;
+        }
+    }
+    const uint64_t span = ceil_div(chunks, best) * chunk;
     return Parts{(uint32_t)ceil_div(a.tokens, span), (uint32_t)span, nullptr};
 }
 
