@@ -9,8 +9,12 @@
 // order: every split of k below is exact and gives the same bits.
 //
 // * Few tokens (skinny): b is read once and straight into registers; the
-//   waves of a block take slices of k and add their sums in LDS.
-// * Tiles: rows of 128 bytes of a and b go through two LDS buffers in turn.
+//   waves of a block take slices of k and add their sums in LDS.  The reading of
+//   b bounds it: 1 x 4096 x 4096 takes 5.4 us, 3.1 TB/s with the launch.
+// * Tiles: rows of 128 bytes of a and b go through LDS buffers in turn.  The
+//   matrix instructions bound large products, 8192 x 8192 x 8192 in 481 us, 2.29
+//   PetaOP/s; the reading of b bounds a few tokens more than a skinny one takes,
+//   64 x 8192 x 8192 in 15.5 us, 4.4 TB/s.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 
@@ -318,10 +322,16 @@ hx_status launch_tiles(const MatmulArgs &p, hipStream_t stream) {
 
 // The largest tile of which there are enough for the 256 CUs: a smaller tile
 // moves more bytes to the same CUs.  Where there are more tiles than CUs two
-// blocks share one, with LDS for half the steps in flight.  Groups that share a
+// blocks share one, with LDS for half the steps in flight.  A last round of the
+// largest tiles that leaves most CUs idle costs more than they gain: two blocks
+// of 128 x 128 on each CU take 0.54 of the time of one of 256 x 256.  Groups that share a
 // block's k keep more loads under way in a block, for about 2 us to add their
 // sums: worth it for long rows, or where tiles are too few to fill the card.
 // Measured (us):
+//   8192 x 8192 x 1024   256 x 256 123     128 x 128 143
+//   831 x 14912 x 1792   256 x 256 39.5    128 x 128 41.4
+//   6144 x 6144 x 6144   256 x 256 280     128 x 128 253     (2.25 rounds, 4.5)
+//   1308 x 11648 x 2624  256 x 256 83.9    128 x 128 48.4    (1.08 rounds, 1.96)
 //   1000 x 8192 x 8192   128 x 128 71.1    64 x 64 109     256 x 256 115
 //   2048 x 2048 x 2048   128 x 128 16.6    64 x 64 19.0    256 x 256 37.8
 //   1500 x 1500 x 8192    96 x  96 28.6    64 x 64 39.2
@@ -333,7 +343,9 @@ template <typename T> hx_status launch_tiled(const MatmulArgs &p, hipStream_t st
     const auto tiles = [&](uint64_t bm, uint64_t bn) { return ceil_div(p.m, bm) * ceil_div(p.n, bn); };
     constexpr uint64_t kCus = 256, kEnough = 160, kFull = 192;
     const bool long_rows = p.k >= 4096;
-    if (tiles(256, 256) >= kEnough) return launch_tiles<T, 256, 256, 2, 4, 1, 2>(p, stream);
+    const uint64_t rounds = ceil_div(tiles(256, 256), kCus), pairs = ceil_div(tiles(128, 128), 2 * kCus);
+    if (tiles(256, 256) >= kEnough && rounds <= 0.54 * pairs)
+        return launch_tiles<T, 256, 256, 2, 4, 1, 2>(p, stream);
     if (tiles(128, 128) > kCus) return launch_tiles<T, 128, 128, 2, 2, 1, 2>(p, stream);
     if (tiles(128, 128) >= kFull) return launch_tiles<T, 128, 128, 2, 4, 1, 4>(p, stream);
     if (long_rows && tiles(96, 96) >= kFull && tiles(96, 96) <= kCus)
