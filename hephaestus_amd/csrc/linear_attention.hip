@@ -150,6 +150,14 @@ template <typename T> hx_status launch_steps(const AttentionArgs &a, hipStream_t
 // columns of v a wave; each wave keeps its columns of S, in f32, in the
 // accumulators of the last product, for the whole prompt.
 //
+// What bounds a block of bf16 is LDS: every wave reads all of q and k, about 4000
+// of a chunk's 9000 cycles at 64 tokens of 128 x 128, and then the arithmetic of
+// the three terms (below).  8 x 32 heads of 128 x 128 over 4096 tokens take 272
+// us, 1.1 GB at 4.1 TB/s; loads and stores alone took 230.  Chunks of 128 tokens
+// have no room beside the next one.  In f32 the matrix instructions weigh most, at
+// a sixteenth of the rate of bf16: half of the 6.3 us of a chunk of 32 tokens of
+// 80 x 96 (5 x 12 heads, up to 1000 tokens: 51 us, and 24 for the parts' sums).
+//
 // The accumulators of a 16 x 16 product hold, in lane l, column l % 16 and rows
 // 4·(l / 16) + i.  An operand holds, in lane l, row or column l % 16 and the
 // terms 4·(l / 16) + i of a run of 16.  So what one product leaves is an operand
@@ -748,35 +756,47 @@ __global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArg
             if (to && state_row<T>(i, e) < dk) to[state_row<T>(i, e) * stride] = s[i][e];
 }
 
-// The state before each part, from the parts' own sums: one element of the
-// state a thread, the parts in order, eight of them loaded together.
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Parts parts) {
-    const uint32_t n = (uint32_t)(a.dk * a.dv), i = blockIdx.x * 256 + threadIdx.x;
+// The state before each part, from the parts' own sums: V elements of a row of
+// the state a thread, the parts in order, sixteen of them loaded together.  V is 4
+// where rows are whole fours: 2 x 32 heads of 128 x 128 in four parts take 8.4 us
+// so, 12.3 with one element a thread.
+template <int V> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Parts parts) {
+    typedef float Values __attribute__((ext_vector_type(V), aligned(4)));
+    const uint32_t n = (uint32_t)(a.dk * a.dv), i = (blockIdx.x * 256 + threadIdx.x) * V;
     if (i >= n) return;
     const uint32_t h = blockIdx.y, b = blockIdx.z, row = i / (uint32_t)a.dv, col = i % (uint32_t)a.dv;
     const uint32_t tokens = (uint32_t)a.tokens, length = a.lengths ? min(a.lengths[b], tokens) : tokens;
+    float *at = parts.states + ((uint64_t)b * a.heads + h) * parts.parts * n + i;
+    constexpr uint32_t kBatch = 16;
+    Values own[kBatch] = {};
+    const auto load = [&](uint32_t p) {
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+            if (p + k < parts.parts) own[k] = *(const Values *)(at + (uint64_t)(p + k) * n);
+    };
+    load(0);
+    Values s = {};
+    if (a.state_in) s = *(const Values *)(a.state_in + b * a.si.batch + h * a.si.head + row * a.si.token + col);
     const double log_decay = a.log_decay[h];
     // Every part but the last with tokens is whole, and those behind it have none.
     const uint32_t whole = length / parts.span, rest = length % parts.span;
     const double of_whole = exp(log_decay * parts.span), of_rest = rest ? exp(log_decay * rest) : 1.0;
     const float whole_high = (float)of_whole, whole_low = (float)(of_whole - whole_high);
     const float rest_high = (float)of_rest, rest_low = (float)(of_rest - rest_high);
-    float s = a.state_in ? a.state_in[b * a.si.batch + h * a.si.head + row * a.si.token + col] : 0.0f;
-    float *at = parts.states + ((uint64_t)b * a.heads + h) * parts.parts * n + i;
-    constexpr uint32_t kBatch = 8;
-    for (uint32_t p = 0; p < parts.parts; p += kBatch, at += (uint64_t)kBatch * n) {
-        float own[kBatch];
-#pragma unroll
-        for (uint32_t k = 0; k < kBatch; ++k) own[k] = p + k < parts.parts ? at[(uint64_t)k * n] : 0.0f;
+    for (uint32_t p = 0;;) {
 #pragma unroll
         for (uint32_t k = 0; k < kBatch; ++k) {
             if (p + k >= parts.parts) break;
-            at[(uint64_t)k * n] = s;
-            if (p + k < whole) s = fmaf(s, whole_high, s * whole_low) + own[k];
-            else if (p + k == whole) s = fmaf(s, rest_high, s * rest_low) + own[k];
+            *(Values *)(at + (uint64_t)(p + k) * n) = s;
+            if (p + k > whole) continue;
+            const float high = p + k < whole ? whole_high : rest_high, low = p + k < whole ? whole_low : rest_low;
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] = fmaf(s[e], high, s[e] * low) + own[k][e];
         }
+        if ((p += kBatch) >= parts.parts) break;
+        load(p);
     }
-    if (a.state_out) a.state_out[b * a.st.batch + h * a.st.head + row * a.st.token + col] = s;
+    if (a.state_out) *(Values *)(a.state_out + b * a.st.batch + h * a.st.head + row * a.st.token + col) = s;
 }
 
 // Waves a block, each with 16 columns of v: with wider keys than 128, two chunks
@@ -792,12 +812,13 @@ uint32_t block_waves(const AttentionArgs &a) { return a.dv <= 64 || a.dk > 128 ?
 //   1 x  8 x 512,           8 parts   21, uncut  32
 //   4 x 16 x 512,           4 parts   39, uncut  35
 //   2 x 64 x 4096 of 64 x 64, 4 parts 115, 2 parts 148, uncut 184
+//   2 x 64 x 512, the same in f32, 4 parts 48, 2 parts 54
 Parts parts_of(const AttentionArgs &a) {
     const bool f32 = a.dtype == HX_DTYPE_F32;
     const uint64_t chunk = f32 ? 32 : 64, chunks = ceil_div(a.tokens, chunk);
     const uint64_t blocks = a.batch * a.heads * ceil_div(a.dv, 16 * block_waves(a));
     // Blocks of the narrowest heads take half a CU's LDS.
-    const uint64_t card = a.dk <= 64 && a.dv <= 64 && !f32 ? 512 : 256;
+    const uint64_t card = a.dk <= 64 && a.dv <= 64 ? 512 : 256;
     const double area = (double)(a.dk * a.dv) / (128 * 128), chunk_us = 2.4 + (f32 ? 3.8 : 2.3) * area;
     uint64_t best = 1;
     double best_us = chunks * chunk_us;
@@ -829,9 +850,10 @@ hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
     };
     if (parts.parts > 1) {
         HX_TRY(run(std::false_type{}));
-        hipLaunchKernelGGL(attention_join_kernel,
-                           dim3((uint32_t)ceil_div(a.dk * a.dv, 256), (uint32_t)a.heads, (uint32_t)a.batch), dim3(256),
-                           0, stream, a, parts);
+        const uint32_t wide = a.dv % 4 == 0 ? 4 : 1;
+        hipLaunchKernelGGL(wide == 4 ? attention_join_kernel<4> : attention_join_kernel<1>,
+                           dim3((uint32_t)ceil_div(a.dk * a.dv, 256 * wide), (uint32_t)a.heads, (uint32_t)a.batch),
+                           dim3(256), 0, stream, a, parts);
         HX_TRY(check_launch("attention_join_kernel"));
     }
     return run(std::true_type{});
