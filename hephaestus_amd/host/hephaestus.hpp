@@ -13,6 +13,8 @@
 //   DeviceApi / LaunchGeometry                crates/hephaestus-core/src/domain/accelerator/device_api.rs:10-133
 //   ComputeDeviceCapabilities / limits        crates/hephaestus-core/src/domain/device.rs:38-80,225-238
 //   HephaestusError                           crates/hephaestus-core/src/domain/error.rs:8-58
+// RocmNormOps, RocmMatrixOps and RocmLinearAttentionOps, the operators of a
+// linear-attention layer served in 8 bits, have no counterpart there.
 // Errors are thrown as hephaestus::Error carrying the variant and the
 // native message; every entry point validates before it writes, so a
 // thrown call leaves its outputs untouched.  Header-only; link
@@ -23,10 +25,12 @@
 
 #include <array>
 #include <cstdint>
+#include <cstring>
 #include <exception>
 #include <functional>
 #include <initializer_list>
 #include <memory>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -72,6 +76,26 @@ template <typename T> struct Scalar;
 template <> struct Scalar<float> { static constexpr hx_dtype dtype = HX_DTYPE_F32; };
 template <> struct Scalar<uint32_t> { static constexpr hx_dtype dtype = HX_DTYPE_U32; };
 template <> struct Scalar<int32_t> { static constexpr hx_dtype dtype = HX_DTYPE_I32; };
+
+// bfloat16 elements of the layer operators' buffers.
+struct Bfloat16 {
+    uint16_t bits = 0;
+    Bfloat16() = default;
+    // Rounded to nearest, ties to even; a NaN stays one.
+    explicit Bfloat16(float value) {
+        uint32_t b;
+        std::memcpy(&b, &value, 4);
+        bits = static_cast<uint16_t>((b & 0x7FFFFFFFu) > 0x7F800000u ? (b >> 16) | 0x40u
+                                                                     : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
+    }
+    explicit operator float() const {
+        const uint32_t b = static_cast<uint32_t>(bits) << 16;
+        float value;
+        std::memcpy(&value, &b, 4);
+        return value;
+    }
+};
+template <> struct Scalar<Bfloat16> { static constexpr hx_dtype dtype = HX_DTYPE_BF16; };
 
 // ------------------------------------------------------- operator markers
 // core ops.rs:735-803 (SumOp ... CumProdOp); MeanOp and ArgMaxOp select the
@@ -640,6 +664,120 @@ class RocmDenseVectorOps {
                                     b ? b->device_ptr() : nullptr, b ? b->len() : 0, b ? la.raw() : nullptr,
                                     out.device_ptr(), 1, &plan));
         return Prepared{PreparedPlan(plan), std::move(out), a.device_ptr(), b ? b->device_ptr() : nullptr};
+    }
+};
+
+// ------------------------------------------------------- layer operators
+// The formulas and rules stand at hx_rms_norm_quantize, hx_matmul_i8 and
+// hx_linear_attention.  T is float or Bfloat16; an operand left out is nullopt.
+namespace detail {
+template <typename T> struct Same { using type = T; }; // T is not deduced from an operand that may be left out
+} // namespace detail
+template <typename T> using OptionalView = std::optional<StridedView<typename detail::Same<T>::type>>;
+
+namespace detail {
+// A view as the C ABI takes it: allocation, its length, layout.
+template <typename T> struct Operand {
+    T *ptr = nullptr;
+    uint64_t len = 0;
+    const hx_layout *layout = nullptr;
+    Operand(const StridedView<T> &v) : ptr(v.buffer.device_ptr()), len(v.buffer.len()), layout(v.layout.raw()) {}
+    Operand(const std::optional<StridedView<T>> &v) {
+        if (v) *this = Operand(*v);
+    }
+};
+} // namespace detail
+
+class RocmNormOps {
+  public:
+    template <typename T>
+    void rms_norm_quantize_into(RocmDevice &dev, StridedView<T> x, const RocmBuffer<T> &weight, float epsilon,
+                                StridedView<int8_t> quantized, RocmBuffer<float> &scales,
+                                OptionalView<T> residual = {}, OptionalView<T> residual_out = {},
+                                hx_stream stream = nullptr) const {
+        call(hx_rms_norm_quantize, dev, x, weight, epsilon, quantized, scales, residual, residual_out, stream);
+    }
+    template <typename T>
+    PreparedPlan prepare_rms_norm_quantize(RocmDevice &dev, StridedView<T> x, const RocmBuffer<T> &weight,
+                                           float epsilon, StridedView<int8_t> quantized, RocmBuffer<float> &scales,
+                                           OptionalView<T> residual = {}, OptionalView<T> residual_out = {}) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_rms_norm_quantize, dev, x, weight, epsilon, quantized, scales, residual, residual_out, &plan);
+        return PreparedPlan(plan);
+    }
+
+  private:
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const StridedView<T> &x, const RocmBuffer<T> &weight, float epsilon,
+              const StridedView<int8_t> &quantized, RocmBuffer<float> &scales, const OptionalView<T> &residual,
+              const OptionalView<T> &residual_out, Last last) const {
+        const detail::Operand<T> ox(x), ores(residual), oout(residual_out);
+        const detail::Operand<int8_t> oq(quantized);
+        check(f(dev.raw(), Scalar<T>::dtype, ox.ptr, ox.len, ox.layout, ores.ptr, ores.len, ores.layout,
+                weight.device_ptr(), weight.len(), epsilon, oout.ptr, oout.len, oout.layout, oq.ptr, oq.len, oq.layout,
+                scales.device_ptr(), scales.len(), last));
+    }
+};
+
+class RocmMatrixOps {
+  public:
+    template <typename T>
+    void matmul_i8_into(RocmDevice &dev, StridedView<int8_t> a, const RocmBuffer<float> &a_scales,
+                        StridedView<int8_t> b, const RocmBuffer<float> &b_scales, StridedView<T> out,
+                        hx_stream stream = nullptr) const {
+        call(hx_matmul_i8, dev, a, a_scales, b, b_scales, out, stream);
+    }
+    template <typename T>
+    PreparedPlan prepare_matmul_i8(RocmDevice &dev, StridedView<int8_t> a, const RocmBuffer<float> &a_scales,
+                                   StridedView<int8_t> b, const RocmBuffer<float> &b_scales, StridedView<T> out) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_matmul_i8, dev, a, a_scales, b, b_scales, out, &plan);
+        return PreparedPlan(plan);
+    }
+
+  private:
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const StridedView<int8_t> &a, const RocmBuffer<float> &a_scales,
+              const StridedView<int8_t> &b, const RocmBuffer<float> &b_scales, const StridedView<T> &out,
+              Last last) const {
+        const detail::Operand<int8_t> oa(a), ob(b);
+        const detail::Operand<T> oo(out);
+        check(f(dev.raw(), oa.ptr, oa.len, oa.layout, a_scales.device_ptr(), a_scales.len(), ob.ptr, ob.len, ob.layout,
+                b_scales.device_ptr(), b_scales.len(), Scalar<T>::dtype, oo.ptr, oo.len, oo.layout, last));
+    }
+};
+
+class RocmLinearAttentionOps {
+  public:
+    template <typename T>
+    void linear_attention_into(RocmDevice &dev, StridedView<T> q, StridedView<T> k, StridedView<T> v,
+                               const RocmBuffer<float> &log_decay, StridedView<T> out, float scale,
+                               OptionalView<float> state_in = {}, OptionalView<float> state_out = {},
+                               const RocmBuffer<uint32_t> *lengths = nullptr, hx_stream stream = nullptr) const {
+        call(hx_linear_attention, dev, q, k, v, log_decay, out, scale, state_in, state_out, lengths, stream);
+    }
+    template <typename T>
+    PreparedPlan prepare_linear_attention(RocmDevice &dev, StridedView<T> q, StridedView<T> k, StridedView<T> v,
+                                          const RocmBuffer<float> &log_decay, StridedView<T> out, float scale,
+                                          OptionalView<float> state_in = {}, OptionalView<float> state_out = {},
+                                          const RocmBuffer<uint32_t> *lengths = nullptr) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_linear_attention, dev, q, k, v, log_decay, out, scale, state_in, state_out, lengths, &plan);
+        return PreparedPlan(plan);
+    }
+
+  private:
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const StridedView<T> &q, const StridedView<T> &k, const StridedView<T> &v,
+              const RocmBuffer<float> &log_decay, const StridedView<T> &out, float scale,
+              const OptionalView<float> &state_in, const OptionalView<float> &state_out,
+              const RocmBuffer<uint32_t> *lengths, Last last) const {
+        const detail::Operand<T> oq(q), ok(k), ov(v), oo(out);
+        const detail::Operand<float> si(state_in), so(state_out);
+        check(f(dev.raw(), Scalar<T>::dtype, oq.ptr, oq.len, oq.layout, ok.ptr, ok.len, ok.layout, ov.ptr, ov.len,
+                ov.layout, log_decay.device_ptr(), log_decay.len(), scale, si.ptr, si.len, si.layout, so.ptr, so.len,
+                so.layout, lengths ? lengths->device_ptr() : nullptr, lengths ? lengths->len() : 0, oo.ptr, oo.len,
+                oo.layout, last));
     }
 };
 
