@@ -459,12 +459,15 @@ template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT> struct Chunk {
     static constexpr int S = DIRECT && 3 * kStage + kScores <= 160 * 1024 ? 3 : 2;
     static constexpr int kLds = S * kStage + kScores;
     static_assert(kLds <= 160 * 1024);
+    // Where LDS holds two blocks of four waves, so must the registers: 1 x 50 heads of
+    // 37 x 53 over 4096 tokens take 146 us with one block a CU, 98 with two.
+    static constexpr int kWavesPerSimd = NW == 4 && 2 * kLds <= 160 * 1024 ? 2 : NW / 4;
 };
 
 // OUTPUTS: the outputs of a part, from the state before it.  Otherwise only the
 // part's own sum, from nothing.
 template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT>
-__global__ __launch_bounds__(NW *kWave) void attention_chunk_kernel(AttentionArgs a, Parts parts) {
+__global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWavesPerSimd)) void attention_chunk_kernel(AttentionArgs a, Parts parts) {
     using G = Chunk<T, DK, NW, OUTPUTS, DIRECT>;
     using F = typename Fragment<T>::type;
     constexpr int C = G::C, B = G::B, S = G::S, WK = G::WK, DV = G::DV;
