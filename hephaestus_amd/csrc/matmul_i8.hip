@@ -33,10 +33,16 @@ __device__ __forceinline__ i32x4v mma(i32x4v b, i32x4v a, i32x4v sum) {
 }
 
 // 16 bytes of a row from `k` on, zeros from `end` on.  Global memory takes
-// vectors at any byte address.
+// vectors at any byte address.  The last bytes of a row come as the sixteen that
+// end it: read one by one they cost a wait each.
 __device__ __forceinline__ i32x4v load_bytes(const int8_t *row, uint32_t k, uint32_t end) {
     if (k + 16 <= end) return __builtin_bit_cast(i32x4v, (u32x4)*(const u32x4_any *)(row + k));
     i32x4v v = {0, 0, 0, 0};
+    if (k >= end) return v;
+    if (end >= 16) {
+        const u32x4 last = *(const u32x4_any *)(row + end - 16);
+        return __builtin_bit_cast(i32x4v, __builtin_bit_cast(unsigned __int128, last) >> (8 * (k + 16 - end)));
+    }
     for (uint32_t i = 0; k + i < end; ++i) v[i / 4] |= (int)((uint32_t)(uint8_t)row[k + i] << (8 * (i % 4)));
     return v;
 }
