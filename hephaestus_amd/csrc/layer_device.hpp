@@ -19,6 +19,28 @@ template <> struct Pack16<bf16> { static constexpr int N = 8; };
 
 __device__ __forceinline__ u32x4 load_raw(const float *p) { return *(const u32x4_a4 *)p; }
 __device__ __forceinline__ u32x4 load_raw(const bf16 *p) { return *(const u32x4_a2 *)p; }
+// 16 bytes of a row of `width` elements from element c on, zeros past its end, in
+// two steps, so that nothing waits for them before all loads are under way: the
+// last, partial vector is loaded as the sixteen bytes that end the row, and
+// shifted when it is used.  Element by element it would cost a wait each.
+template <typename T> __device__ __forceinline__ u32x4 load_part(const T *row, uint32_t c, uint32_t width) {
+    constexpr uint32_t N = Pack16<T>::N;
+    u32x4 v = {0, 0, 0, 0};
+    if (width >= N) {
+        if (c < width) v = load_raw(row + min(c, width - N));
+    } else if (c == 0) {
+        T part[N];
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) part[i] = i < width ? row[i] : (T)0.0f;
+        __builtin_memcpy(&v, part, 16);
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ u32x4 place_part(u32x4 v, uint32_t c, uint32_t width) {
+    constexpr uint32_t N = Pack16<T>::N;
+    if (width < N || c >= width || c + N <= width) return v;
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (8 * sizeof(T) * (c + N - width)));
+}
 // f32 values of 16 bytes of elements.
 template <typename T, int N> __device__ __forceinline__ void unpack(u32x4 v, float (&x)[N]) {
     static_assert(N == Pack16<T>::N);

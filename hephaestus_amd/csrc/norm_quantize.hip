@@ -10,8 +10,9 @@
 //
 // Memory bounds long inputs: 16384 x 8192 bf16 with a residual, 940 MB, takes
 // 156 us, 6.0 TB/s.  One row of 4096 takes 2.7 us, a launch and one wait for
-// memory.  Rows of f32 at an odd width begin on any dword: 1000 x 5001 takes
-// 9.8 us, 2.6 TB/s, where the vectors of a row cross the 128-byte lines.
+// memory.  Rows of odd width begin anywhere and end in part of a vector: 1000 x 5001
+// f32 takes 8.8 us, 2.8 TB/s, and 6932 x 9681 bf16 115 us, 4.1 TB/s, where vectors
+// cross the 128-byte lines.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 
@@ -68,21 +69,6 @@ template <int WAVES> __device__ __forceinline__ void combine_waves(float &sum, u
     }
 }
 
-// The 16 bytes at column c, zeros past the row's end: as loaded, so that nothing
-// waits for them before all of a row's loads are under way.
-template <typename T> __device__ __forceinline__ u32x4 load_row(const T *p, uint32_t c, uint32_t cols) {
-    constexpr uint32_t N = Pack16<T>::N;
-    if (c + N <= cols) return load_raw(p + c);
-    u32x4 v = {0, 0, 0, 0};
-    if (c < cols) {
-        T part[N];
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) part[i] = c + i < cols ? p[c + i] : (T)0.0f;
-        __builtin_memcpy(&v, part, 16);
-    }
-    return v;
-}
-
 template <typename T, int N>
 __device__ __forceinline__ void store_row(T *p, uint32_t c, uint32_t cols, const float (&x)[N]) {
     if (c + N <= cols) {
@@ -130,10 +116,18 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows_kernel(No
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const uint32_t c = ((uint32_t)s * LANES + lane) * N;
-        vx[s] = load_row(x, c, cols);
+        vx[s] = load_part(x, c, cols);
         vr[s] = u32x4{0, 0, 0, 0};
-        if (a.residual) vr[s] = load_row(res, c, cols);
-        vw[s] = load_row(w, c, cols);
+        if (a.residual) vr[s] = load_part(res, c, cols);
+        vw[s] = load_part(w, c, cols);
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const uint32_t c = ((uint32_t)s * LANES + lane) * N;
+        if (c + N <= cols) continue;
+        vx[s] = place_part<T>(vx[s], c, cols);
+        if (a.residual) vr[s] = place_part<T>(vr[s], c, cols);
+        vw[s] = place_part<T>(vw[s], c, cols);
     }
     // h and h·w of a vector, from the registers it was loaded into.
     const auto values = [&](int s, float(&h)[N], float(&hw)[N]) {
@@ -188,14 +182,17 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_long_rows_ker
     T *ho = (T *)a.residual_out + (int64_t)row * a.residual_out_stride;
     int8_t *q = a.quantized + (int64_t)row * a.quantized_stride;
     const auto sweep = [&](uint32_t c, float (&h)[N], float (&hw)[N]) {
-        unpack<T>(load_row(x, c, cols), h);
+        const u32x4 vx = load_part(x, c, cols), vw = load_part(w, c, cols);
+        u32x4 vr = {0, 0, 0, 0};
+        if (a.residual) vr = load_part(res, c, cols);
+        unpack<T>(place_part<T>(vx, c, cols), h);
         if (a.residual) {
             float r[N];
-            unpack<T>(load_row(res, c, cols), r);
+            unpack<T>(place_part<T>(vr, c, cols), r);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] += r[i];
         }
-        unpack<T>(load_row(w, c, cols), hw);
+        unpack<T>(place_part<T>(vw, c, cols), hw);
 #pragma unroll
         for (int i = 0; i < N; ++i) hw[i] *= h[i];
     };
