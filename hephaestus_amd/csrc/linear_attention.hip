@@ -414,24 +414,18 @@ template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIREC
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t row = row_of(threadIdx.x, i), c = slot_of(threadIdx.x, i) * V;
-            const T *p = base + (int64_t)row * stride + c;
             if constexpr (!DIRECT) {
                 held[i] = u32x4{0, 0, 0, 0};
-                if (row < rows && c + V <= width) {
-                    held[i] = *(const Vec *)p;
-                } else if (row < rows) {
-                    T part[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) part[e] = c + e < width ? p[e] : (T)0.0f;
-                    __builtin_memcpy(&held[i], part, 16);
-                }
+                if (row < rows) held[i] = load_part(base + (int64_t)row * stride, c, width);
             }
         }
     }
-    __device__ __forceinline__ void store(char *tile) const {
+    __device__ __forceinline__ void store(char *tile, uint32_t width) const {
         if constexpr (!DIRECT)
 #pragma unroll
-            for (int i = 0; i < N; ++i) *(u32x4 *)(tile + (threadIdx.x + i * THREADS) * 16) = held[i];
+            for (int i = 0; i < N; ++i)
+                *(u32x4 *)(tile + (threadIdx.x + i * THREADS) * 16) =
+                    place_part<T>(held[i], slot_of(threadIdx.x, i) * V, width);
     }
 };
 
@@ -460,8 +454,9 @@ template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT> struct Chunk {
     static constexpr int kLds = S * kStage + kScores;
     static_assert(kLds <= 160 * 1024);
     // Where LDS holds two blocks of four waves, so must the registers: 1 x 50 heads of
-    // 37 x 53 over 4096 tokens take 146 us with one block a CU, 98 with two.
-    static constexpr int kWavesPerSimd = NW == 4 && 2 * kLds <= 160 * 1024 ? 2 : NW / 4;
+    // 37 x 53 over 4096 tokens take 84 us with one block a CU, 65 with two.  (At dk of
+    // 256 they would spill.)
+    static constexpr int kWavesPerSimd = NW == 4 && DK <= 128 && 2 * kLds <= 160 * 1024 ? 2 : NW / 4;
 };
 
 // OUTPUTS: the outputs of a part, from the state before it.  Otherwise only the
@@ -538,9 +533,9 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
     };
     const auto settle = [&](uint32_t n) { // what went through registers
         char *stage = stage_of(n);
-        to_k.store(stage);
-        to_v.store(stage + G::kTileK);
-        if constexpr (OUTPUTS) to_q.store(stage + G::kTileK + G::kTileV);
+        to_k.store(stage, dk);
+        to_v.store(stage + G::kTileK, dv);
+        if constexpr (OUTPUTS) to_q.store(stage + G::kTileK + G::kTileV, dk);
     };
     if constexpr (DIRECT) {
         for (uint32_t n = 0; n < S - 1 && n < chunks; ++n) fetch(n);
