@@ -6,9 +6,10 @@
 // head's state in registers, eight lanes of four columns by 32 groups of rows,
 // and steps through the tokens.  Each step is a rank-1 update of the lane's own
 // elements and a sum over the rows: within the wave by lane exchange, across the
-// four waves through LDS (two buffers in turn, so one barrier a token).  The
-// state's bytes, in and out, bound it: 128 sequences of 32 heads of 128 x 128
-// take 97 us, 5.5 TB/s.  Blocks of 64 or 128 columns, with whole rows of the
+// four waves through LDS (two buffers in turn, so one barrier a token); the next
+// token's elements are on their way meanwhile.  The state's bytes, in and out,
+// bound it: 128 sequences of 32 heads of 128 x 128 take 98 us, 5.5 TB/s; 50 of 4
+// heads of 256 x 128 10.8.  Blocks of 64 or 128 columns, with whole rows of the
 // state side by side but more registers, took 154 and 95 us, and for one
 // sequence of 16 heads 6.3 and 6.8 us against 4.7.
 //
@@ -23,44 +24,59 @@
 namespace hx {
 namespace {
 
-// Four columns of a row from column c on.  VEC: the rows are 16-byte aligned
-// and the width a multiple of four.  NT: streamed, not kept in the caches.
-template <bool VEC, bool NT> __device__ __forceinline__ f32x4 load4(const float *row, uint32_t c, uint32_t width) {
-    if constexpr (VEC) return c < width ? load_vec<NT>((const f32x4 *)(row + c)) : f32x4{0, 0, 0, 0};
-    f32x4 v = {0, 0, 0, 0};
+// N neighbours of a row of T, in two steps, so that nothing waits for them before
+// all loads are under way: where the row ends among them the N that end it are
+// loaded, and shifted when they are used.  Past the row's end anything may come.
+template <int N, typename T> struct RunOf {
+    typedef T type __attribute__((ext_vector_type(N)));
+    typedef T loaded __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <int N, typename T>
+__device__ __forceinline__ typename RunOf<N, T>::type load_run(const T *p, uint32_t from, uint32_t end) {
+    if (end >= N) return *(const typename RunOf<N, T>::loaded *)(p + min(from, end - N));
+    typename RunOf<N, T>::type x = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (c + i < width) v[i] = row[c + i];
-    return v;
+    for (int i = 0; i < N; ++i)
+        if (from + i < end) x[i] = p[from + i];
+    return x;
 }
-template <bool VEC, bool NT> __device__ __forceinline__ void store4(float *row, uint32_t c, uint32_t width, f32x4 v) {
-    if constexpr (VEC) {
-        if (c < width) store_vec<NT>(v, (f32x4 *)(row + c));
+template <int N, typename V> __device__ __forceinline__ V place_run(V x, uint32_t from, uint32_t end) {
+    if (from + N <= end || end < N) return x;
+    const uint32_t by = from + N - end;
+#pragma unroll
+    for (int d = 1; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i + 1 < N; ++i) x[i] = by >= (uint32_t)d ? x[i + 1] : x[i];
+    return x;
+}
+
+// Four columns of a row of the state from column c on, at any dword.  NT:
+// streamed, not kept in the caches.
+template <bool NT> __device__ __forceinline__ f32x4 load4(const float *row, uint32_t c, uint32_t width) {
+    if (width < 4) return load_run<4>(row, c, width);
+    return load_a4<NT>((const f32x4_a4 *)(row + min(c, width - 4)));
+}
+template <bool NT> __device__ __forceinline__ void store4(float *row, uint32_t c, uint32_t width, f32x4 v) {
+    if (c + 4 <= width) {
+        store_a4<NT>(v, (f32x4_a4 *)(row + c));
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (c + i < width) row[c + i] = v[i];
 }
-// N neighbours of a row of T in f32, zeros past its end.
-template <int N, typename T> __device__ __forceinline__ void load_run(const T *p, uint32_t from, uint32_t end, float (&x)[N]) {
-    if (from + N <= end) {
-        typedef T Run __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-        const Run v = *(const Run *)(p + from);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = (float)v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = from + i < end ? (float)p[from + i] : 0.0f;
-    }
-}
+
+// All of the wave's LDS reads and writes have ended when it passes; loads from
+// memory may be under way.
+__device__ __forceinline__ void meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 constexpr uint64_t kStreamedBytes = 64ull << 20;
 
 // A block takes COLUMNS columns of a state, four a lane, and all its rows, ROWS
-// neighbours a lane: dk at most ROWS·1024 / COLUMNS.
-template <typename T, int COLUMNS, int ROWS, bool VEC, bool NT>
-__global__ __launch_bounds__(256) void attention_step_kernel(AttentionArgs a) {
+// neighbours a lane: dk at most ROWS·1024 / COLUMNS.  Held to four waves a SIMD: eight
+// rows a lane took 268 registers and 30 us for 50 x 4 heads of 256 x 128, 10.8 so.
+template <typename T, int COLUMNS, int ROWS, bool NT>
+__global__ __launch_bounds__(256, 4) void attention_step_kernel(AttentionArgs a) {
     constexpr int kLanes = COLUMNS / 4; // of a row
     __shared__ f32x4 part[2][4][kLanes];
     const uint32_t h = blockIdx.y, b = blockIdx.z, hk = (uint32_t)(h / (a.heads / a.kv_heads));
@@ -78,28 +94,39 @@ __global__ __launch_bounds__(256) void attention_step_kernel(AttentionArgs a) {
     for (int r = 0; r < ROWS; ++r) {
         s[r] = f32x4{0, 0, 0, 0};
         if (a.state_in && row0 + r < dk)
-            s[r] = load4<VEC, NT>(a.state_in + b * a.si.batch + h * a.si.head + (row0 + r) * a.si.token, c, dv);
+            s[r] = load4<NT>(a.state_in + b * a.si.batch + h * a.si.head + (row0 + r) * a.si.token, c, dv);
     }
+    typename RunOf<4, T>::type vt = {};
+    typename RunOf<ROWS, T>::type kt = {}, qt = {};
+    const auto load = [&](uint64_t t) { // a token's elements, under way while the last one's output is summed
+        vt = load_run<4>(v + (int64_t)t * a.sv.token, c, dv);
+        kt = load_run<ROWS>(k + (int64_t)t * a.sk.token, row0, dk);
+        qt = load_run<ROWS>(q + (int64_t)t * a.sq.token, row0, dk);
+    };
+    if (length) load(0);
+    if (c + 4 > dv)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) s[r] = place_run<4>(s[r], c, dv);
     for (uint64_t t = 0; t < length; ++t) {
-        float vt[4], kt[ROWS], qt[ROWS];
-        load_run<4>(v + (int64_t)t * a.sv.token, c, dv, vt);
-        load_run<ROWS>(k + (int64_t)t * a.sk.token, row0, dk, kt);
-        load_run<ROWS>(q + (int64_t)t * a.sq.token, row0, dk, qt);
-        const f32x4 values = {vt[0], vt[1], vt[2], vt[3]};
+        vt = place_run<4>(vt, c, dv);
+        kt = place_run<ROWS>(kt, row0, dk);
+        qt = place_run<ROWS>(qt, row0, dk);
+        const f32x4 values = {(float)vt[0], (float)vt[1], (float)vt[2], (float)vt[3]};
         f32x4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            s[r] = decay * s[r] + kt[r] * values;
+            s[r] = decay * s[r] + (float)kt[r] * values;
             // A row past dk adds nothing, whatever the value.
-            if (row0 + r < dk) o += qt[r] * s[r];
+            if (row0 + r < dk) o += (float)qt[r] * s[r];
         }
+        if (t + 1 < length) load(t + 1);
 #pragma unroll
         for (int d = kLanes; d < kWave; d *= 2)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d);
         f32x4(*buffer)[kLanes] = part[t & 1];
         if (lane_id() < kLanes) buffer[wave][lane_id()] = o;
-        __syncthreads();
+        meet_lds();
         if (threadIdx.x < kLanes) {
             o = (buffer[0][threadIdx.x] + buffer[1][threadIdx.x]) + (buffer[2][threadIdx.x] + buffer[3][threadIdx.x]);
 #pragma unroll
@@ -115,22 +142,15 @@ __global__ __launch_bounds__(256) void attention_step_kernel(AttentionArgs a) {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
         if (row0 + r < dk)
-            store4<VEC, NT>(a.state_out + b * a.st.batch + h * a.st.head + (row0 + r) * a.st.token, c, dv, s[r]);
-}
-
-bool vector_rows(const float *base, const AttentionView &s, uint64_t dv) {
-    return base == nullptr || ((uintptr_t)base % 16 == 0 && dv % 4 == 0 && s.batch % 4 == 0 && s.head % 4 == 0 &&
-                               s.token % 4 == 0);
+            store4<NT>(a.state_out + b * a.st.batch + h * a.st.head + (row0 + r) * a.st.token, c, dv, s[r]);
 }
 
 template <typename T, int COLUMNS, int ROWS> hx_status launch_step(const AttentionArgs &a, hipStream_t stream) {
     const dim3 grid((uint32_t)ceil_div(a.dv, COLUMNS), (uint32_t)a.heads, (uint32_t)a.batch);
-    const bool vec = vector_rows(a.state_in, a.si, a.dv) && vector_rows(a.state_out, a.st, a.dv);
     // States that the caches cannot hold until the next token are streamed.
     const bool nt = a.batch * a.heads * a.dk * a.dv * sizeof(float) > kStreamedBytes;
-    if (vec && nt) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true, true>), grid, dim3(256), 0, stream, a);
-    else if (vec) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true, false>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, false, false>), grid, dim3(256), 0, stream, a);
+    if (nt) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, false>), grid, dim3(256), 0, stream, a);
     return check_launch("attention_step_kernel");
 }
 
@@ -434,7 +454,6 @@ template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIREC
 template <int N> __device__ __forceinline__ void meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
-__device__ __forceinline__ void meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A prompt cut into `parts` of `span` tokens each, a multiple of the chunk.
 struct Parts {
@@ -874,11 +893,15 @@ template <typename T, bool DIRECT> hx_status launch_chunked(const AttentionArgs 
     return block_waves(a) == 4 ? launch_width<T, 4, DIRECT>(a, ws, stream) : launch_width<T, 8, DIRECT>(a, ws, stream);
 }
 
-// Up to 4 tokens (10 in f32, whose matrix instructions are slower) the recurrence
-// is faster: 32 heads of one sequence take 4.9 us for one token and 1.1 us for
-// each more (0.8 in f32), chunks 11 us (14) however few the tokens; 32 sequences
-// 32 us and 5.2 (3.4), chunks 50 (70).
-bool by_chunks(const AttentionArgs &a) { return a.tokens > (a.dtype == HX_DTYPE_F32 ? 10 : 4) && a.dk > 0; }
+// A few tokens go through the recurrence.  Its time grows with each, that of a
+// chunk does not (us, recurrence and chunk):
+//   1 x 32 heads of 128 x 128    4 tokens 6.4, 11.0    8 tokens 9.5, 11.5     10 tokens 11.4, 11.0
+//   32 x 32, the same            34.4, 51.2            48.5, 51.6             55.9, 50.6
+//   32 x 32, the same in f32     37.6, 72.3            12 tokens 64.1, 70.8   16 tokens 77.3, 71.3
+//   8 x 32 heads of 64 x 64      6.5, 8.0              6 tokens 8.2, 8.2      8 tokens 9.9, 8.0
+bool by_chunks(const AttentionArgs &a) {
+    return a.tokens > (a.dk <= 64 ? 6 : a.dtype == HX_DTYPE_F32 ? 12 : 8) && a.dk > 0;
+}
 
 template <typename T> hx_status launch(const AttentionArgs &a, void *ws, hipStream_t stream) {
     if (by_chunks(a)) {
