@@ -8,7 +8,7 @@
 // elements and a sum over the rows: within the wave by lane exchange, across the
 // four waves through LDS (two buffers in turn, so one barrier a token); the next
 // token's elements are on their way meanwhile.  The state's bytes, in and out,
-// bound it: 128 sequences of 32 heads of 128 x 128 take 98 us, 5.5 TB/s; 50 of 4
+// bound it: 128 sequences of 32 heads of 128 x 128 take 97 us, 5.6 TB/s; 50 of 4
 // heads of 256 x 128 10.8.  Blocks of 64 or 128 columns, with whole rows of the
 // state side by side but more registers, took 154 and 95 us, and for one
 // sequence of 16 heads 6.3 and 6.8 us against 4.7.
@@ -73,10 +73,12 @@ __device__ __forceinline__ void meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\
 constexpr uint64_t kStreamedBytes = 64ull << 20;
 
 // A block takes COLUMNS columns of a state, four a lane, and all its rows, ROWS
-// neighbours a lane: dk at most ROWS·1024 / COLUMNS.  Held to four waves a SIMD: eight
-// rows a lane took 268 registers and 30 us for 50 x 4 heads of 256 x 128, 10.8 so.
+// neighbours a lane: dk at most ROWS·1024 / COLUMNS.  Registers for four waves a SIMD:
+// 32 x 32 heads of 64 x 64 take 8.4 us so and 9.8 without the bound, 50 x 4 of 256 x
+// 128 10.8 and 30 (268 registers); streamed states, 128 x 32 heads of 128 x 128,
+// 100 and 96.7, so they go without it up to four rows a lane.
 template <typename T, int COLUMNS, int ROWS, bool NT>
-__global__ __launch_bounds__(256, 4) void attention_step_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_kernel(AttentionArgs a) {
     constexpr int kLanes = COLUMNS / 4; // of a row
     __shared__ f32x4 part[2][4][kLanes];
     const uint32_t h = blockIdx.y, b = blockIdx.z, hk = (uint32_t)(h / (a.heads / a.kv_heads));
