@@ -368,14 +368,17 @@ template <typename T> hx_status launch_tiled(const MatmulArgs &p, hipStream_t st
 
 // ----------------------------------------------------------- rows on dwords
 // Rows of a and b at any byte, copied to rows of whole 128 bytes with zeros
-// after their ends.  Loading such rows through registers in every tile took
-// 29 us for 1000 x 1027 x 4099; the copy and then direct loads take 23.
+// after their ends, sixteen bytes a thread, the rows end to end.  Loading such rows
+// through registers in every tile took 29 us for 1000 x 1027 x 4099; the copy and
+// then direct loads take 23.
 __global__ __launch_bounds__(256) void matmul_align_kernel(MatmulArgs p, int8_t *rows, uint32_t pitch) {
-    const uint32_t chunk = (blockIdx.x * 256 + threadIdx.x) * 16;
-    if (chunk >= pitch) return;
-    for (uint64_t r = blockIdx.y; r < p.m + p.n; r += gridDim.y) {
+    const uint32_t chunks = pitch / 16; // of a row
+    for (uint64_t first = (uint64_t)blockIdx.x * 256; first < (p.m + p.n) * chunks; first += (uint64_t)gridDim.x * 256) {
+        const uint32_t i = (uint32_t)(first % chunks) + threadIdx.x, at = i % chunks * 16;
+        const uint64_t r = first / chunks + i / chunks;
+        if (r >= p.m + p.n) return;
         const int8_t *from = r < p.m ? p.a + (int64_t)r * p.a_stride : p.b + (int64_t)(r - p.m) * p.b_stride;
-        *(i32x4v *)(rows + r * pitch + chunk) = load_bytes(from, chunk, (uint32_t)p.k);
+        *(i32x4v *)(rows + r * pitch + at) = load_bytes(from, at, (uint32_t)p.k);
     }
 }
 
@@ -391,8 +394,8 @@ template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t strea
     if (p.m <= kSkinnyTokens) return launch_skinny<T>(p, stream);
     if (needs_copy(p)) {
         const uint32_t pitch = (uint32_t)copy_pitch(p);
-        const dim3 grid((uint32_t)ceil_div(pitch, 256 * 16), (uint32_t)min(p.m + p.n, (uint64_t)65535));
-        hipLaunchKernelGGL(matmul_align_kernel, grid, dim3(256), 0, stream, p, (int8_t *)ws, pitch);
+        const uint64_t blocks = min(ceil_div((p.m + p.n) * (pitch / 16), 256), (uint64_t)1 << 22);
+        hipLaunchKernelGGL(matmul_align_kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, p, (int8_t *)ws, pitch);
         HX_TRY(check_launch("matmul_align_kernel"));
         p.a = (const int8_t *)ws;
         p.b = p.a + p.m * pitch;

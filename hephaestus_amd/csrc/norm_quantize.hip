@@ -218,12 +218,30 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_long_rows_ker
     }
 }
 
+// The rows from `first` on.
+template <typename T> NormArgs rows_from(NormArgs a, uint64_t first) {
+    const int64_t n = (int64_t)first;
+    a.rows -= first;
+    a.x = (const T *)a.x + n * a.x_stride;
+    if (a.residual) a.residual = (const T *)a.residual + n * a.residual_stride;
+    if (a.residual_out) a.residual_out = (T *)a.residual_out + n * a.residual_out_stride;
+    a.quantized += n * a.quantized_stride;
+    a.scales += n;
+    return a;
+}
+
 template <typename T> hx_status launch(const NormArgs &a, hipStream_t stream) {
     const uint64_t vectors = ceil_div(a.cols, Pack16<T>::N);
+    // A launch has fewer than 2^32 threads: more rows take several.
+    constexpr uint64_t kBlocks = 1 << 21;
     const auto run = [&](auto kernel, uint64_t lanes) {
         const uint64_t rows = lanes <= kWave ? 256 / lanes : 1;
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)ceil_div(a.rows, rows)), dim3((uint32_t)(lanes < 256 ? 256 : lanes)), 0,
-                           stream, a);
+        for (uint64_t first = 0; first < a.rows; first += kBlocks * rows) {
+            NormArgs part = rows_from<T>(a, first);
+            part.rows = min(part.rows, kBlocks * rows);
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)ceil_div(part.rows, rows)),
+                               dim3((uint32_t)(lanes < 256 ? 256 : lanes)), 0, stream, part);
+        }
     };
     // One or two vectors a thread as long as rows allow: a thread that holds
     // more keeps fewer waves on a CU.  Measured (us): 16384 x 128 16 lanes 5.5, 64

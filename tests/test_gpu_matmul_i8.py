@@ -115,3 +115,12 @@ def test_same_bits_every_run(device):
     first = run(device, *ops, np.float32)
     for _ in range(3):
         assert first.tobytes() == run(device, *ops, np.float32, prepared=True).tobytes()
+
+
+@pytest.mark.parametrize("k", [1, 15, 17, 129, 1500, 4099])
+@pytest.mark.parametrize("m,n", [(17, 3), (33, 260)])
+def test_rows_off_dwords(device, m, n, k):
+    """Rows copied end to end: a block's part of the copy crosses rows and the
+    border of a and b."""
+    ops = operands(m, n, k, 7)
+    check(*ops, run(device, *ops, np.float32, pad=1, offset=1))

@@ -157,3 +157,13 @@ def test_no_rows_and_no_columns(device):
     for rows, cols in ((0, 64), (3, 0)):
         _, q, scales = run(device, np.zeros((rows, cols), np.float32), None, np.ones(cols, np.float32), keep_h=False)
         assert q.shape == (rows, cols) and not scales.any()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_more_rows_than_a_launch_takes(device, residual):
+    """Sixteen rows a block and at most 2^21 blocks a launch."""
+    rows = 2**25 + 21
+    x = ((np.arange(rows) * 7) % 97 - 48).astype(np.float32)[:, None]
+    r = np.flip(x, 0).copy() if residual else None
+    w = np.full(1, 1.25, np.float32)
+    check(x, r, w, run(device, x, r, w, keep_h=residual))
