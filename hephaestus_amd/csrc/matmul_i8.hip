@@ -10,7 +10,8 @@
 //
 // * Few tokens (skinny): b is read once and straight into registers; the
 //   waves of a block take slices of k and add their sums in LDS.  The reading of
-//   b bounds it: 1 x 4096 x 4096 takes 5.4 us, 3.1 TB/s with the launch.
+//   b bounds it: 1 x 4096 x 4096 takes 4.8 us, 3.5 TB/s with the launch; 4097 bytes
+//   of k, rows at any byte, 6.1.
 // * Tiles: rows of 128 bytes of a and b go through LDS buffers in turn.  The
 //   matrix instructions bound large products, 8192 x 8192 x 8192 in 481 us, 2.29
 //   PetaOP/s; the reading of b bounds a few tokens more than a skinny one takes,
@@ -19,6 +20,7 @@
 #include "layer_device.hpp"
 
 #include <atomic>
+#include <type_traits>
 
 namespace hx {
 namespace {
@@ -72,39 +74,73 @@ __device__ __forceinline__ void store_scaled(T *row, uint64_t n, uint64_t end, i
     }
 }
 
+// 16 bytes of a row at any address, from the dwords that hold them, which are
+// shifted when they are used: vectors off dwords load at half the rate (7 x 8192 x
+// 8192 27.5 us, 16.4 so).  The dword after the first sixteen bytes is read only where
+// some of the row's lie in it.
+struct AnyBytes {
+    u32x4 v;
+    uint32_t next;
+};
+__device__ __forceinline__ AnyBytes load_dwords(const int8_t *p) {
+    const int8_t *down = p - ((uintptr_t)p & 3);
+    return {*(const u32x4_a4 *)down, *(const uint32_t *)(down + ((uintptr_t)p & 3 ? 16 : 12))};
+}
+__device__ __forceinline__ i32x4v shift_bytes(const AnyBytes &b, uint32_t by) {
+    return i32x4v{(int)__builtin_amdgcn_alignbyte(b.v[1], b.v[0], by), (int)__builtin_amdgcn_alignbyte(b.v[2], b.v[1], by),
+                  (int)__builtin_amdgcn_alignbyte(b.v[3], b.v[2], by), (int)__builtin_amdgcn_alignbyte(b.next, b.v[3], by)};
+}
+
 // ------------------------------------------------------------------ skinny
-// Up to 16 tokens; a block takes 16·NF channels, each of its eight waves every
+// Up to 16·MF tokens; a block takes 16·NF channels, each of its eight waves every
 // eighth 128 bytes of k.
 constexpr int kSkinnyWaves = 8;
 
-template <typename T, int NF>
+template <typename T, int MF, int NF, bool DWORDS>
 __global__ __launch_bounds__(kSkinnyWaves *kWave) void matmul_skinny_kernel(MatmulArgs p) {
-    __shared__ int sums[NF * 4 * kWave];
+    __shared__ int sums[MF * NF * 4 * kWave];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    static_assert(MF * NF <= kSkinnyWaves); // a wave stores one of the fragments
     const uint64_t n0 = (uint64_t)blockIdx.x * (16 * NF);
     const uint32_t k_end = (uint32_t)p.k, at = lane / 16 * 16;
-    for (int i = threadIdx.x; i < NF * 4 * kWave; i += kSkinnyWaves * kWave) sums[i] = 0;
-    const uint64_t m = lane % 16;
-    const uint32_t a_end = m < p.m ? k_end : 0; // rows that are not there are zeros
-    const int8_t *a = p.a + (int64_t)(m < p.m ? m : 0) * p.a_stride, *b[NF];
+    for (int i = threadIdx.x; i < MF * NF * 4 * kWave; i += kSkinnyWaves * kWave) sums[i] = 0;
+    uint32_t a_end[MF]; // rows that are not there are zeros
+    const int8_t *a[MF], *b[NF];
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+        const uint64_t m = 16 * f + lane % 16;
+        a_end[f] = m < p.m ? k_end : 0;
+        a[f] = p.a + (int64_t)(m < p.m ? m : 0) * p.a_stride;
+    }
 #pragma unroll
     for (int j = 0; j < NF; ++j) // channels past the end are summed and dropped
         b[j] = p.b + (int64_t)min(n0 + 16 * j + lane % 16, p.n - 1) * p.b_stride;
-    i32x4v acc[NF] = {};
+    i32x4v acc[MF][NF] = {};
     const uint32_t whole = k_end / kDepth * kDepth;
     constexpr uint32_t kTurn = kSkinnyWaves * kDepth;
     // The next turn's bytes are on their way while this turn is summed.
+    using Bytes = typename std::conditional<DWORDS, u32x4, AnyBytes>::type;
     struct Turn {
-        i32x4v b[NF][2], a[2];
+        Bytes b[NF][2], a[MF][2];
     } now, next;
+    const auto load = [](const int8_t *p) {
+        if constexpr (DWORDS) return (u32x4)*(const u32x4_a4 *)p;
+        else return load_dwords(p);
+    };
+    const auto whole_of = [](const Bytes &v, const int8_t *row) { // rows of one address modulo 4 throughout
+        if constexpr (DWORDS) return __builtin_bit_cast(i32x4v, v);
+        else return shift_bytes(v, (uint32_t)(uintptr_t)row & 3);
+    };
     const auto fetch = [&](uint32_t k, Turn &t) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int j = 0; j < NF; ++j)
-                t.b[j][s] = __builtin_bit_cast(i32x4v, (u32x4)*(const u32x4_any *)(b[j] + k + 64 * s + at));
-            t.a[s] = a_end ? __builtin_bit_cast(i32x4v, (u32x4)*(const u32x4_any *)(a + k + 64 * s + at))
-                           : i32x4v{0, 0, 0, 0};
+            for (int j = 0; j < NF; ++j) t.b[j][s] = load(b[j] + k + 64 * s + at);
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                t.a[f][s] = Bytes{};
+                if (a_end[f]) t.a[f][s] = load(a[f] + k + 64 * s + at);
+            }
         }
     };
     // Blocks begin at different turns: rows a power of two apart lie on the
@@ -117,9 +153,17 @@ __global__ __launch_bounds__(kSkinnyWaves *kWave) void matmul_skinny_kernel(Matm
         t = t + 1 < turns ? t + 1 : 0;
         if (left > 1) fetch(first + t * kTurn, next);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
+            i32x4v fb[NF];
 #pragma unroll
-            for (int j = 0; j < NF; ++j) acc[j] = mma(now.b[j][s], now.a[s], acc[j]);
+            for (int j = 0; j < NF; ++j) fb[j] = whole_of(now.b[j][s], b[j]);
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                const i32x4v fa = whole_of(now.a[f][s], a[f]);
+#pragma unroll
+                for (int j = 0; j < NF; ++j) acc[f][j] = mma(fb[j], fa, acc[f][j]);
+            }
+        }
         now = next;
     }
     // The last, partial 128 bytes: to the wave whose turn it is.
@@ -127,33 +171,43 @@ __global__ __launch_bounds__(kSkinnyWaves *kWave) void matmul_skinny_kernel(Matm
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const uint32_t k = whole + 64 * s + at;
-            const i32x4v fa = load_bytes(a, k, a_end);
+            i32x4v fa[MF], fb[NF];
 #pragma unroll
-            for (int j = 0; j < NF; ++j) acc[j] = mma(load_bytes(b[j], k, k_end), fa, acc[j]);
+            for (int f = 0; f < MF; ++f) fa[f] = load_bytes(a[f], k, a_end[f]);
+#pragma unroll
+            for (int j = 0; j < NF; ++j) fb[j] = load_bytes(b[j], k, k_end);
+#pragma unroll
+            for (int f = 0; f < MF; ++f)
+#pragma unroll
+                for (int j = 0; j < NF; ++j) acc[f][j] = mma(fb[j], fa[f], acc[f][j]);
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < NF; ++j)
+    for (int f = 0; f < MF; ++f)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) atomicAdd(&sums[(j * 4 + e) * kWave + lane], acc[j][e]);
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) atomicAdd(&sums[((f * NF + j) * 4 + e) * kWave + lane], acc[f][j][e]);
     __syncthreads();
-    if (wave >= NF || m >= p.m) return;
+    if (wave >= MF * NF) return;
+    const uint64_t m = 16 * (wave / NF) + lane % 16;
+    if (m >= p.m) return;
     i32x4v s;
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = sums[(wave * 4 + e) * kWave + lane];
-    store_scaled((T *)p.out + (int64_t)m * p.out_stride, n0 + 16 * wave + lane / 16 * 4, p.n, s, p.a_scales[m],
+    store_scaled((T *)p.out + (int64_t)m * p.out_stride, n0 + 16 * (wave % NF) + lane / 16 * 4, p.n, s, p.a_scales[m],
                  p.b_scales);
 }
 
-template <typename T> hx_status launch_skinny(const MatmulArgs &p, hipStream_t stream) {
+template <typename T, int MF, bool DWORDS> hx_status launch_skinny(const MatmulArgs &p, hipStream_t stream) {
     const auto run = [&](auto kernel, uint64_t channels) {
         hipLaunchKernelGGL(kernel, dim3((uint32_t)ceil_div(p.n, channels)), dim3(kSkinnyWaves * kWave), 0, stream, p);
     };
     // Two fragments of channels a block halve its reads of a, from the size
     // on where there is a block for each CU all the same.
-    if (p.n >= 2 * 16 * 256) run(matmul_skinny_kernel<T, 2>, 32);
-    else run(matmul_skinny_kernel<T, 1>, 16);
+    if (p.n >= 2 * 16 * 256) run(matmul_skinny_kernel<T, MF, 2, DWORDS>, 32);
+    else run(matmul_skinny_kernel<T, MF, 1, DWORDS>, 16);
     return check_launch("matmul_skinny_kernel");
 }
 
@@ -370,7 +424,7 @@ template <typename T> hx_status launch_tiled(const MatmulArgs &p, hipStream_t st
 // Rows of a and b at any byte, copied to rows of whole 128 bytes with zeros
 // after their ends, sixteen bytes a thread, the rows end to end.  Loading such rows
 // through registers in every tile took 29 us for 1000 x 1027 x 4099; the copy and
-// then direct loads take 23.
+// then direct loads take 19.7.
 __global__ __launch_bounds__(256) void matmul_align_kernel(MatmulArgs p, int8_t *rows, uint32_t pitch) {
     const uint32_t chunks = pitch / 16; // of a row
     for (uint64_t first = (uint64_t)blockIdx.x * 256; first < (p.m + p.n) * chunks; first += (uint64_t)gridDim.x * 256) {
@@ -382,16 +436,28 @@ __global__ __launch_bounds__(256) void matmul_align_kernel(MatmulArgs p, int8_t 
     }
 }
 
-constexpr uint64_t kSkinnyTokens = 16;
-
-bool needs_copy(const MatmulArgs &p) {
-    const uint64_t bits = (uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.a_stride | (uint64_t)p.b_stride;
-    return p.m > kSkinnyTokens && p.k > 0 && bits % 4 != 0;
+// Up to 16 tokens take the form that reads rows as they lie.  Up to 32 do where
+// rows lie off dwords, so that tiles would need a copy first, unless a few blocks
+// would have long rows to read (us, so and by copy and tiles):
+//   20 x 8192 x 16384   46.2, 87.2     32 x 8192 x 16384   52.3, 89.0
+//   20 x 4096 x 4097     9.7, 13.3     32 x 4096 x 4097    11.1, 13.2
+//   20 x 1000 x 1001     4.0,  7.7     32 x 16384 x 600     6.3, 11.1
+//   20 x 100 x 16384    24.4, 12.3     64 x 4096 x 4097    16.8, 14.4
+bool off_dwords(const MatmulArgs &p) {
+    return ((uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.a_stride | (uint64_t)p.b_stride) % 4 != 0;
 }
+bool is_skinny(const MatmulArgs &p) {
+    return p.m <= 16 || (p.m <= 32 && off_dwords(p) && (p.k <= 4096 || p.n >= 4096));
+}
+bool needs_copy(const MatmulArgs &p) { return !is_skinny(p) && p.k > 0 && off_dwords(p); }
 uint64_t copy_pitch(const MatmulArgs &p) { return ceil_div(p.k, kDepth) * kDepth; }
 
 template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t stream) {
-    if (p.m <= kSkinnyTokens) return launch_skinny<T>(p, stream);
+    if (is_skinny(p)) {
+        if (!off_dwords(p)) return launch_skinny<T, 1, true>(p, stream);
+        if (p.m <= 16) return launch_skinny<T, 1, false>(p, stream);
+        return launch_skinny<T, 2, false>(p, stream);
+    }
     if (needs_copy(p)) {
         const uint32_t pitch = (uint32_t)copy_pitch(p);
         const uint64_t blocks = min(ceil_div((p.m + p.n) * (pitch / 16), 256), (uint64_t)1 << 22);

@@ -124,3 +124,14 @@ def test_rows_off_dwords(device, m, n, k):
     border of a and b."""
     ops = operands(m, n, k, 7)
     check(*ops, run(device, *ops, np.float32, pad=1, offset=1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (2, 1), (1, 2), (3, 3)])
+@pytest.mark.parametrize("m,n,k", [(1, 16, 127), (15, 40, 1025), (16, 33, 4099), (17, 100, 129), (31, 70, 2047),
+                                   (32, 8200, 257), (32, 33, 4097), (33, 33, 1023)])
+def test_few_tokens_off_dwords(device, dtype, m, n, k, pad, offset):
+    """Each row at its own address modulo 4; both sides of the bounds on tokens,
+    channels and depth."""
+    ops = operands(m, n, k, 8)
+    check(*ops, run(device, *ops, TYPES[dtype], pad=pad, offset=offset, prepared=True))
