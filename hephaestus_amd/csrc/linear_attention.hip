@@ -173,9 +173,9 @@ template <typename T> hx_status launch_steps(const AttentionArgs &a, hipStream_t
 // accumulators of the last product, for the whole prompt.
 //
 // What bounds a block of bf16 is LDS: every wave reads all of q and k, about 4000
-// of a chunk's 9000 cycles at 64 tokens of 128 x 128, and then the arithmetic of
-// the three terms (below).  8 x 32 heads of 128 x 128 over 4096 tokens take 272
-// us, 1.1 GB at 4.1 TB/s; loads and stores alone took 230.  Chunks of 128 tokens
+// of a chunk's 10000 cycles at 64 tokens of 128 x 128, and then the arithmetic of
+// the two and three terms (below).  8 x 32 heads of 128 x 128 over 4096 tokens take
+// 302 us, 1.1 GB at 3.7 TB/s; loads and stores alone took 230.  Chunks of 128 tokens
 // have no room beside the next one.  In f32 the matrix instructions weigh most, at
 // a sixteenth of the rate of bf16: half of the 6.3 us of a chunk of 32 tokens of
 // 80 x 96 (5 x 12 heads, up to 1000 tokens: 51 us, and 24 for the parts' sums).
@@ -188,8 +188,11 @@ template <typename T> hx_status launch_steps(const AttentionArgs &a, hipStream_t
 // every wave needs all of it.
 //
 // Roundings, where the elements are bf16: an element of P, and of S where a
-// query meets it, is rounded to bf16 once.  The sums that go into S are not: a
-// weighted value D^(r-1-s)·v is taken as three bf16 terms, which hold 24 bits.
+// query meets it, is taken as two bf16 terms, which hold 16 bits, so that an
+// output keeps the 8 bits of its own rounding, as those of single tokens do.  One
+// term each took 270 us where these take 302, and made the error of an output in
+// the norm 1.4 times as large.  The sums that go into S keep all bits: a weighted
+// value D^(r-1-s)·v is three terms.
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -233,6 +236,17 @@ __device__ __forceinline__ void split(f32x4v v, bf16x4 (&to)[3]) {
     }
 }
 __device__ __forceinline__ void split(f32x4v v, f32x4v (&to)[1]) { to[0] = v; }
+
+// The same in the two terms that an output needs: the first cut off, so that no
+// finite value becomes an infinity, the second rounded.
+template <typename T> constexpr int kOutTerms = sizeof(T) == 2 ? 2 : 1;
+__device__ __forceinline__ void split_two(f32x4v v, bf16x4 (&to)[2]) {
+    const s16x4 high = {(short)(__float_as_uint(v[0]) >> 16), (short)(__float_as_uint(v[1]) >> 16),
+                        (short)(__float_as_uint(v[2]) >> 16), (short)(__float_as_uint(v[3]) >> 16)};
+    to[0] = __builtin_bit_cast(bf16x4, high);
+    to[1] = rounded(v - widened(to[0]), bf16{});
+}
+__device__ __forceinline__ void split_two(f32x4v v, f32x4v (&to)[1]) { to[0] = v; }
 
 // The same value, which the compiler cannot know: what is computed from it stays
 // where it is written, in a branch that is seldom taken, and takes up no
@@ -469,9 +483,14 @@ template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT> struct Chunk {
     static constexpr int WK = DK <= 64 ? 64 : DK <= 128 ? 128 : 256; // rows of q and k in LDS
     static constexpr int kTileK = C * WK * (int)sizeof(T), kTileV = C * DV * (int)sizeof(T);
     static constexpr int kStage = (OUTPUTS ? 2 : 1) * kTileK + kTileV;
-    static constexpr int kScores = OUTPUTS ? B * (B + 1) / 2 * 4 * kWave * (int)sizeof(T) : 0; // P, on and below the diagonal
-    // Chunks in LDS: one read, the others on their way.
-    static constexpr int S = DIRECT && 3 * kStage + kScores <= 160 * 1024 ? 3 : 2;
+    // P, on and below the diagonal.
+    static constexpr int kTiles = B * (B + 1) / 2;
+    static constexpr int kScores = OUTPUTS ? kTiles * kOutTerms<T> * 4 * kWave * (int)sizeof(T) : 0;
+    // Chunks in LDS: one read, the others on their way; two where that lets LDS
+    // hold two blocks.
+    static constexpr int kHalf = 80 * 1024;
+    static constexpr int kRoom = NW == 4 && DK <= 128 && 2 * kStage + kScores <= kHalf ? kHalf : 2 * kHalf;
+    static constexpr int S = DIRECT && 3 * kStage + kScores <= kRoom ? 3 : 2;
     static constexpr int kLds = S * kStage + kScores;
     static_assert(kLds <= 160 * 1024);
     // Where LDS holds two blocks of four waves, so must the registers: 1 x 50 heads of
@@ -643,17 +662,26 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
                     const int far = (y * 16 + col) - (x * 16 + quad * 4 + e);
                     p[e] = far >= 0 ? p[e] * (power(far) * a.scale) : 0.0f;
                 }
-                ps[tile * kWave + lane] = rounded(p, T{});
+                F terms[kOutTerms<T>];
+                split_two(p, terms);
+#pragma unroll
+                for (int m = 0; m < kOutTerms<T>; ++m) ps[(m * G::kTiles + tile) * kWave + lane] = terms[m];
             }
             // The state's part of the outputs.
 #pragma unroll
             for (int i = 0; i < DK / 32; ++i) {
-                const F state[2] = {rounded(s[2 * i], T{}), rounded(s[2 * i + 1], T{})};
+                F even[kOutTerms<T>], odd[kOutTerms<T>];
+                split_two(s[2 * i], even);
+                split_two(s[2 * i + 1], odd);
 #pragma unroll
                 for (int y = 0; y < B; ++y) {
                     F fq[2];
                     load_state_terms<WK>(qs, y * 16, i, fq);
-                    o[y] = mma(state, fq, o[y]);
+#pragma unroll
+                    for (int m = kOutTerms<T> - 1; m >= 0; --m) {
+                        const F state[2] = {even[m], odd[m]};
+                        o[y] = mma(state, fq, o[y]);
+                    }
                 }
             }
             float weight = query_weight;
@@ -727,9 +755,12 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
 #pragma unroll
                 for (int x = 0; x <= y; x += 2) {
                     const F fv[2] = {vf[x], vf[x + 1]};
-                    F fp[2] = {ps[(y * (y + 1) / 2 + x) * kWave + lane], F{}};
-                    if (x < y) fp[1] = ps[(y * (y + 1) / 2 + x + 1) * kWave + lane];
-                    o[y] = mma(fv, fp, o[y]);
+#pragma unroll
+                    for (int m = kOutTerms<T> - 1; m >= 0; --m) {
+                        const F *p = ps + (m * G::kTiles + y * (y + 1) / 2 + x) * kWave + lane;
+                        const F fp[2] = {p[0], x < y ? p[kWave] : F{}};
+                        o[y] = mma(fv, fp, o[y]);
+                    }
                 }
             if (__any(first_bad < C)) {
 #pragma unroll
