@@ -597,26 +597,17 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
                 if (from && state_row<T>(i, e) < dk) s[i][e] = from[state_row<T>(i, e) * stride];
     }
 
-    // The decay over a chunk is rounded to a float; what that leaves out of the
-    // state is made good every kSettle chunks, so that the state keeps the
-    // precision of f32 however many there are.
-    constexpr uint32_t kSettle = 8;
+    // The decay over a chunk, as a float and what its rounding leaves out: the
+    // state keeps the precision of f32 however many chunks there are.
     struct Decay {
-        float by, drift; // the factor, and its rounding's relative error
+        float by, rest;
     };
     const auto decay_over = [&](uint32_t rows) {
         const double d = exp((double)log_decay * rows);
         const float by = (float)d;
-        return Decay{by, by > 0.0f ? (float)((d - by) / by) : 0.0f};
+        return Decay{by, (float)(d - by)};
     };
-    Decay decay = decay_over(C);
-    const Decay last_decay = decay_over(chunks ? end - begin - (chunks - 1) * C : 1);
-    const auto make_good = [&](uint32_t chunks) {
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] = fmaf(s[i][e], decay.drift * (float)chunks, s[i][e]);
-    };
+    const Decay decay = decay_over(C), last_decay = decay_over(chunks ? end - begin - (chunks - 1) * C : 1);
     // Powers of the decay: over 16 tokens; in a whole chunk's last 16 rows, the
     // weight of a row in the state; at a token of the first 16, of the state.
     const float over16 = power(16), query_weight = power(col + 1) * a.scale;
@@ -690,12 +681,11 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
         };
         const auto advance = [&] {
             // The state: decayed over the chunk, then the chunk's sum.
-            if (rows < C) { // the last one
-                make_good(n % kSettle);
-                decay = last_decay;
-            }
+            const Decay over = rows < C ? last_decay : decay;
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) s[i] *= decay.by;
+            for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][e] = fmaf(s[i][e], over.by, s[i][e] * over.rest);
             F terms[B][kTerms<T>];
             f32x4v weight = last_weight;
 #pragma unroll
@@ -723,7 +713,6 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
                         }
                     }
             }
-            if (rows < C || n % kSettle == kSettle - 1) make_good(rows < C ? 1 : kSettle);
         };
         if constexpr (OUTPUTS) outputs();
         advance();

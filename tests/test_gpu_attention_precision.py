@@ -30,3 +30,49 @@ def test_bf16_prompts_round_once(device, tokens, heads, dk, dv):
     # of the rounding: 2^-15 against 2^-10 or more.
     rounding = as_float64(hx.bfloat16_from_float32(want.astype(np.float32))) - want
     assert np.linalg.norm(got - want) <= 1.02 * np.linalg.norm(rounding)
+
+
+def drifting_decays(rng, heads, chunk):
+    """Log decays whose factor over a chunk, as a float, is too small by most of
+    half a unit: 2^-25, relative."""
+    found = []
+    while len(found) < heads:
+        g = rng.uniform(-0.1 / chunk, -0.02 / chunk, 4096).astype(np.float32)
+        d = np.exp(g.astype(np.float64) * chunk)
+        found.extend(g[(d - d.astype(np.float32)) / d >= 0.7 * 2.0**-25])
+    return np.array(found[:heads], np.float32)
+
+
+def bias(got, want):
+    return float(np.vdot(got.astype(np.float64) - want, want) / np.vdot(want, want))
+
+
+# Few tokens of 260 heads, so that a prompt is not cut and its chunks follow one
+# another in a block.  Roundings of 66560 elements average out to less than
+# 2^-30 of them; a decay that is short by 0.7·2^-25 a chunk does not.
+@pytest.mark.parametrize("dtype,chunk", [(np.float32, 32), (hx.bfloat16, 64)], ids=["f32", "bf16"])
+@pytest.mark.parametrize("chunks", [1, 2, 7, 8, 9, 15])
+@pytest.mark.parametrize("rest", [0, 1])
+def test_a_state_decays_without_drift(device, dtype, chunk, chunks, rest):
+    tokens = chunks * chunk + rest
+    q, k, v, _, state = operands(dtype, 1, tokens, 260, 260, 16, 16, 22)
+    decay = drifting_decays(np.random.default_rng(chunks), 260, chunk)
+    v = np.zeros_like(v)
+    _, last = run(device, q, k, v, decay, state)
+    want = np.exp(decay.astype(np.float64) * tokens)[:, None, None] * state[0]
+    assert abs(bias(last[0], want)) <= 2.0**-27
+
+
+@pytest.mark.parametrize("dtype,chunk", [(np.float32, 32), (hx.bfloat16, 64)], ids=["f32", "bf16"])
+@pytest.mark.parametrize("chunks,at", [(8, 7), (8, 6), (8, 0), (9, 8), (9, 7), (16, 14), (11, 3)])
+def test_a_token_is_decayed_as_often_as_it_has_to_be(device, dtype, chunk, chunks, at):
+    """One token's values, at the end of chunk `at`: what is made good for a
+    state's earlier part must not reach them."""
+    tokens, t = chunks * chunk, (at + 1) * chunk - 1
+    q, k, v, _, _ = operands(dtype, 1, tokens, 260, 260, 16, 16, 23)
+    decay = drifting_decays(np.random.default_rng(chunks), 260, chunk)
+    v[:, :t], v[:, t + 1:] = np.zeros(1, v.dtype), np.zeros(1, v.dtype)
+    _, last = run(device, q, k, v, decay)
+    want = (np.exp(decay.astype(np.float64) * (tokens - 1 - t))[:, None, None]
+            * as_float64(k)[0, t, :, :, None] * as_float64(v)[0, t, :, None, :])
+    assert abs(bias(last[0], want)) <= 2.0**-27
