@@ -521,8 +521,10 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
     T *out = (T *)a.out + b * a.so.batch + h * a.so.head + dv0;
     const uint32_t vcol = wave * 16 + col; // this lane's column of v and of the state
 
-    // The decay as a power of two a token; minus infinity would make 0·log a NaN.
-    const float log_decay = a.log_decay[h], log2_decay = fmaxf(log_decay * 1.44269504f, -1e30f);
+    // The decay as a power of two a token; minus infinity would make 0·log a NaN,
+    // and a NaN has to stay one.
+    const float log_decay = a.log_decay[h];
+    const float log2_decay = log_decay < -1e30f ? -1e30f : log_decay * 1.44269504f;
     const auto power = [&](int n) { return __builtin_amdgcn_exp2f(log2_decay * (float)n); };
 
     const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;

@@ -1,0 +1,24 @@
+"""Operands of linear attention that are no numbers: what they reach, and what they must not."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import hephaestus_amd as hx
+from layer_reference import as_float64
+from test_gpu_linear_attention import TYPES, operands, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 5, 20, 64, 70, 1500])
+def test_a_decay_that_is_no_number_spoils_its_head_only(device, dtype, tokens):
+    """In single tokens, within a chunk, over chunks and in a prompt that is cut."""
+    q, k, v, decay, state = operands(TYPES[dtype], 1, tokens, 3, 3, 32, 32, 31)
+    decay[1] = np.nan
+    for first in (state, None):
+        got, last = run(device, q, k, v, decay, first)
+        got = as_float64(got)
+        assert np.isnan(got[:, :, 1]).all() and np.isnan(last[:, 1]).all()
+        assert np.isfinite(np.delete(got, 1, 2)).all() and np.isfinite(np.delete(last, 1, 1)).all()
