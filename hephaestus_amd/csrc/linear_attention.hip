@@ -819,9 +819,10 @@ template <int V> __global__ __launch_bounds__(256) void attention_join_kernel(At
     Values s = {};
     if (a.state_in) s = *(const Values *)(a.state_in + b * a.si.batch + h * a.si.head + row * a.si.token + col);
     const double log_decay = a.log_decay[h];
-    // Every part but the last with tokens is whole, and those behind it have none.
-    const uint32_t whole = length / parts.span, rest = length % parts.span;
-    const double of_whole = exp(log_decay * parts.span), of_rest = rest ? exp(log_decay * rest) : 1.0;
+    // Every part but the last with tokens is whole, and those behind it have none:
+    // there the state stays as it is, whatever it holds.
+    const uint32_t whole = length / parts.span, rest = length % parts.span, used = whole + (rest != 0);
+    const double of_whole = exp(log_decay * parts.span), of_rest = exp(log_decay * rest);
     const float whole_high = (float)of_whole, whole_low = (float)(of_whole - whole_high);
     const float rest_high = (float)of_rest, rest_low = (float)(of_rest - rest_high);
     for (uint32_t p = 0;;) {
@@ -829,7 +830,7 @@ template <int V> __global__ __launch_bounds__(256) void attention_join_kernel(At
         for (uint32_t k = 0; k < kBatch; ++k) {
             if (p + k >= parts.parts) break;
             *(Values *)(at + (uint64_t)(p + k) * n) = s;
-            if (p + k > whole) continue;
+            if (p + k >= used) continue;
             const float high = p + k < whole ? whole_high : rest_high, low = p + k < whole ? whole_low : rest_low;
 #pragma unroll
             for (int e = 0; e < V; ++e) s[e] = fmaf(s[e], high, s[e] * low) + own[k][e];

@@ -22,3 +22,16 @@ def test_a_decay_that_is_no_number_spoils_its_head_only(device, dtype, tokens):
         got = as_float64(got)
         assert np.isnan(got[:, :, 1]).all() and np.isnan(last[:, 1]).all()
         assert np.isfinite(np.delete(got, 1, 2)).all() and np.isfinite(np.delete(last, 1, 1)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 5, 70, 4100])
+def test_a_sequence_of_no_tokens_keeps_any_state(device, dtype, tokens):
+    """To the bit, infinities, NaN and negative zeros too; beside it a sequence
+    that ends where a part of a cut prompt does."""
+    q, k, v, decay, state = operands(TYPES[dtype], 2, tokens, 1, 1, 16, 16, 32)
+    state[0, 0, 3, :4] = np.inf, -np.inf, np.nan, -0.0
+    state[0, 0, 9, 5:7] = -0.0, 1e-40
+    got, last = run(device, q, k, v, decay, state, [0, tokens])
+    assert np.array_equal(last[0].view(np.uint32), state[0].view(np.uint32))
+    assert not as_float64(got)[0].any() and np.isfinite(last[1]).all()
