@@ -585,7 +585,12 @@ hx_status hx_prepare_matmul_i8(hx_device *dev, const void *a,
  * token; either may be NULL (state_in: zeros), and they may be the very same
  * view.  `lengths` (u32[batch], or NULL for `tokens` everywhere) counts each
  * sequence's tokens, at most `tokens`: later rows of q, k and v are not read,
- * later rows of out are 0, and a sequence of no tokens keeps its state. */
+ * later rows of out are 0, and a sequence of no tokens keeps its state.
+ * Outputs are sums in f32 rounded once; in prompts of bf16 a score q_t k_s, and
+ * an element of the state that a query meets, keep 16 bits.  An infinity or a
+ * NaN in q, k, v, log_decay or state_in reaches the outputs and elements of
+ * the state that depend on it by the formula, and no others; whether they
+ * become an infinity or a NaN depends on how tokens are taken together. */
 hx_status hx_linear_attention(
     hx_device *dev, hx_dtype dtype, const void *q, uint64_t q_buf_len,
     const hx_layout *q_layout, const void *k, uint64_t k_buf_len,

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import hephaestus_amd as hx
-from layer_reference import as_float64
+from layer_reference import as_float64, linear_attention, rounded
 from test_gpu_linear_attention import TYPES, operands, run
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +35,24 @@ def test_a_sequence_of_no_tokens_keeps_any_state(device, dtype, tokens):
     got, last = run(device, q, k, v, decay, state, [0, tokens])
     assert np.array_equal(last[0].view(np.uint32), state[0].view(np.uint32))
     assert not as_float64(got)[0].any() and np.isfinite(last[1]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 6, 70, 700])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("where", ["q", "k", "v", "state"])
+def test_what_is_not_finite_reaches_what_the_formula_says(device, dtype, tokens, value, where):
+    """Which of infinity and NaN it is depends on the order of the sums."""
+    q, k, v, decay, state = operands(TYPES[dtype], 1, tokens, 2, 1, 32, 32, 33)
+    state = state.copy()
+    t = tokens // 2
+    bad = rounded(np.array([value]), TYPES[dtype])[0]
+    if where == "state":
+        state[0, 1, 7, 3] = value
+    else:
+        {"q": q, "k": k, "v": v}[where][0, t, 0, 7] = bad
+    got, last = run(device, q, k, v, decay, state)
+    with np.errstate(invalid="ignore"):
+        want, want_last, _, _ = linear_attention(q, k, v, decay, 32 ** -0.5, state)
+    assert np.array_equal(np.isfinite(as_float64(got)), np.isfinite(want))
+    assert np.array_equal(np.isfinite(last), np.isfinite(want_last))
