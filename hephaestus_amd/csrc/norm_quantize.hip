@@ -6,7 +6,7 @@
 // One sweep over h therefore gives both Σh² and max|h·w|, one combine across
 // the row's waves gives both results, and the row is written from the
 // registers that it was read into.  Rows too long for the registers are read
-// twice.
+// twice; rows too small for f32 to hold their squares, thrice more (is_tiny).
 //
 // Memory bounds long inputs: 16384 x 8192 bf16 with a residual, 940 MB, takes
 // 156 us, 6.0 TB/s.  One row of 4096 takes 2.7 us, a launch and one wait for
@@ -19,24 +19,26 @@
 namespace hx {
 namespace {
 
-// Scaling of one row from Σh² and max|h·w|.  The maximum is taken of the bits
-// of |h·w| as integers: they order as the values do, with infinities and then
-// NaN above them, so that neither is lost.
+// Scaling of one row from Σh² and max|h·w|, or from 1 and max|y|.  The maximum is
+// taken of the bits as integers: they order as the magnitudes do, with infinities
+// and then NaN above them, so that neither is lost.
 constexpr uint32_t kInfinity = 0x7F800000u;
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
 struct RowScale {
     float scale;   // s
     float up, inv; // q = round(h·w·up·inv)
 };
-__device__ __forceinline__ RowScale row_scale(float sum, uint32_t bits, float cols, float epsilon) {
+__device__ __forceinline__ RowScale scale_of(float rstd, uint32_t bits, bool finite) {
     RowScale r;
-    const float rstd = 1.0f / sqrtf(sum / cols + epsilon), top = __builtin_bit_cast(float, bits);
-    const bool finite = magnitude(sum) < kInfinity && bits < kInfinity;
+    const float top = __builtin_bit_cast(float, bits);
     r.scale = finite ? (top > 0.0f ? rstd * top / 127.0f : 0.0f) : __builtin_nanf("");
     // 127 / top overflows for the tiniest rows; two factors do not.
     r.up = top < 0x1p-60f ? 0x1p60f : 1.0f;
     r.inv = finite && top > 0.0f ? 127.0f / (top * r.up) : 0.0f;
     return r;
+}
+__device__ __forceinline__ RowScale row_scale(float sum, uint32_t bits, float cols, float epsilon) {
+    return scale_of(1.0f / sqrtf(sum / cols + epsilon), bits, magnitude(sum) < kInfinity && bits < kInfinity);
 }
 __device__ __forceinline__ int quantize(float hw, const RowScale &r) {
     return r.inv > 0.0f ? (int)fminf(fmaxf(rintf(hw * r.up * r.inv), -127.0f), 127.0f) : 0;
@@ -99,6 +101,90 @@ __device__ __forceinline__ void store_bytes(int8_t *p, uint32_t c, uint32_t cols
     }
 }
 
+// A row in memory, swept by LANES threads: h is written by the sweep that reads it
+// last, so residual_out may lie on x or the residual.
+template <typename T, int LANES> struct SweptRow {
+    static constexpr int N = Pack16<T>::N;
+    const NormArgs &a;
+    const uint64_t row;
+    const uint32_t lane;
+
+    // f(c, h, w) for each vector of the row that is this thread's.
+    template <typename F> __device__ __forceinline__ void sweep(F f) const {
+        const uint32_t cols = (uint32_t)a.cols;
+        const T *x = (const T *)a.x + (int64_t)row * a.x_stride;
+        const T *res = (const T *)a.residual + (int64_t)row * a.residual_stride;
+        const T *w = (const T *)a.weight;
+#pragma unroll 1
+        for (uint32_t c = lane * N; c < cols; c += LANES * N) {
+            const u32x4 vx = load_part(x, c, cols), vw = load_part(w, c, cols);
+            u32x4 vr = {0, 0, 0, 0};
+            if (a.residual) vr = load_part(res, c, cols);
+            float h[N], r[N], wv[N];
+            unpack<T>(place_part<T>(vx, c, cols), h);
+            if (a.residual) {
+                unpack<T>(place_part<T>(vr, c, cols), r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[i] += r[i];
+            }
+            unpack<T>(place_part<T>(vw, c, cols), wv);
+            f(c, h, wv);
+        }
+    }
+    // Σ(h·up)² and the largest |of(h, w)|.
+    template <typename F> __device__ __forceinline__ void total(float up, F of, float &sum, uint32_t &top) const {
+        sum = 0.0f;
+        top = 0;
+        sweep([&](uint32_t, const float(&h)[N], const float(&w)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sum += h[i] * up * (h[i] * up);
+                top = max(top, magnitude(of(h[i], w[i])));
+            }
+        });
+        if constexpr (LANES <= kWave) combine_lanes<LANES>(sum, top);
+        else combine_waves<LANES / kWave>(sum, top);
+    }
+    template <typename F> __device__ __forceinline__ void write(const RowScale &r, F of) const {
+        const uint32_t cols = (uint32_t)a.cols;
+        if (lane == 0) a.scales[row] = r.scale;
+        T *ho = (T *)a.residual_out + (int64_t)row * a.residual_out_stride;
+        int8_t *q = a.quantized + (int64_t)row * a.quantized_stride;
+        sweep([&](uint32_t c, const float(&h)[N], const float(&w)[N]) {
+            float y[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = of(h[i], w[i]);
+            if (a.residual_out) store_row(ho, c, cols, h);
+            store_bytes(q, c, cols, y, r);
+        });
+    }
+};
+
+// Rows that are read again because f32 cannot hold what the one sweep takes:
+// * The squares lose bits or vanish, and epsilon does not outweigh them: the mean
+//   has an error of 2^-150 at most, which counts below 2^-120.  They are taken from
+//   h·2^100: whole from the least float on, and their mean is below 2^80.
+// * h·w loses bits where y does not: the largest is below 2^-100.
+// Both take y itself, h·rstd first.
+constexpr float kTinyMean = 0x1p-120f, kTinyTop = 0x1p-100f;
+__device__ __forceinline__ bool is_tiny(float sum, uint32_t bits, float cols, float epsilon) {
+    return bits < kInfinity &&
+           (sum / cols + epsilon < kTinyMean || (bits > 0 && bits < __builtin_bit_cast(uint32_t, kTinyTop)));
+}
+template <typename T, int LANES> __device__ __forceinline__ void write_tiny_row(const SweptRow<T, LANES> &row, float sum) {
+    const float cols = (float)row.a.cols, epsilon = row.a.epsilon;
+    const float lift = sum / cols + epsilon < kTinyMean ? 0x1p100f : 1.0f;
+    uint32_t top;
+    float none;
+    if constexpr (LANES > kWave) __syncthreads(); // the last sums have been read
+    row.total(lift, [](float, float) { return 0.0f; }, sum, top);
+    const float mean = sum / cols + epsilon * lift * lift, rstd = mean > 0.0f ? 1.0f / sqrtf(mean) : 0.0f;
+    const auto y = [&](float h, float w) { return h * lift * rstd * w; };
+    if constexpr (LANES > kWave) __syncthreads();
+    row.total(1.0f, y, none, top);
+    row.write(scale_of(1.0f, top, magnitude(sum) < kInfinity && top < kInfinity), y);
+}
+
 // Rows of up to LANES·STEPS vectors, LANES threads a row.  A block has one row,
 // or, where a row has less than four waves, as many as fill four.
 template <typename T, int LANES, int STEPS>
@@ -155,6 +241,10 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows_kernel(No
     }
     if constexpr (LANES <= kWave) combine_lanes<LANES>(sum, top);
     else combine_waves<LANES / kWave>(sum, top);
+    if (is_tiny(sum, top, (float)a.cols, a.epsilon)) { // the same for all lanes of a row
+        write_tiny_row(SweptRow<T, LANES>{a, row, lane}, sum);
+        return;
+    }
     const RowScale r = row_scale(sum, top, (float)a.cols, a.epsilon);
     if (lane == 0) a.scales[row] = r.scale;
     T *ho = (T *)a.residual_out + (int64_t)row * a.residual_out_stride;
@@ -170,52 +260,15 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_rows_kernel(No
     }
 }
 
-// Rows of any length, read twice by one block; h is written by the sweep
-// that reads it last, so residual_out may lie on x or the residual.
+// Rows of any length, read twice by one block.
 template <typename T> __global__ __launch_bounds__(1024) void norm_long_rows_kernel(NormArgs a) {
-    constexpr int N = Pack16<T>::N;
-    const uint64_t row = blockIdx.x;
-    const uint32_t cols = (uint32_t)a.cols;
-    const T *x = (const T *)a.x + (int64_t)row * a.x_stride;
-    const T *res = (const T *)a.residual + (int64_t)row * a.residual_stride;
-    const T *w = (const T *)a.weight;
-    T *ho = (T *)a.residual_out + (int64_t)row * a.residual_out_stride;
-    int8_t *q = a.quantized + (int64_t)row * a.quantized_stride;
-    const auto sweep = [&](uint32_t c, float (&h)[N], float (&hw)[N]) {
-        const u32x4 vx = load_part(x, c, cols), vw = load_part(w, c, cols);
-        u32x4 vr = {0, 0, 0, 0};
-        if (a.residual) vr = load_part(res, c, cols);
-        unpack<T>(place_part<T>(vx, c, cols), h);
-        if (a.residual) {
-            float r[N];
-            unpack<T>(place_part<T>(vr, c, cols), r);
-#pragma unroll
-            for (int i = 0; i < N; ++i) h[i] += r[i];
-        }
-        unpack<T>(place_part<T>(vw, c, cols), hw);
-#pragma unroll
-        for (int i = 0; i < N; ++i) hw[i] *= h[i];
-    };
-    float sum = 0.0f;
-    uint32_t top = 0;
-    for (uint32_t c = threadIdx.x * N; c < cols; c += 1024 * N) {
-        float h[N], hw[N];
-        sweep(c, h, hw);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            sum += h[i] * h[i];
-            top = max(top, magnitude(hw[i]));
-        }
-    }
-    combine_waves<16>(sum, top);
-    const RowScale r = row_scale(sum, top, (float)a.cols, a.epsilon);
-    if (threadIdx.x == 0) a.scales[row] = r.scale;
-    for (uint32_t c = threadIdx.x * N; c < cols; c += 1024 * N) {
-        float h[N], hw[N];
-        sweep(c, h, hw);
-        if (a.residual_out) store_row(ho, c, cols, h);
-        store_bytes(q, c, cols, hw, r);
-    }
+    const SweptRow<T, 1024> row{a, blockIdx.x, threadIdx.x};
+    const auto product = [](float h, float w) { return h * w; };
+    float sum;
+    uint32_t top;
+    row.total(1.0f, product, sum, top);
+    if (is_tiny(sum, top, (float)a.cols, a.epsilon)) write_tiny_row(row, sum);
+    else row.write(row_scale(sum, top, (float)a.cols, a.epsilon), product);
 }
 
 // The rows from `first` on.

@@ -532,7 +532,8 @@ hx_status hx_vector_binary(hx_device *dev, hx_vector_op op, hx_dtype dtype,
  * before that rounding.  `quantized` is an int8 view of x's shape, `scales`
  * f32[rows].  A row of zeros has s = 0 and q = 0; a row with a NaN or an
  * infinity in h or h * weight, or whose sum of squares exceeds the range of
- * f32, has s = NaN and q = 0.  residual_out may be the very view of x or of residual. */
+ * f32, has s = NaN and q = 0.  Rows whose squares are below that range are as
+ * exact as others.  residual_out may be the very view of x or of residual. */
 hx_status hx_rms_norm_quantize(hx_device *dev, hx_dtype dtype, const void *x,
                                uint64_t x_buf_len, const hx_layout *x_layout,
                                const void *residual, uint64_t residual_buf_len,
