@@ -373,7 +373,7 @@ hx_status launch_tiles(const MatmulArgs &p, hipStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     HX_TRY(allow_lds((const void *)kernel, C::kLds, allowed));
     const uint64_t tm = ceil_div(p.m, BM), tn = ceil_div(p.n, BN);
-    if (tm * tn > 0x7FFFFFFFull)
+    if (tm * tn * C::kThreads > 0xFFFFFFFFull)
         return fail(HX_ERR_DISPATCH_FAILED, "matmul of %llu tiles exceeds the grid range", (unsigned long long)(tm * tn));
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(C::kThreads), C::kLds, stream, p, (uint32_t)tm,
                        (uint32_t)tn);
@@ -452,12 +452,32 @@ bool is_skinny(const MatmulArgs &p) {
 bool needs_copy(const MatmulArgs &p) { return !is_skinny(p) && p.k > 0 && off_dwords(p); }
 uint64_t copy_pitch(const MatmulArgs &p) { return ceil_div(p.k, kDepth) * kDepth; }
 
+// A launch has fewer than 2^32 threads: 16 a channel for a few tokens, up to 12 a
+// channel or 2 a token in tiles.  More channels or tokens take several launches.
+constexpr uint64_t kMostRows = 1ull << 27;
+template <typename T, typename F> hx_status in_parts(const MatmulArgs &p, F run) {
+    for (uint64_t m = 0; m < p.m; m += kMostRows)
+        for (uint64_t n = 0; n < p.n; n += kMostRows) {
+            MatmulArgs part = p;
+            part.m = min(p.m - m, kMostRows);
+            part.n = min(p.n - n, kMostRows);
+            part.a += (int64_t)m * p.a_stride;
+            part.b += (int64_t)n * p.b_stride;
+            part.a_scales += m;
+            part.b_scales += n;
+            part.out = (T *)p.out + (int64_t)m * p.out_stride + (int64_t)n;
+            HX_TRY(run(part));
+        }
+    return HX_OK;
+}
+
 template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t stream) {
-    if (is_skinny(p)) {
-        if (!off_dwords(p)) return launch_skinny<T, 1, true>(p, stream);
-        if (p.m <= 16) return launch_skinny<T, 1, false>(p, stream);
-        return launch_skinny<T, 2, false>(p, stream);
-    }
+    if (is_skinny(p))
+        return in_parts<T>(p, [&](const MatmulArgs &part) {
+            if (!off_dwords(p)) return launch_skinny<T, 1, true>(part, stream);
+            if (p.m <= 16) return launch_skinny<T, 1, false>(part, stream);
+            return launch_skinny<T, 2, false>(part, stream);
+        });
     if (needs_copy(p)) {
         const uint32_t pitch = (uint32_t)copy_pitch(p);
         const uint64_t blocks = min(ceil_div((p.m + p.n) * (pitch / 16), 256), (uint64_t)1 << 22);
@@ -468,7 +488,7 @@ template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t strea
         p.a_stride = p.b_stride = pitch;
         p.k = pitch;
     }
-    return launch_tiled<T>(p, stream);
+    return in_parts<T>(p, [&](const MatmulArgs &part) { return launch_tiled<T>(part, stream); });
 }
 
 } // namespace
