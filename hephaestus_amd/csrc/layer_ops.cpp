@@ -22,14 +22,72 @@ hx_status check_layer_dtype(hx_dtype d, uint32_t *size) {
     return HX_OK;
 }
 
-// The bytes that a view reaches, [first, end); empty views reach none.
+// The bytes that a view reaches lie in [first, end): from first on, `run` bytes at
+// each sum of whole steps.  Empty views reach none.
 struct Span {
     uintptr_t first = 0, end = 0;
     const void *base = nullptr;
     const hx_layout *layout = nullptr;
+    uint64_t run = 0;
+    uint32_t steps = 0;
+    uint64_t step[HX_MAX_RANK] = {}, count[HX_MAX_RANK] = {};
 };
 
-bool overlap(const Span &a, const Span &b) { return a.first < b.end && b.first < a.end; }
+// Whether Σ step·x = target has a solution with each x in [0, most], by trying
+// the values of x that the smaller steps can complete, the largest step first.
+// Where each step passes what the smaller ones reach together, as in views of
+// rows within rows, those are a few; a search that grows beyond `kTries` is given
+// up and counts as a solution.
+class StepSums {
+  public:
+    void add(uint64_t step, uint64_t most) {
+        if (step == 0 || most == 0) return;
+        uint32_t at = 0;
+        while (at < n_ && step_[at] > step) ++at;
+        if (at < n_ && step_[at] == step) {
+            most_[at] += most;
+            return;
+        }
+        for (uint32_t i = n_++; i > at; --i) step_[i] = step_[i - 1], most_[i] = most_[i - 1];
+        step_[at] = step;
+        most_[at] = most;
+    }
+    bool reach(__int128 target) {
+        __int128 sum = 0;
+        reach_[n_] = 0;
+        for (uint32_t i = n_; i-- > 0;) reach_[i] = sum += (__int128)step_[i] * most_[i];
+        tries_ = 0;
+        return from(0, target);
+    }
+
+  private:
+    static constexpr uint32_t kMost = 2 * HX_MAX_RANK + 1, kTries = 1 << 14;
+    uint32_t n_ = 0, tries_ = 0;
+    uint64_t step_[kMost], most_[kMost];
+    __int128 reach_[kMost + 1];
+
+    bool from(uint32_t i, __int128 target) {
+        if (target < 0 || target > reach_[i]) return false;
+        if (target == 0) return true;
+        if (++tries_ > kTries) return true;
+        const __int128 step = step_[i], rest = target - reach_[i + 1];
+        const __int128 low = rest > 0 ? (rest + step - 1) / step : 0, high = target / step;
+        for (__int128 x = low; x <= high && x <= most_[i]; ++x)
+            if (from(i + 1, target - x * step)) return true;
+        return false;
+    }
+};
+
+// Whether two views share a byte: a.first + Σ a's steps + a byte of the run meets
+// the same of b.  With b's steps counted from their ends all of them add up.
+bool overlap(const Span &a, const Span &b) {
+    if (a.first >= b.end || b.first >= a.end) return false;
+    StepSums sums;
+    for (uint32_t i = 0; i < a.steps; ++i) sums.add(a.step[i], a.count[i] - 1);
+    for (uint32_t i = 0; i < b.steps; ++i) sums.add(b.step[i], b.count[i] - 1);
+    sums.add(1, a.run - 1 + (b.run - 1));
+    return sums.reach((__int128)b.end - 1 - (__int128)a.first);
+}
 
 // The same elements at the same indices.
 bool same_view(const Span &a, const Span &b) {
@@ -95,6 +153,11 @@ hx_status check_view(const void *buf, uint64_t buf_len, const hx_layout *l, uint
     }
     span->first = (uintptr_t)buf + (uint64_t)lo * size;
     span->end = (uintptr_t)buf + ((uint64_t)hi + 1) * size;
+    span->run = l->shape[rank - 1] * size;
+    for (uint32_t d = 0; d + 1 < rank; ++d) {
+        span->step[span->steps] = (uint64_t)std::llabs(l->strides[d]) * size;
+        span->count[span->steps++] = l->shape[d];
+    }
     return HX_OK;
 }
 
@@ -108,6 +171,7 @@ hx_status check_vector(const void *buf, uint64_t len, uint64_t want, uint32_t si
     if ((uintptr_t)buf % size) return fail(HX_ERR_DISPATCH_FAILED, "%s is not aligned to its elements", what);
     span->first = (uintptr_t)buf;
     span->end = span->first + want * size;
+    span->run = want * size;
     return HX_OK;
 }
 
