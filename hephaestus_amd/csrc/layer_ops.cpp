@@ -97,22 +97,24 @@ bool same_view(const Span &a, const Span &b) {
     return true;
 }
 
-// Distinct indices reach distinct elements: taken by rising stride, every
-// dimension steps over all that the ones before it reach.
+// Distinct indices reach distinct elements: no two differ by a whole number y of
+// steps in each dimension that come to nothing, Σ stride·y = 0.  With d the first
+// dimension of y ≠ 0, y_d is taken as 1 on and the later ones from 1 - shape on.
 bool is_injective(const hx_layout &l) {
-    bool used[HX_MAX_RANK] = {};
-    __int128 reach = 1;
-    for (uint32_t i = 0; i < l.rank; ++i) {
-        uint32_t best = HX_MAX_RANK;
-        for (uint32_t d = 0; d < l.rank; ++d)
-            if (!used[d] && l.shape[d] > 1 &&
-                (best == HX_MAX_RANK || std::llabs(l.strides[d]) < std::llabs(l.strides[best])))
-                best = d;
-        if (best == HX_MAX_RANK) break;
-        used[best] = true;
-        const __int128 step = l.strides[best] < 0 ? -(__int128)l.strides[best] : (__int128)l.strides[best];
-        if (step < reach) return false;
-        reach += step * (__int128)(l.shape[best] - 1);
+    for (uint32_t d = 0; d < l.rank; ++d) {
+        if (l.shape[d] <= 1) continue;
+        const uint64_t step = (uint64_t)std::llabs(l.strides[d]);
+        if (step == 0) return false;
+        StepSums sums;
+        __int128 target = -(__int128)step;
+        sums.add(step, l.shape[d] - 2);
+        for (uint32_t e = d + 1; e < l.rank; ++e) {
+            if (l.shape[e] <= 1) continue;
+            const uint64_t other = (uint64_t)std::llabs(l.strides[e]);
+            sums.add(other, 2 * (l.shape[e] - 1));
+            target += (__int128)other * (l.shape[e] - 1);
+        }
+        if (sums.reach(target)) return false;
     }
     return true;
 }
