@@ -163,6 +163,14 @@ hx_status check_view(const void *buf, uint64_t buf_len, const hx_layout *l, uint
     return HX_OK;
 }
 
+// An operand that may be left out is so by its layout; a buffer without one is
+// not what its caller means.
+hx_status check_left_out(const void *buf, uint64_t buf_len, const hx_layout *l, const char *what) {
+    if (!l && (buf || buf_len))
+        return fail(HX_ERR_INVALID_CONFIGURATION, "%s has a buffer and no layout", what);
+    return HX_OK;
+}
+
 // A whole buffer of `len` elements where `want` are expected.
 hx_status check_vector(const void *buf, uint64_t len, uint64_t want, uint32_t size, const char *what, Span *span) {
     if (len != want) return length_mismatch(want, len);
@@ -205,6 +213,8 @@ hx_status plan_norm(hx_dtype dtype, const void *x, uint64_t x_buf_len, const hx_
     const uint64_t shape[2] = {x_layout->shape[0], x_layout->shape[1]};
     Span sx, sr, sw, so, sq, ss;
     HX_TRY(check_view(x, x_buf_len, x_layout, 2, shape, size, false, "norm input", &sx));
+    HX_TRY(check_left_out(residual, residual_buf_len, residual_layout, "residual"));
+    HX_TRY(check_left_out(residual_out, residual_out_buf_len, residual_out_layout, "residual output"));
     if (residual_layout)
         HX_TRY(check_view(residual, residual_buf_len, residual_layout, 2, shape, size, false, "residual", &sr));
     HX_TRY(check_vector(weight, weight_len, shape[1], size, "norm weight", &sw));
@@ -350,6 +360,8 @@ hx_status plan_attention(hx_dtype dtype, const void *q, uint64_t q_buf_len, cons
                     (unsigned long long)kMaxAttentionDk, (unsigned long long)dk);
     HX_TRY(check_vector(log_decay, log_decay_len, heads, 4, "log decay", &sd));
     if (lengths || lengths_len) HX_TRY(check_vector(lengths, lengths_len, batch, 4, "sequence lengths", &sl));
+    HX_TRY(check_left_out(state_in, state_in_buf_len, state_in_layout, "attention state"));
+    HX_TRY(check_left_out(state_out, state_out_buf_len, state_out_layout, "attention state output"));
     if (state_in_layout)
         HX_TRY(check_view(state_in, state_in_buf_len, state_in_layout, 4, s_shape, 4, false, "attention state", &si));
     if (state_out_layout)

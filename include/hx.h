@@ -520,8 +520,11 @@ hx_status hx_vector_binary(hx_device *dev, hx_vector_op op, hx_dtype dtype,
  * taken in 32 bits either way.  Operands are strided views whose last
  * dimension is contiguous (stride 1, or an extent of at most 1); other
  * strides are free, zero and negative ones included, at any alignment of
- * the elements.  Outputs must not overlap themselves, each other or an
- * input, except where stated.  Empty outputs are a no-op. */
+ * the elements.  Outputs must not share an element with themselves, each other
+ * or an input, except where stated; they may lie between another view's rows
+ * (views too tangled to tell are refused).  An operand that may be NULL is
+ * left out by a NULL layout, and its buffer must then be NULL too.  Empty
+ * outputs are a no-op. */
 
 /* Rows of a residual stream, normalised and quantised in one pass over the
  * data.  x is [rows, cols]:

@@ -160,3 +160,17 @@ def test_views_too_tangled_to_decide_are_refused():
                    output=view(0x5000000, Layout.c_contiguous([200, 1, 200, 2]), F), log_decay=buffer(0x4000000, 200, F),
                    lengths=None, state_in=view(0x10000000, first, F, n), state_out=view(0x10000000, last, F, n))
     assert said is None or "view of the state" in said
+
+
+@pytest.mark.parametrize("call,at,what", [(norm, "residual", "residual"), (norm, "residual_out", "residual output"),
+                                          (attention, "state_in", "attention state"),
+                                          (attention, "state_out", "attention state output")])
+def test_a_buffer_without_a_layout_is_refused(monkeypatch, call, at, what):
+    """It would be left out without a word: h without the residual, an empty state."""
+    from hephaestus_amd import layer_ops
+
+    plain = layer_ops._view
+    lost = view(0x9000000, Layout.c_contiguous([2]), F)
+    monkeypatch.setattr(layer_ops, "_view", lambda v: (*plain(v)[:2], None) if v is lost else plain(v))
+    monkeypatch.setattr(layer_ops, "_typed", lambda *_: None)
+    assert refusal(call, **{at: lost}) == f"invalid configuration: {what} has a buffer and no layout"
