@@ -3,6 +3,7 @@
 #pragma once
 
 #include "../../include/hx.h"
+#include "layer_forms.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -382,47 +383,10 @@ hx_status launch_vector_op(hx_vector_op op, const float *t, const float *s, floa
 // current device.  `allowed` remembers the devices, a bit each.
 hx_status allow_lds(const void *kernel, uint32_t bytes, std::atomic<uint64_t> &allowed);
 
-// Layer operators (layer_ops.cpp checks, then launches).  Pointers are to the
-// first element of each view, strides count elements; the last dimension of
-// every view has stride 1.
-struct NormArgs {
-    hx_dtype dtype;
-    const void *x, *residual, *weight; // residual may be null
-    void *residual_out;                // may be null
-    int8_t *quantized;
-    float *scales;
-    uint64_t rows, cols;
-    int64_t x_stride, residual_stride, residual_out_stride, quantized_stride;
-    float epsilon;
-};
+// Layer operators: layer_forms.hpp has their arguments and which kernel takes a call.
 hx_status launch_norm_quantize(const NormArgs &args, hipStream_t stream);
-
-struct MatmulArgs {
-    hx_dtype dtype; // of out
-    const int8_t *a, *b;
-    const float *a_scales, *b_scales;
-    void *out;
-    uint64_t m, n, k;
-    int64_t a_stride, b_stride, out_stride;
-};
 uint64_t matmul_i8_workspace_bytes(const MatmulArgs &args);
 hx_status launch_matmul_i8(const MatmulArgs &args, void *ws, hipStream_t stream);
-
-struct AttentionView {
-    int64_t batch, token, head; // strides; of a state `token` is the stride of dk
-};
-struct AttentionArgs {
-    hx_dtype dtype;
-    const void *q, *k, *v;
-    void *out;
-    const float *log_decay;
-    const float *state_in; // may be null
-    float *state_out;      // may be null
-    const uint32_t *lengths; // may be null
-    uint64_t batch, tokens, heads, kv_heads, dk, dv;
-    AttentionView sq, sk, sv, so, si, st; // q, k, v, out, state_in, state_out
-    float scale;
-};
 uint64_t linear_attention_workspace_bytes(const AttentionArgs &args);
 hx_status launch_linear_attention(const AttentionArgs &args, void *ws, hipStream_t stream);
 
@@ -443,7 +407,6 @@ hx_status launch_fill_random(void *dst, uint64_t n, hx_dtype dtype,
                              double p1, hipStream_t stream);
 
 // Grid sizing shared by the launchers.
-inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 } // namespace hx
 

@@ -70,8 +70,6 @@ template <bool NT> __device__ __forceinline__ void store4(float *row, uint32_t c
 // memory may be under way.
 __device__ __forceinline__ void meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-constexpr uint64_t kStreamedBytes = 64ull << 20;
-
 // A block takes COLUMNS columns of a state, four a lane, and all its rows, ROWS
 // neighbours a lane: dk at most ROWS·1024 / COLUMNS.  Registers for four waves a SIMD:
 // 32 x 32 heads of 64 x 64 take 8.4 us so and 9.8 without the bound, 50 x 4 of 256 x
@@ -149,9 +147,7 @@ __global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_ke
 
 template <typename T, int COLUMNS, int ROWS> hx_status launch_step(const AttentionArgs &a, hipStream_t stream) {
     const dim3 grid((uint32_t)ceil_div(a.dv, COLUMNS), (uint32_t)a.heads, (uint32_t)a.batch);
-    // States that the caches cannot hold until the next token are streamed.
-    const bool nt = a.batch * a.heads * a.dk * a.dv * sizeof(float) > kStreamedBytes;
-    if (nt) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true>), grid, dim3(256), 0, stream, a);
+    if (attention_streams_state(a)) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, false>), grid, dim3(256), 0, stream, a);
     return check_launch("attention_step_kernel");
 }
@@ -471,12 +467,6 @@ template <int N> __device__ __forceinline__ void meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
-// A prompt cut into `parts` of `span` tokens each, a multiple of the chunk.
-struct Parts {
-    uint32_t parts, span;
-    float *states; // [batch, heads, parts, dk, dv]: each part's own sum, then the state before it
-};
-
 template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT> struct Chunk {
     static constexpr int C = sizeof(T) == 2 ? 64 : 32, B = C / 16, // tokens, and sixteens of them
                           kThreads = NW * kWave, DV = NW * 16;
@@ -502,7 +492,7 @@ template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT> struct Chunk {
 // OUTPUTS: the outputs of a part, from the state before it.  Otherwise only the
 // part's own sum, from nothing.
 template <typename T, int DK, int NW, bool OUTPUTS, bool DIRECT>
-__global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWavesPerSimd)) void attention_chunk_kernel(AttentionArgs a, Parts parts) {
+__global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWavesPerSimd)) void attention_chunk_kernel(AttentionArgs a, AttentionParts parts) {
     using G = Chunk<T, DK, NW, OUTPUTS, DIRECT>;
     using F = typename Fragment<T>::type;
     constexpr int C = G::C, B = G::B, S = G::S, WK = G::WK, DV = G::DV;
@@ -801,7 +791,7 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
 // the state a thread, the parts in order, sixteen of them loaded together.  V is 4
 // where rows are whole fours: 2 x 32 heads of 128 x 128 in four parts take 8.4 us
 // so, 12.3 with one element a thread.
-template <int V> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Parts parts) {
+template <int V> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, AttentionParts parts) {
     typedef float Values __attribute__((ext_vector_type(V), aligned(4)));
     const uint32_t n = (uint32_t)(a.dk * a.dv), i = (blockIdx.x * 256 + threadIdx.x) * V;
     if (i >= n) return;
@@ -841,44 +831,9 @@ template <int V> __global__ __launch_bounds__(256) void attention_join_kernel(At
     if (a.state_out) *(Values *)(a.state_out + b * a.st.batch + h * a.st.head + row * a.st.token + col) = s;
 }
 
-// Waves a block, each with 16 columns of v: with wider keys than 128, two chunks
-// of q, k and 128 columns of v would not fit LDS.
-uint32_t block_waves(const AttentionArgs &a) { return a.dv <= 64 || a.dk > 128 ? 4 : 8; }
-
-// How many parts a prompt is cut into where there are fewer heads than the card
-// takes blocks.  The parts run side by side, but their own sums have to be taken
-// first, in half the time of the outputs, and their states written, joined and
-// read.  Times in us as measured: a chunk 4.7 for heads of 128 x 128 (6.2 in f32,
-// of 32 tokens), 3.0 for 64 x 64; two more launches 12; the states 5 TB/s.
-//   1 x 16 x 16384 tokens, 16 parts  121, uncut 860
-//   1 x  8 x 512,           8 parts   21, uncut  32
-//   4 x 16 x 512,           4 parts   39, uncut  35
-//   2 x 64 x 4096 of 64 x 64, 4 parts 115, 2 parts 148, uncut 184
-//   2 x 64 x 512, the same in f32, 4 parts 48, 2 parts 54
-Parts parts_of(const AttentionArgs &a) {
-    const bool f32 = a.dtype == HX_DTYPE_F32;
-    const uint64_t chunk = f32 ? 32 : 64, chunks = ceil_div(a.tokens, chunk);
-    const uint64_t blocks = a.batch * a.heads * ceil_div(a.dv, 16 * block_waves(a));
-    // Blocks of the narrowest heads take half a CU's LDS.
-    const uint64_t card = a.dk <= 64 && a.dv <= 64 ? 512 : 256;
-    const double area = (double)(a.dk * a.dv) / (128 * 128), chunk_us = 2.4 + (f32 ? 3.8 : 2.3) * area;
-    uint64_t best = 1;
-    double best_us = chunks * chunk_us;
-    for (uint64_t parts = 2; parts <= std::min(chunks, card / blocks); ++parts) {
-        const double states_us = (double)(a.batch * a.heads * parts) * area * (128 * 128 * 16) / 5e6;
-        const double us = ceil_div(chunks, parts) * 1.5 * chunk_us + 12 + states_us;
-        if (us < best_us) {
-            best_us = us;
-            best = parts;
-        }
-    }
-    const uint64_t span = ceil_div(chunks, best) * chunk;
-    return Parts{(uint32_t)ceil_div(a.tokens, span), (uint32_t)span, nullptr};
-}
-
 template <typename T, int DK, int NW, bool DIRECT>
 hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    Parts parts = parts_of(a);
+    AttentionParts parts = attention_parts(a);
     parts.states = (float *)ws;
     const auto run = [&](auto outputs) {
         using G = Chunk<T, DK, NW, decltype(outputs)::value, DIRECT>;
@@ -901,12 +856,6 @@ hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
     return run(std::true_type{});
 }
 
-// Whether the rows of a chunk can be loaded without registers (Stager).
-template <typename T> bool direct_rows(const void *base, const AttentionView &s, uint64_t width) {
-    const uint64_t bits = (uintptr_t)base | (uint64_t)(s.token | s.head | s.batch) * sizeof(T);
-    return bits % 4 == 0 && width % (16 / sizeof(T)) == 0 && s.token >= 0 && s.token < 1 << 24;
-}
-
 template <typename T, int NW, bool DIRECT> hx_status launch_width(const AttentionArgs &a, void *ws, hipStream_t stream) {
     if (a.dk <= 64) return launch_chunks<T, 64, NW, DIRECT>(a, ws, stream);
     if (a.dk <= 96) return launch_chunks<T, 96, NW, DIRECT>(a, ws, stream);
@@ -915,24 +864,12 @@ template <typename T, int NW, bool DIRECT> hx_status launch_width(const Attentio
     return fail(HX_ERR_DISPATCH_FAILED, "no attention block for keys of width %llu", (unsigned long long)a.dk);
 }
 template <typename T, bool DIRECT> hx_status launch_chunked(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    return block_waves(a) == 4 ? launch_width<T, 4, DIRECT>(a, ws, stream) : launch_width<T, 8, DIRECT>(a, ws, stream);
-}
-
-// A few tokens go through the recurrence.  Its time grows with each, that of a
-// chunk does not (us, recurrence and chunk):
-//   1 x 32 heads of 128 x 128    4 tokens 6.4, 11.0    8 tokens 9.5, 11.5     10 tokens 11.4, 11.0
-//   32 x 32, the same            34.4, 51.2            48.5, 51.6             55.9, 50.6
-//   32 x 32, the same in f32     37.6, 72.3            12 tokens 64.1, 70.8   16 tokens 77.3, 71.3
-//   8 x 32 heads of 64 x 64      6.5, 8.0              6 tokens 8.2, 8.2      8 tokens 9.9, 8.0
-bool by_chunks(const AttentionArgs &a) {
-    return a.tokens > (a.dk <= 64 ? 6 : a.dtype == HX_DTYPE_F32 ? 12 : 8) && a.dk > 0;
+    return attention_waves(a) == 4 ? launch_width<T, 4, DIRECT>(a, ws, stream) : launch_width<T, 8, DIRECT>(a, ws, stream);
 }
 
 template <typename T> hx_status launch(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    if (by_chunks(a)) {
-        const bool direct = direct_rows<T>(a.q, a.sq, a.dk) && direct_rows<T>(a.k, a.sk, a.dk) &&
-                            direct_rows<T>(a.v, a.sv, a.dv);
-        return direct ? launch_chunked<T, true>(a, ws, stream) : launch_chunked<T, false>(a, ws, stream);
+    if (attention_by_chunks(a)) {
+        return attention_is_direct(a) ? launch_chunked<T, true>(a, ws, stream) : launch_chunked<T, false>(a, ws, stream);
     }
     return launch_steps<T>(a, stream);
 }
@@ -940,8 +877,8 @@ template <typename T> hx_status launch(const AttentionArgs &a, void *ws, hipStre
 } // namespace
 
 uint64_t linear_attention_workspace_bytes(const AttentionArgs &args) {
-    if (args.batch == 0 || args.heads == 0 || args.dv == 0 || !by_chunks(args)) return 0;
-    const Parts parts = parts_of(args);
+    if (args.batch == 0 || args.heads == 0 || args.dv == 0 || !attention_by_chunks(args)) return 0;
+    const AttentionParts parts = attention_parts(args);
     return parts.parts > 1 ? args.batch * args.heads * parts.parts * args.dk * args.dv * sizeof(float) : 0;
 }
 

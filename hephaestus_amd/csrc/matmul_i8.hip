@@ -28,7 +28,7 @@ namespace {
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kDepth = 128; // bytes of k a step
+constexpr int kDepth = kMatmulDepth;
 
 __device__ __forceinline__ i32x4v mma(i32x4v b, i32x4v a, i32x4v sum) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, sum, 0, 0, 0);
@@ -204,9 +204,7 @@ template <typename T, int MF, bool DWORDS> hx_status launch_skinny(const MatmulA
     const auto run = [&](auto kernel, uint64_t channels) {
         hipLaunchKernelGGL(kernel, dim3((uint32_t)ceil_div(p.n, channels)), dim3(kSkinnyWaves * kWave), 0, stream, p);
     };
-    // Two fragments of channels a block halve its reads of a, from the size
-    // on where there is a block for each CU all the same.
-    if (p.n >= 2 * 16 * 256) run(matmul_skinny_kernel<T, MF, 2, DWORDS>, 32);
+    if (skinny_is_wide(p.n)) run(matmul_skinny_kernel<T, MF, 2, DWORDS>, 32);
     else run(matmul_skinny_kernel<T, MF, 1, DWORDS>, 16);
     return check_launch("matmul_skinny_kernel");
 }
@@ -380,44 +378,22 @@ hx_status launch_tiles(const MatmulArgs &p, hipStream_t stream) {
     return check_launch("matmul_tiles_kernel");
 }
 
-// The largest tile of which there are enough for the 256 CUs: a smaller tile
-// moves more bytes to the same CUs.  Where there are more tiles than CUs two
-// blocks share one, with LDS for half the steps in flight.  A last round of the
-// largest tiles that leaves most CUs idle costs more than they gain: two blocks
-// of 128 x 128 on each CU take 0.54 of the time of one of 256 x 256.  Groups that share a
-// block's k keep more loads under way in a block, for about 2 us to add their
-// sums: worth it for long rows, or where tiles are too few to fill the card.
-// Measured (us):
-//   8192 x 8192 x 1024   256 x 256 123     128 x 128 143
-//   831 x 14912 x 1792   256 x 256 39.5    128 x 128 41.4
-//   6144 x 6144 x 6144   256 x 256 280     128 x 128 253     (2.25 rounds, 4.5)
-//   1308 x 11648 x 2624  256 x 256 83.9    128 x 128 48.4    (1.08 rounds, 1.96)
-//   1000 x 8192 x 8192   128 x 128 71.1    64 x 64 109     256 x 256 115
-//   2048 x 2048 x 2048   128 x 128 16.6    64 x 64 19.0    256 x 256 37.8
-//   1500 x 1500 x 8192    96 x  96 28.6    64 x 64 39.2
-//   128 x 8192 x 4096     64 x  64 10.9 in three groups, 11.8 in one
-//   700 x 1500 x 1500     64 x  64 22.5 in three groups, 12.6 in one
-//   256 x 1024 x 8192     32 x  32 10.2    64 x 32 13.5    64 x 64 17.4
-//   20 x 4096 x 4096      32 x  16 6.0     32 x 32 7.0     64 x 32 8.3
 template <typename T> hx_status launch_tiled(const MatmulArgs &p, hipStream_t stream) {
-    const auto tiles = [&](uint64_t bm, uint64_t bn) { return ceil_div(p.m, bm) * ceil_div(p.n, bn); };
-    constexpr uint64_t kCus = 256, kEnough = 160, kFull = 192;
-    const bool long_rows = p.k >= 4096;
-    const uint64_t rounds = ceil_div(tiles(256, 256), kCus), pairs = ceil_div(tiles(128, 128), 2 * kCus);
-    if (tiles(256, 256) >= kEnough && rounds <= 0.54 * pairs)
-        return launch_tiles<T, 256, 256, 2, 4, 1, 2>(p, stream);
-    if (tiles(128, 128) > kCus) return launch_tiles<T, 128, 128, 2, 2, 1, 2>(p, stream);
-    if (tiles(128, 128) >= kFull) return launch_tiles<T, 128, 128, 2, 4, 1, 4>(p, stream);
-    if (long_rows && tiles(96, 96) >= kFull && tiles(96, 96) <= kCus)
-        return launch_tiles<T, 96, 96, 2, 2, 2, 3>(p, stream);
-    if (long_rows && tiles(64, 64) >= kEnough && tiles(64, 64) <= kCus)
-        return launch_tiles<T, 64, 64, 2, 2, 3, 3>(p, stream);
-    if (tiles(64, 64) >= kEnough) return launch_tiles<T, 64, 64, 4, 2, 1, 4>(p, stream);
-    if (tiles(64, 32) > kCus) return launch_tiles<T, 64, 32, 2, 1, 3, 2>(p, stream);
-    if (tiles(64, 32) >= kEnough) return launch_tiles<T, 64, 32, 2, 1, 6, 2>(p, stream);
-    if (tiles(32, 32) > kCus) return launch_tiles<T, 32, 32, 1, 2, 4, 2>(p, stream);
-    if (tiles(32, 32) >= kEnough) return launch_tiles<T, 32, 32, 1, 2, 8, 2>(p, stream);
-    return launch_tiles<T, 32, 16, 1, 1, 8, 3>(p, stream);
+    switch (matmul_tile(p.m, p.n, p.k)) {
+    case MatmulTile::k256x256: return launch_tiles<T, 256, 256, 2, 4, 1, 2>(p, stream);
+    case MatmulTile::k128x128Pairs: return launch_tiles<T, 128, 128, 2, 2, 1, 2>(p, stream);
+    case MatmulTile::k128x128: return launch_tiles<T, 128, 128, 2, 4, 1, 4>(p, stream);
+    case MatmulTile::k96x96: return launch_tiles<T, 96, 96, 2, 2, 2, 3>(p, stream);
+    case MatmulTile::k64x64Groups: return launch_tiles<T, 64, 64, 2, 2, 3, 3>(p, stream);
+    case MatmulTile::k64x64: return launch_tiles<T, 64, 64, 4, 2, 1, 4>(p, stream);
+    case MatmulTile::k64x32Pairs: return launch_tiles<T, 64, 32, 2, 1, 3, 2>(p, stream);
+    case MatmulTile::k64x32: return launch_tiles<T, 64, 32, 2, 1, 6, 2>(p, stream);
+    case MatmulTile::k32x32Pairs: return launch_tiles<T, 32, 32, 1, 2, 4, 2>(p, stream);
+    case MatmulTile::k32x32: return launch_tiles<T, 32, 32, 1, 2, 8, 2>(p, stream);
+    case MatmulTile::k32x16: return launch_tiles<T, 32, 16, 1, 1, 8, 3>(p, stream);
+    }
+    return fail(HX_ERR_DISPATCH_FAILED, "no tile for a matmul of %llu x %llu", (unsigned long long)p.m,
+                (unsigned long long)p.n);
 }
 
 // ----------------------------------------------------------- rows on dwords
@@ -435,22 +411,6 @@ __global__ __launch_bounds__(256) void matmul_align_kernel(MatmulArgs p, int8_t 
         *(i32x4v *)(rows + r * pitch + at) = load_bytes(from, at, (uint32_t)p.k);
     }
 }
-
-// Up to 16 tokens take the form that reads rows as they lie.  Up to 32 do where
-// rows lie off dwords, so that tiles would need a copy first, unless a few blocks
-// would have long rows to read (us, so and by copy and tiles):
-//   20 x 8192 x 16384   46.2, 87.2     32 x 8192 x 16384   52.3, 89.0
-//   20 x 4096 x 4097     9.7, 13.3     32 x 4096 x 4097    11.1, 13.2
-//   20 x 1000 x 1001     4.0,  7.7     32 x 16384 x 600     6.3, 11.1
-//   20 x 100 x 16384    24.4, 12.3     64 x 4096 x 4097    16.8, 14.4
-bool off_dwords(const MatmulArgs &p) {
-    return ((uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.a_stride | (uint64_t)p.b_stride) % 4 != 0;
-}
-bool is_skinny(const MatmulArgs &p) {
-    return p.m <= 16 || (p.m <= 32 && off_dwords(p) && (p.k <= 4096 || p.n >= 4096));
-}
-bool needs_copy(const MatmulArgs &p) { return !is_skinny(p) && p.k > 0 && off_dwords(p); }
-uint64_t copy_pitch(const MatmulArgs &p) { return ceil_div(p.k, kDepth) * kDepth; }
 
 // A launch has fewer than 2^32 threads: 16 a channel for a few tokens, up to 12 a
 // channel or 2 a token in tiles.  More channels or tokens take several launches.
@@ -472,14 +432,14 @@ template <typename T, typename F> hx_status in_parts(const MatmulArgs &p, F run)
 }
 
 template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t stream) {
-    if (is_skinny(p))
+    if (matmul_is_skinny(p))
         return in_parts<T>(p, [&](const MatmulArgs &part) {
-            if (!off_dwords(p)) return launch_skinny<T, 1, true>(part, stream);
+            if (!matmul_off_dwords(p)) return launch_skinny<T, 1, true>(part, stream);
             if (p.m <= 16) return launch_skinny<T, 1, false>(part, stream);
             return launch_skinny<T, 2, false>(part, stream);
         });
-    if (needs_copy(p)) {
-        const uint32_t pitch = (uint32_t)copy_pitch(p);
+    if (matmul_needs_copy(p)) {
+        const uint32_t pitch = (uint32_t)matmul_copy_pitch(p);
         const uint64_t blocks = min(ceil_div((p.m + p.n) * (pitch / 16), 256), (uint64_t)1 << 22);
         hipLaunchKernelGGL(matmul_align_kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, p, (int8_t *)ws, pitch);
         HX_TRY(check_launch("matmul_align_kernel"));
@@ -494,7 +454,7 @@ template <typename T> hx_status launch(MatmulArgs p, void *ws, hipStream_t strea
 } // namespace
 
 uint64_t matmul_i8_workspace_bytes(const MatmulArgs &args) {
-    return args.m && args.n && needs_copy(args) ? (args.m + args.n) * copy_pitch(args) : 0;
+    return args.m && args.n && matmul_needs_copy(args) ? (args.m + args.n) * matmul_copy_pitch(args) : 0;
 }
 
 hx_status launch_matmul_i8(const MatmulArgs &args, void *ws, hipStream_t stream) {
