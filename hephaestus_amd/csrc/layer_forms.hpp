@@ -160,6 +160,9 @@ inline bool attention_is_direct(const AttentionArgs &a) {
 // of q, k and 128 columns of v would not fit LDS.
 inline uint32_t attention_waves(const AttentionArgs &a) { return a.dv <= 64 || a.dk > 128 ? 4 : 8; }
 
+// The keys' width that a kernel is made for.
+inline uint32_t attention_key_width(uint64_t dk) { return dk <= 64 ? 64 : dk <= 96 ? 96 : dk <= 128 ? 128 : 256; }
+
 // A prompt cut into `parts` of `span` tokens each, a multiple of the chunk.
 struct AttentionParts {
     uint32_t parts, span;
@@ -169,25 +172,30 @@ struct AttentionParts {
 // How many parts a prompt is cut into where there are fewer heads than the card
 // takes blocks.  The parts run side by side, but their own sums have to be taken
 // first, in half the time of the outputs, and their states written, joined and
-// read.  Times in us as measured: a chunk 4.7 for heads of 128 x 128 (6.2 in f32,
-// of 32 tokens), 3.0 for 64 x 64; two more launches 12; the states 5 TB/s.
-//   1 x 16 x 16384 tokens, 16 parts  121, uncut 860
-//   1 x  8 x 512,           8 parts   21, uncut  32
-//   4 x 16 x 512,           4 parts   39, uncut  35
-//   2 x 64 x 4096 of 64 x 64, 4 parts 115, 2 parts 148, uncut 184
-//   2 x 64 x 512, the same in f32, 4 parts 48, 2 parts 54
+// read.  Times in us as measured: a chunk of bf16 3.0, 4.2 and 6.6 for keys of 64,
+// 128 and 256, whatever the columns (LDS reads of q and k); of f32 3.0 to 6.9 for
+// 64 x 64 to 128 x 128 a block (matrix instructions); two more launches 7.5; the
+// states 7 TB/s.  Heads x tokens of keys x columns, us:
+//   16 x 16384 of 128 x 128, 16 parts 124, 8 parts 195, uncut 1003
+//   64 x 512, the same, 4 parts 36.5, 2 parts 40.0, uncut 38.4
+//   8 x 256 of 128 x 2048, 2 parts 34.6, uncut 25.1
+//   16 x 256 and 16 x 192 of 128 x 128, one chunk a part 20.7 and 20.1, uncut 21.6 and 17.9
+//   8 x 256 of 64 x 64, 4 parts 16.5, uncut 14.7;  8 x 384, 6 parts 16.1, uncut 19.7
+//   128 x 4096, the same, 4 parts 113, 2 parts 145, uncut 201
+//   8 x 128 of 128 x 1024 in f32, 4 parts 32.0, 2 parts 37.7, uncut 34.7
 inline AttentionParts attention_parts(const AttentionArgs &a) {
     const bool f32 = a.dtype == HX_DTYPE_F32;
-    const uint64_t chunk = f32 ? 32 : 64, chunks = ceil_div(a.tokens, chunk);
-    const uint64_t blocks = a.batch * a.heads * ceil_div(a.dv, 16 * attention_waves(a));
+    const uint64_t chunk = f32 ? 32 : 64, chunks = ceil_div(a.tokens, chunk), columns = 16 * attention_waves(a);
+    const uint64_t blocks = a.batch * a.heads * ceil_div(a.dv, columns);
     // Blocks of the narrowest heads take half a CU's LDS.
     const uint64_t card = a.dk <= 64 && a.dv <= 64 ? 512 : 256;
-    const double area = (double)(a.dk * a.dv) / (128 * 128), chunk_us = 2.4 + (f32 ? 3.8 : 2.3) * area;
+    const double width = attention_key_width(a.dk);
+    const double chunk_us = f32 ? 1.7 + 5.2 * (width * columns) / (128 * 128) : 1.8 + 2.4 * width / 128;
     uint64_t best = 1;
     double best_us = chunks * chunk_us;
     for (uint64_t parts = 2; parts <= std::min(chunks, card / blocks); ++parts) {
-        const double states_us = (double)(a.batch * a.heads * parts) * area * (128 * 128 * 16) / 5e6;
-        const double us = ceil_div(chunks, parts) * 1.5 * chunk_us + 12 + states_us;
+        const double states_us = (double)(a.batch * a.heads * parts) * (a.dk * a.dv * 16) / 7e6;
+        const double us = ceil_div(chunks, parts) * 1.5 * chunk_us + 7.5 + states_us;
         if (us < best_us) {
             best_us = us;
             best = parts;

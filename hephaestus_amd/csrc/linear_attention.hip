@@ -857,10 +857,13 @@ hx_status launch_chunks(const AttentionArgs &a, void *ws, hipStream_t stream) {
 }
 
 template <typename T, int NW, bool DIRECT> hx_status launch_width(const AttentionArgs &a, void *ws, hipStream_t stream) {
-    if (a.dk <= 64) return launch_chunks<T, 64, NW, DIRECT>(a, ws, stream);
-    if (a.dk <= 96) return launch_chunks<T, 96, NW, DIRECT>(a, ws, stream);
-    if (a.dk <= 128) return launch_chunks<T, 128, NW, DIRECT>(a, ws, stream);
-    if constexpr (NW == 4) return launch_chunks<T, 256, NW, DIRECT>(a, ws, stream);
+    switch (attention_key_width(a.dk)) {
+    case 64: return launch_chunks<T, 64, NW, DIRECT>(a, ws, stream);
+    case 96: return launch_chunks<T, 96, NW, DIRECT>(a, ws, stream);
+    case 128: return launch_chunks<T, 128, NW, DIRECT>(a, ws, stream);
+    default:
+        if constexpr (NW == 4) return launch_chunks<T, 256, NW, DIRECT>(a, ws, stream);
+    }
     return fail(HX_ERR_DISPATCH_FAILED, "no attention block for keys of width %llu", (unsigned long long)a.dk);
 }
 template <typename T, bool DIRECT> hx_status launch_chunked(const AttentionArgs &a, void *ws, hipStream_t stream) {

@@ -97,3 +97,14 @@ def test_every_width_of_norms_is_reached():
     for elements in (4, 8):
         reached = {sum(-(-cols // elements) > b for b in bounds) for cols in tiny.COLS}
         assert reached == set(range(9))
+
+
+def test_wide_heads_are_not_cut_too_early(rules):
+    """A block has at most 128 columns of v, whatever the head: its chunks take no longer."""
+    for dtype, tokens, heads, dk, dv in (("bf16", 256, 8, 128, 2048), ("bf16", 192, 8, 128, 1024),
+                                         ("bf16", 256, 8, 256, 1024), ("bf16", 128, 4, 256, 1024),
+                                         ("f32", 64, 8, 128, 2048)):
+        assert attention_form(rules, dtype, 1, tokens, heads, dk, dv)[4] == 1
+    for dtype, tokens, heads, dk, dv, parts in (("bf16", 1024, 8, 128, 512, 8), ("bf16", 640, 32, 128, 256, 4),
+                                                ("f32", 512, 8, 128, 512, 8)):
+        assert attention_form(rules, dtype, 1, tokens, heads, dk, dv)[4] == parts
