@@ -402,10 +402,13 @@ __device__ __forceinline__ void load_columns(const char *tile, int i, f32x4v (&t
 // DIRECT: loads that write LDS without registers, for rows that begin on dwords
 // and are whole 16-byte slots.  Every lane loads every time, so that a count of
 // loads under way says which have landed: lanes outside the rows load zeros.
-// Otherwise through registers.
+// Otherwise through registers.  AGAIN: places and addresses are computed anew for
+// each chunk, where the registers do not hold them all: eight waves with keys of
+// 128 in bf16 spilled five a lane (8 x 32 heads of 127 x 127 over 2048 tokens 256
+// us, 236 so; elsewhere it costs 2 to 5%).
 __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIRECT> struct Stager {
+template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIRECT, bool AGAIN> struct Stager {
     using Tile = TileOf<T, WIDTH, BY_ROWS>;
     static constexpr int V = Tile::V, N = ROWS * Tile::kSlots / THREADS;
     static_assert(N * THREADS == ROWS * Tile::kSlots);
@@ -443,9 +446,10 @@ template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIREC
             }
             return;
         }
+        const uint32_t t = AGAIN ? here(threadIdx.x) : threadIdx.x;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t row = row_of(threadIdx.x, i), c = slot_of(threadIdx.x, i) * V;
+            const uint32_t row = row_of(t, i), c = slot_of(t, i) * V;
             if constexpr (!DIRECT) {
                 held[i] = u32x4{0, 0, 0, 0};
                 if (row < rows) held[i] = load_part(base + (int64_t)row * stride, c, width);
@@ -453,11 +457,12 @@ template <typename T, int ROWS, int WIDTH, bool BY_ROWS, int THREADS, bool DIREC
         }
     }
     __device__ __forceinline__ void store(char *tile, uint32_t width) const {
-        if constexpr (!DIRECT)
+        if constexpr (!DIRECT) {
+            const uint32_t t = AGAIN ? here(threadIdx.x) : threadIdx.x;
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                *(u32x4 *)(tile + (threadIdx.x + i * THREADS) * 16) =
-                    place_part<T>(held[i], slot_of(threadIdx.x, i) * V, width);
+                *(u32x4 *)(tile + (t + i * THREADS) * 16) = place_part<T>(held[i], slot_of(t, i) * V, width);
+        }
     }
 };
 
@@ -518,9 +523,10 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
     const auto power = [&](int n) { return __builtin_amdgcn_exp2f(log2_decay * (float)n); };
 
     const uint32_t chunks = begin < end ? (end - begin + C - 1) / C : 0;
-    Stager<T, C, WK, true, G::kThreads, DIRECT> to_q;
-    Stager<T, C, WK, false, G::kThreads, DIRECT> to_k;
-    Stager<T, C, DV, false, G::kThreads, DIRECT> to_v;
+    constexpr bool kAgain = !DIRECT && OUTPUTS && sizeof(T) == 2 && DK == 128 && NW == 8;
+    Stager<T, C, WK, true, G::kThreads, DIRECT, kAgain> to_q;
+    Stager<T, C, WK, false, G::kThreads, DIRECT, kAgain> to_k;
+    Stager<T, C, DV, false, G::kThreads, DIRECT, kAgain> to_v;
     to_k.begin(a.sk.token);
     to_v.begin(a.sv.token);
     if constexpr (OUTPUTS) to_q.begin(a.sq.token);
@@ -543,7 +549,7 @@ __global__ __launch_bounds__(NW *kWave, (Chunk<T, DK, NW, OUTPUTS, DIRECT>::kWav
         const char *tile = stage_of(n) + G::kTileK;
         const uint32_t t0 = begin + n * C;
         T *rows = out + (int64_t)t0 * a.so.token;
-        using ToOut = Stager<T, C, DV, false, G::kThreads, false>;
+        using ToOut = Stager<T, C, DV, false, G::kThreads, false, false>;
         u32x4 held[ToOut::N];
 #pragma unroll
         for (int i = 0; i < ToOut::N; ++i) held[i] = *(const u32x4 *)(tile + (threadIdx.x + i * G::kThreads) * 16);
