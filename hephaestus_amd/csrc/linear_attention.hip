@@ -171,10 +171,10 @@ template <typename T> hx_status launch_steps(const AttentionArgs &a, hipStream_t
 // What bounds a block of bf16 is LDS: every wave reads all of q and k, about 4000
 // of a chunk's 10000 cycles at 64 tokens of 128 x 128, and then the arithmetic of
 // the two and three terms (below).  8 x 32 heads of 128 x 128 over 4096 tokens take
-// 302 us, 1.1 GB at 3.7 TB/s; loads and stores alone took 230.  Chunks of 128 tokens
+// 306 us, 1.1 GB at 3.6 TB/s; loads and stores alone took 230.  Chunks of 128 tokens
 // have no room beside the next one.  In f32 the matrix instructions weigh most, at
 // a sixteenth of the rate of bf16: half of the 6.3 us of a chunk of 32 tokens of
-// 80 x 96 (5 x 12 heads, up to 1000 tokens: 51 us, and 24 for the parts' sums).
+// 80 x 96 (5 x 12 heads, up to 1000 tokens: 49 us, and 23 for the parts' sums).
 //
 // The accumulators of a 16 x 16 product hold, in lane l, column l % 16 and rows
 // 4·(l / 16) + i.  An operand holds, in lane l, row or column l % 16 and the

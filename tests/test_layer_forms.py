@@ -108,3 +108,9 @@ def test_wide_heads_are_not_cut_too_early(rules):
     for dtype, tokens, heads, dk, dv, parts in (("bf16", 1024, 8, 128, 512, 8), ("bf16", 640, 32, 128, 256, 4),
                                                 ("f32", 512, 8, 128, 512, 8)):
         assert attention_form(rules, dtype, 1, tokens, heads, dk, dv)[4] == parts
+
+
+def test_the_prompt_under_capture_is_cut(rules):
+    """The one of tests/test_gpu_layer_streams.py, and the longer one with workspaces."""
+    assert attention_form(rules, "bf16", 1, 300, 2, 64, 48)[4] > 1
+    assert attention_form(rules, "bf16", 1, 2500, 2, 64, 48)[4] > 1
