@@ -6,6 +6,7 @@ import pytest
 
 import hephaestus_amd as hx
 from layer_reference import EPS16, EPS32, as_float64, linear_attention
+from test_gpu_layer_forms import by_pairs
 from test_gpu_linear_attention import operands, run
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +77,24 @@ def test_a_token_is_decayed_as_often_as_it_has_to_be(device, dtype, chunk, chunk
     want = (np.exp(decay.astype(np.float64) * (tokens - 1 - t))[:, None, None]
             * as_float64(k)[0, t, :, :, None] * as_float64(v)[0, t, :, None, :])
     assert abs(bias(last[0], want)) <= 2.0**-27
+
+
+@pytest.mark.parametrize("dtype", [np.float32, hx.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("tokens,heads,dk,dv", [(2048, 300, 32, 32), (512, 300, 32, 32), (2048, 140, 64, 96),
+                                                (4096, 2, 64, 64)])
+def test_long_memories_keep_the_bits_of_f32(device, dtype, tokens, heads, dk, dv):
+    """Heads that remember from four tokens to all, in prompts that are taken
+    whole and (the last) cut into parts of a chunk.  Errors in the norm: rounding an
+    f32 number errs by 0.2·2^-24 of it.  A state is rounded at most twice a chunk
+    and twice a part, at most 256 times: 16·0.2·2^-24; the chunks' own sums and the
+    weights (a unit of exp2 each) add 2^-24 each, in all less than 2^-22.  Outputs
+    in f32 add as much again at most from sums over a chunk and dk."""
+    q, k, v, _, state = operands(dtype, 1, tokens, heads, heads, dk, dv, 24)
+    decay = np.log1p(-(2.0 ** -np.linspace(2, 12, heads))).astype(np.float32)
+    got, last = run(device, q, k, v, decay, state)
+    scale = float(np.float32(dk ** -0.5))
+    for h in sorted({0, heads // 4, heads // 2, 3 * heads // 4, heads - 1}):
+        want, want_last, _, _ = by_pairs(q[0, :, h], k[0, :, h], v[0, :, h], decay[h], scale, state[0, h])
+        assert np.linalg.norm(last[0, h] - want_last) <= 2.0**-22 * np.linalg.norm(want_last), h
+        if dtype == np.float32:
+            assert np.linalg.norm(got[0, :, h] - want) <= 2.0**-21 * np.linalg.norm(want), h
