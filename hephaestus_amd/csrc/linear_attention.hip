@@ -70,6 +70,19 @@ template <bool NT> __device__ __forceinline__ void store4(float *row, uint32_t c
 // memory may be under way.
 __device__ __forceinline__ void meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// The decay of one token as a float and what its rounding leaves out, so that a
+// state keeps the precision of f32 over any number of calls: by the float alone one
+// that remembers 2^10 tokens is off by up to 2^-15.  Where the memory is long the
+// rest comes from the series of e^g - 1; one of 16 tokens needs none.
+struct StepDecay {
+    float by, rest;
+};
+__device__ __forceinline__ StepDecay step_decay(float g) {
+    if (!(g > -0.0625f)) return {expf(g), 0.0f};
+    const float less = g * (1.0f + g * (1.0f / 2 + g * (1.0f / 6 + g * (1.0f / 24)))), by = 1.0f + less;
+    return {by, less - (by - 1.0f)};
+}
+
 // A block takes COLUMNS columns of a state, four a lane, and all its rows, ROWS
 // neighbours a lane: dk at most ROWS·1024 / COLUMNS.  Registers for four waves a SIMD:
 // 32 x 32 heads of 64 x 64 take 8.4 us so and 9.8 without the bound, 50 x 4 of 256 x
@@ -88,7 +101,7 @@ __global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_ke
     const T *k = (const T *)a.k + b * a.sk.batch + hk * a.sk.head;
     const T *v = (const T *)a.v + b * a.sv.batch + hk * a.sv.head;
     T *out = (T *)a.out + b * a.so.batch + h * a.so.head;
-    const float decay = expf(a.log_decay[h]);
+    const float log_decay = a.log_decay[h];
     f32x4 s[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -104,10 +117,14 @@ __global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_ke
         qt = load_run<ROWS>(q + (int64_t)t * a.sq.token, row0, dk);
     };
     if (length) load(0);
+    const StepDecay decay = step_decay(log_decay);
     if (c + 4 > dv)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) s[r] = place_run<4>(s[r], c, dv);
-    for (uint64_t t = 0; t < length; ++t) {
+    // rest: what the token's decay takes off besides.  That of all the call's decays
+    // goes with its first token; a token of the call itself lacks it, 2^-25 for each
+    // of the few that follow.
+    const auto token = [&](uint64_t t, auto rest) {
         vt = place_run<4>(vt, c, dv);
         kt = place_run<ROWS>(kt, row0, dk);
         qt = place_run<ROWS>(qt, row0, dk);
@@ -115,7 +132,7 @@ __global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_ke
         f32x4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            s[r] = decay * s[r] + (float)kt[r] * values;
+            s[r] = decay.by * s[r] + rest(s[r], (float)kt[r] * values);
             // A row past dk adds nothing, whatever the value.
             if (row0 + r < dk) o += (float)qt[r] * s[r];
         }
@@ -133,7 +150,12 @@ __global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_ke
             for (int i = 0; i < 4; ++i)
                 if (c + i < dv) out[(int64_t)t * a.so.token + c + i] = (T)(o[i] * a.scale);
         }
+    };
+    if (length) {
+        const float rest = decay.rest * (float)length;
+        token(0, [&](f32x4 state, f32x4 added) { return rest * state + added; });
     }
+    for (uint64_t t = 1; t < length; ++t) token(t, [](f32x4, f32x4 added) { return added; });
     for (uint64_t t = length + threadIdx.x / kLanes; t < a.tokens; t += 256 / kLanes)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -147,7 +169,12 @@ __global__ __launch_bounds__(256, NT && ROWS < 8 ? 1 : 4) void attention_step_ke
 
 template <typename T, int COLUMNS, int ROWS> hx_status launch_step(const AttentionArgs &a, hipStream_t stream) {
     const dim3 grid((uint32_t)ceil_div(a.dv, COLUMNS), (uint32_t)a.heads, (uint32_t)a.batch);
-    if (attention_streams_state(a)) hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true>), grid, dim3(256), 0, stream, a);
+    // Streams of four rows a lane are faster with five blocks a CU than with six: 31 KiB
+    // of LDS, not used, leave room for five (128 x 32 heads of 128 x 128 96.6 us, 99.2; 40 x
+    // 32 31.3, 32.3; of two rows 96.5, 90.4, of one 77.0, 53.1).
+    const uint32_t lds = ROWS == 4 ? 31 * 1024 : 0;
+    if (attention_streams_state(a))
+        hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, true>), grid, dim3(256), lds, stream, a);
     else hipLaunchKernelGGL((attention_step_kernel<T, COLUMNS, ROWS, false>), grid, dim3(256), 0, stream, a);
     return check_launch("attention_step_kernel");
 }

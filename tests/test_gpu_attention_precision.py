@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import hephaestus_amd as hx
-from layer_reference import EPS16, EPS32, as_float64, linear_attention
+from layer_reference import EPS16, EPS32, as_float64, linear_attention, padded
 from test_gpu_layer_forms import by_pairs
 from test_gpu_linear_attention import operands, run
 
@@ -98,3 +98,28 @@ def test_long_memories_keep_the_bits_of_f32(device, dtype, tokens, heads, dk, dv
         assert np.linalg.norm(last[0, h] - want_last) <= 2.0**-22 * np.linalg.norm(want_last), h
         if dtype == np.float32:
             assert np.linalg.norm(got[0, :, h] - want) <= 2.0**-21 * np.linalg.norm(want), h
+
+
+@pytest.mark.parametrize("dtype", [np.float32, hx.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("tokens,dk", [(1, 16), (3, 16), (1, 48), (1, 100), (1, 200)])
+def test_single_tokens_decay_without_drift(device, dtype, tokens, dk):
+    """2000 calls on a state in place, with no values: a decay that is a float alone
+    is off by up to 2^-25 a token, 2^-14 in the end.  e^g - 1, below 2^-8 here, is
+    within two units of its own last place, 2^-30 a token: 2^-19 in 2000."""
+    calls, heads = 2000, 40
+    q, k, v, _, state = operands(dtype, 1, tokens, heads, heads, dk, 16, 25)
+    decay = np.log1p(-(2.0 ** -np.random.default_rng(dk).uniform(8.5, 11, heads))).astype(np.float32)
+    off = np.exp(decay.astype(np.float64)) - np.exp(decay.astype(np.float64)).astype(np.float32)
+    assert np.abs(off).max() > 2.0**-26  # of a decay near 1: there is something to make good
+    v = np.zeros_like(v)
+    (vq, _), (vk, _), (vv, _), (vs, read) = (padded(device, x) for x in (q, k, v, state))
+    vo, _ = padded(device, v)
+    plan = hx.RocmLinearAttentionOps().prepare_linear_attention(device, vq, vk, vv, device.upload(decay), vo,
+                                                                state_in=vs, state_out=vs)
+    for _ in range(calls):
+        plan.dispatch()
+    device.synchronize()
+    last = read()
+    for h in range(heads):
+        want = np.exp(decay[h].astype(np.float64) * tokens * calls) * state[0, h]
+        assert abs(bias(last[0, h], want)) <= tokens * 2.0**-19, h
