@@ -8,8 +8,8 @@
 // elements and a sum over the rows: within the wave by lane exchange, across the
 // four waves through LDS (two buffers in turn, so one barrier a token); the next
 // token's elements are on their way meanwhile.  The state's bytes, in and out,
-// bound it: 128 sequences of 32 heads of 128 x 128 take 97 us, 5.6 TB/s; 50 of 4
-// heads of 256 x 128 10.8.  Blocks of 64 or 128 columns, with whole rows of the
+// bound it: 128 sequences of 32 heads of 128 x 128 take 96 us, 5.6 TB/s; 50 of 4
+// heads of 256 x 128 10.2.  Blocks of 64 or 128 columns, with whole rows of the
 // state side by side but more registers, took 154 and 95 us, and for one
 // sequence of 16 heads 6.3 and 6.8 us against 4.7.
 //
@@ -17,7 +17,6 @@
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 
-#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
