@@ -1,8 +1,9 @@
 """hephaestus_amd — MI355X (gfx950) backend for Hephaestus's reduction / scan
 path: full and row-wise reduce (sum, max, argmax, ...), inclusive and
 exclusive prefix scans, segmented sum and the fused y = fmaf(a, x, b)
-prologue, and the operators of a linear-attention layer served in 8 bits
-(layer_ops.py), as hand-written HIP kernels behind the C ABI of include/hx.h.
+prologue, the operators of a linear-attention layer served in 8 bits
+(layer_ops.py) and those that a scan-type model is trained with
+(training_ops.py), as hand-written HIP kernels behind the C ABI of include/hx.h.
 
 This package is the Python host side of that ABI.  It has no compute path of
 its own: every operation is a call into the native library, which must have
@@ -36,6 +37,7 @@ from .errors import (
 )
 from .layer_ops import RocmLinearAttentionOps, RocmMatrixOps, RocmNormOps
 from .layout import Layout, StridedView
+from .training_ops import NO_TARGET, RocmLayerNormOps, RocmLossOps, RocmRecurrenceOps
 from .vector_ops import (
     PreparedMapReduction,
     RocmDenseVectorOps,

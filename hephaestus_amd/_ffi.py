@@ -181,6 +181,28 @@ SIGNATURES = {
                                   P, U64, P, U64, LP, P]),
     "hx_prepare_linear_attention": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, c_float, P, U64, LP, P,
                                           U64, LP, P, U64, P, U64, LP, POINTER(P)]),
+    "hx_layer_norm": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, c_float, P, U64, LP, P, U64, LP, P, U64,
+                            P, U64, P]),
+    "hx_prepare_layer_norm": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, c_float, P, U64, LP, P, U64, LP,
+                                    P, U64, P, U64, POINTER(P)]),
+    "hx_layer_norm_backward": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, P, U64, P, U64, LP, P, U64, LP,
+                                     P, U64, P, U64, P]),
+    "hx_prepare_layer_norm_backward": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, P, U64, P, U64, LP, P,
+                                             U64, LP, P, U64, P, U64, POINTER(P)]),
+    "hx_gated_recurrence": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, P, U64, LP, P, U64, LP, P]),
+    "hx_prepare_gated_recurrence": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, P, U64, LP, P, U64, LP,
+                                          POINTER(P)]),
+    "hx_gated_recurrence_backward": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, P, U64, LP,
+                                           P, U64, LP, P, U64, LP, P, U64, LP, P, U64, LP, P]),
+    "hx_prepare_gated_recurrence_backward": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, P,
+                                                   U64, LP, P, U64, LP, P, U64, LP, P, U64, LP, P, U64, LP,
+                                                   POINTER(P)]),
+    "hx_linear_cross_entropy": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, P, U64, P]),
+    "hx_prepare_linear_cross_entropy": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, P, U64, POINTER(P)]),
+    "hx_linear_cross_entropy_backward": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, P, U64, P, U64, LP, P,
+                                               U64, LP, P]),
+    "hx_prepare_linear_cross_entropy_backward": (I32, [P, I32, P, U64, LP, P, U64, LP, P, U64, P, U64, P, U64, P, U64,
+                                                       LP, P, U64, LP, POINTER(P)]),
     "hx_plan_dispatch": (I32, [P, P]),
     "hx_plan_dispatch_batch": (I32, [P, U64, P]),
     "hx_plan_destroy": (I32, [P]),

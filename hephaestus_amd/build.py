@@ -36,6 +36,10 @@ SOURCES = [
     "csrc/norm_quantize.hip",
     "csrc/matmul_i8.hip",
     "csrc/linear_attention.hip",
+    "csrc/training_ops.cpp",
+    "csrc/layer_norm.hip",
+    "csrc/gated_recurrence.hip",
+    "csrc/cross_entropy.hip",
 ]
 HEADERS = ["csrc/hx_device.hpp", "csrc/hx_internal.hpp"]
 ARCH = "gfx950"

@@ -3,7 +3,7 @@
 #pragma once
 
 #include "../../include/hx.h"
-#include "layer_forms.hpp"
+#include "training_forms.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -389,6 +389,19 @@ uint64_t matmul_i8_workspace_bytes(const MatmulArgs &args);
 hx_status launch_matmul_i8(const MatmulArgs &args, void *ws, hipStream_t stream);
 uint64_t linear_attention_workspace_bytes(const AttentionArgs &args);
 hx_status launch_linear_attention(const AttentionArgs &args, void *ws, hipStream_t stream);
+
+// Training operators: training_forms.hpp has theirs.
+hx_status launch_layer_norm(const LayerNormArgs &args, hipStream_t stream);
+uint64_t layer_norm_grad_workspace_bytes(const LayerNormGradArgs &args);
+hx_status launch_layer_norm_grad(const LayerNormGradArgs &args, void *ws, hipStream_t stream);
+uint64_t gated_recurrence_workspace_bytes(const RecurrenceArgs &args);
+hx_status launch_gated_recurrence(const RecurrenceArgs &args, void *ws, hipStream_t stream);
+uint64_t gated_recurrence_grad_workspace_bytes(const RecurrenceGradArgs &args);
+hx_status launch_gated_recurrence_grad(const RecurrenceGradArgs &args, void *ws, hipStream_t stream);
+uint64_t cross_entropy_workspace_bytes(const CrossEntropyArgs &args);
+hx_status launch_cross_entropy(const CrossEntropyArgs &args, void *ws, hipStream_t stream);
+uint64_t cross_entropy_grad_workspace_bytes(const CrossEntropyGradArgs &args);
+hx_status launch_cross_entropy_grad(const CrossEntropyGradArgs &args, void *ws, hipStream_t stream);
 
 // Stream-ordered device-to-device copy of `bytes` bytes (a streaming kernel).
 hx_status launch_copy(const void *src, void *dst, uint64_t bytes, hipStream_t stream);

@@ -781,4 +781,182 @@ class RocmLinearAttentionOps {
     }
 };
 
+// ----------------------------------------------------- training operators
+// The formulas and rules stand at hx_layer_norm, hx_gated_recurrence,
+// hx_linear_cross_entropy and their backward passes.  T is float or Bfloat16; an
+// operand left out is nullopt, a vector left out nullptr.
+namespace detail {
+template <typename T> struct Elements {
+    T *ptr = nullptr;
+    uint64_t len = 0;
+    Elements(const RocmBuffer<typename std::remove_const<T>::type> *b) {
+        if (b) {
+            ptr = const_cast<T *>(b->device_ptr());
+            len = b->len();
+        }
+    }
+};
+} // namespace detail
+
+class RocmLayerNormOps {
+  public:
+    template <typename T> struct Forward {
+        StridedView<T> x;
+        const RocmBuffer<T> &weight;
+        const RocmBuffer<T> *bias;
+        float epsilon;
+        StridedView<T> out;
+        OptionalView<T> residual = {}, residual_out = {};
+        RocmBuffer<float> *mean = nullptr, *rstd = nullptr;
+    };
+    template <typename T> struct Backward {
+        StridedView<T> grad_out, x;
+        const RocmBuffer<T> &weight;
+        const RocmBuffer<float> &mean, &rstd;
+        StridedView<T> grad_in;
+        OptionalView<T> residual_grad = {};
+        RocmBuffer<float> *grad_weight = nullptr, *grad_bias = nullptr;
+    };
+    template <typename T> void layer_norm_into(RocmDevice &dev, const Forward<T> &a, hx_stream stream = nullptr) const {
+        call(hx_layer_norm, dev, a, stream);
+    }
+    template <typename T> PreparedPlan prepare_layer_norm(RocmDevice &dev, const Forward<T> &a) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_layer_norm, dev, a, &plan);
+        return PreparedPlan(plan);
+    }
+    template <typename T>
+    void layer_norm_backward_into(RocmDevice &dev, const Backward<T> &a, hx_stream stream = nullptr) const {
+        call(hx_layer_norm_backward, dev, a, stream);
+    }
+    template <typename T> PreparedPlan prepare_layer_norm_backward(RocmDevice &dev, const Backward<T> &a) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_layer_norm_backward, dev, a, &plan);
+        return PreparedPlan(plan);
+    }
+
+  private:
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const Forward<T> &a, Last last) const {
+        const detail::Operand<T> x(a.x), r(a.residual), ro(a.residual_out), o(a.out);
+        const detail::Elements<T> b(a.bias);
+        const detail::Elements<float> m(a.mean), s(a.rstd);
+        check(f(dev.raw(), Scalar<T>::dtype, x.ptr, x.len, x.layout, r.ptr, r.len, r.layout, a.weight.device_ptr(),
+                a.weight.len(), b.ptr, b.len, a.epsilon, ro.ptr, ro.len, ro.layout, o.ptr, o.len, o.layout, m.ptr, m.len,
+                s.ptr, s.len, last));
+    }
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const Backward<T> &a, Last last) const {
+        const detail::Operand<T> g(a.grad_out), x(a.x), r(a.residual_grad), o(a.grad_in);
+        const detail::Elements<float> gw(a.grad_weight), gb(a.grad_bias);
+        check(f(dev.raw(), Scalar<T>::dtype, g.ptr, g.len, g.layout, x.ptr, x.len, x.layout, a.weight.device_ptr(),
+                a.weight.len(), a.mean.device_ptr(), a.mean.len(), a.rstd.device_ptr(), a.rstd.len(), r.ptr, r.len,
+                r.layout, o.ptr, o.len, o.layout, gw.ptr, gw.len, gb.ptr, gb.len, last));
+    }
+};
+
+class RocmRecurrenceOps {
+  public:
+    template <typename T> struct Forward {
+        StridedView<T> gate, x, out;
+        OptionalView<float> state_in = {}, state_out = {};
+        const RocmBuffer<uint32_t> *lengths = nullptr;
+    };
+    template <typename T> struct Backward {
+        StridedView<T> gate, x, h, grad_out, grad_gate, grad_x;
+        OptionalView<float> state_in = {}, grad_state_out = {}, grad_state_in = {};
+        const RocmBuffer<uint32_t> *lengths = nullptr;
+    };
+    template <typename T>
+    void gated_recurrence_into(RocmDevice &dev, const Forward<T> &a, hx_stream stream = nullptr) const {
+        call(hx_gated_recurrence, dev, a, stream);
+    }
+    template <typename T> PreparedPlan prepare_gated_recurrence(RocmDevice &dev, const Forward<T> &a) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_gated_recurrence, dev, a, &plan);
+        return PreparedPlan(plan);
+    }
+    template <typename T>
+    void gated_recurrence_backward_into(RocmDevice &dev, const Backward<T> &a, hx_stream stream = nullptr) const {
+        call(hx_gated_recurrence_backward, dev, a, stream);
+    }
+    template <typename T> PreparedPlan prepare_gated_recurrence_backward(RocmDevice &dev, const Backward<T> &a) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_gated_recurrence_backward, dev, a, &plan);
+        return PreparedPlan(plan);
+    }
+
+  private:
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const Forward<T> &a, Last last) const {
+        const detail::Operand<T> z(a.gate), x(a.x), o(a.out);
+        const detail::Operand<float> si(a.state_in), so(a.state_out);
+        const detail::Elements<uint32_t> n(a.lengths);
+        check(f(dev.raw(), Scalar<T>::dtype, z.ptr, z.len, z.layout, x.ptr, x.len, x.layout, si.ptr, si.len, si.layout,
+                n.ptr, n.len, o.ptr, o.len, o.layout, so.ptr, so.len, so.layout, last));
+    }
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const Backward<T> &a, Last last) const {
+        const detail::Operand<T> z(a.gate), x(a.x), h(a.h), g(a.grad_out), gz(a.grad_gate), gx(a.grad_x);
+        const detail::Operand<float> si(a.state_in), go(a.grad_state_out), gi(a.grad_state_in);
+        const detail::Elements<uint32_t> n(a.lengths);
+        check(f(dev.raw(), Scalar<T>::dtype, z.ptr, z.len, z.layout, x.ptr, x.len, x.layout, h.ptr, h.len, h.layout,
+                si.ptr, si.len, si.layout, n.ptr, n.len, g.ptr, g.len, g.layout, go.ptr, go.len, go.layout, gz.ptr,
+                gz.len, gz.layout, gx.ptr, gx.len, gx.layout, gi.ptr, gi.len, gi.layout, last));
+    }
+};
+
+class RocmLossOps {
+  public:
+    // A target that leaves its row out, whatever the vocabulary.
+    static constexpr uint32_t no_target = 0xFFFFFFFFu;
+    template <typename T> struct Forward {
+        StridedView<T> x, weight;
+        const RocmBuffer<uint32_t> &targets;
+        RocmBuffer<float> &loss;
+        RocmBuffer<float> *lse = nullptr;
+    };
+    template <typename T> struct Backward {
+        StridedView<T> x, weight;
+        const RocmBuffer<uint32_t> &targets;
+        const RocmBuffer<float> &lse, &grad;
+        OptionalView<T> grad_x = {}, grad_weight = {};
+    };
+    template <typename T>
+    void linear_cross_entropy_into(RocmDevice &dev, const Forward<T> &a, hx_stream stream = nullptr) const {
+        call(hx_linear_cross_entropy, dev, a, stream);
+    }
+    template <typename T> PreparedPlan prepare_linear_cross_entropy(RocmDevice &dev, const Forward<T> &a) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_linear_cross_entropy, dev, a, &plan);
+        return PreparedPlan(plan);
+    }
+    template <typename T>
+    void linear_cross_entropy_backward_into(RocmDevice &dev, const Backward<T> &a, hx_stream stream = nullptr) const {
+        call(hx_linear_cross_entropy_backward, dev, a, stream);
+    }
+    template <typename T>
+    PreparedPlan prepare_linear_cross_entropy_backward(RocmDevice &dev, const Backward<T> &a) const {
+        hx_plan *plan = nullptr;
+        call(hx_prepare_linear_cross_entropy_backward, dev, a, &plan);
+        return PreparedPlan(plan);
+    }
+
+  private:
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const Forward<T> &a, Last last) const {
+        const detail::Operand<T> x(a.x), w(a.weight);
+        const detail::Elements<float> lse(a.lse);
+        check(f(dev.raw(), Scalar<T>::dtype, x.ptr, x.len, x.layout, w.ptr, w.len, w.layout, a.targets.device_ptr(),
+                a.targets.len(), a.loss.device_ptr(), a.loss.len(), lse.ptr, lse.len, last));
+    }
+    template <typename F, typename T, typename Last>
+    void call(F f, RocmDevice &dev, const Backward<T> &a, Last last) const {
+        const detail::Operand<T> x(a.x), w(a.weight), gx(a.grad_x), gw(a.grad_weight);
+        check(f(dev.raw(), Scalar<T>::dtype, x.ptr, x.len, x.layout, w.ptr, w.len, w.layout, a.targets.device_ptr(),
+                a.targets.len(), a.lse.device_ptr(), a.lse.len(), a.grad.device_ptr(), a.grad.len(), gx.ptr, gx.len,
+                gx.layout, gw.ptr, gw.len, gw.layout, last));
+    }
+};
+
 } // namespace hephaestus

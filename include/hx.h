@@ -47,10 +47,11 @@
  * hx_segmented_reduce, hx_map_reduce, hx_trace) draw a fresh tag per call
  * and may grow their stream's buffers, so on a capturing stream they fail
  * with HX_ERR_DISPATCH_FAILED before anything is queued, and so do the
- * immediate layer operators that take scratch (hx_matmul_i8,
- * hx_linear_attention); hx_scan_noalloc, the vector forms, hx_copy_async,
- * hx_fill_random and hx_rms_norm_quantize queue plain kernels and may be
- * captured.
+ * immediate layer and training operators that take scratch (hx_matmul_i8,
+ * hx_linear_attention, hx_linear_cross_entropy and the backward passes;
+ * hx_gated_recurrence where tokens are cut into parts); hx_scan_noalloc, the
+ * vector forms, hx_copy_async, hx_fill_random, hx_rms_norm_quantize and
+ * hx_layer_norm queue plain kernels and may be captured.
  */
 #ifndef HX_H
 #define HX_H
@@ -615,6 +616,197 @@ hx_status hx_prepare_linear_attention(
     uint64_t state_out_buf_len, const hx_layout *state_out_layout,
     const uint32_t *lengths, uint64_t lengths_len, void *out,
     uint64_t out_buf_len, const hx_layout *out_layout, hx_plan **plan);
+
+/* ----------------------------------------------------- training operators */
+/* What a scan-type language model is trained with (no counterpart in the
+ * reference): each operator and its backward pass.  Operands as for the layer
+ * operators: F32 or BF16, sums in 32 bits, strided views whose last
+ * dimension is contiguous, outputs apart from each other and from inputs
+ * except where stated, operands that may be NULL left out by a NULL layout
+ * (vectors: NULL and length 0).  Results have one order of summation: every
+ * run gives the same bits. */
+
+/* Layer norm of rows, with the residual's addition.  x is [rows, cols]:
+ *   h    = x + residual                      (residual may be NULL: h = x)
+ *   mean = mean of h,  rstd = (mean of (h - mean)^2 + epsilon)^(-1/2)
+ *   out  = (h - mean) * rstd * weight + bias    (weight[cols], bias[cols] of
+ *                                              dtype; bias may be NULL: 0)
+ * residual_out (may be NULL) receives h rounded to dtype, and may be the very
+ * view of x or of residual; out is taken from h before that rounding.  mean
+ * and rstd are f32[rows], each may be NULL.  A row of equal elements has out =
+ * bias, and rstd = 0 where epsilon is 0.  Rows whose sums or squares leave the
+ * range of f32 are as exact as others; a row with a NaN or an infinity is NaN.
+ * cols = 0 leaves mean and rstd NaN. */
+hx_status hx_layer_norm(hx_device *dev, hx_dtype dtype, const void *x,
+                        uint64_t x_buf_len, const hx_layout *x_layout,
+                        const void *residual, uint64_t residual_buf_len,
+                        const hx_layout *residual_layout, const void *weight,
+                        uint64_t weight_len, const void *bias,
+                        uint64_t bias_len, float epsilon, void *residual_out,
+                        uint64_t residual_out_buf_len,
+                        const hx_layout *residual_out_layout, void *out,
+                        uint64_t out_buf_len, const hx_layout *out_layout,
+                        float *mean, uint64_t mean_len, float *rstd,
+                        uint64_t rstd_len, hx_stream stream);
+hx_status hx_prepare_layer_norm(
+    hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *residual, uint64_t residual_buf_len,
+    const hx_layout *residual_layout, const void *weight, uint64_t weight_len,
+    const void *bias, uint64_t bias_len, float epsilon, void *residual_out,
+    uint64_t residual_out_buf_len, const hx_layout *residual_out_layout,
+    void *out, uint64_t out_buf_len, const hx_layout *out_layout, float *mean,
+    uint64_t mean_len, float *rstd, uint64_t rstd_len, hx_plan **plan);
+
+/* Its backward pass.  x is the h that was normalised (residual_out, or x where
+ * there was no residual), mean and rstd are the forward pass's, grad_out is the
+ * gradient of out:
+ *   u = (x - mean) * rstd,  t = grad_out * weight
+ *   grad_in     = rstd * (t - mean of t - u * mean of t*u) + residual_grad
+ *   grad_weight = sum over rows of grad_out * u,  grad_bias = ... of grad_out
+ * residual_grad (may be NULL) is the gradient that reaches h past the norm.
+ * grad_in is the gradient of x and of residual alike, and may be the very view
+ * of grad_out or of residual_grad.  grad_weight and grad_bias are f32[cols],
+ * overwritten; each may be NULL. */
+hx_status hx_layer_norm_backward(
+    hx_device *dev, hx_dtype dtype, const void *grad_out,
+    uint64_t grad_out_buf_len, const hx_layout *grad_out_layout, const void *x,
+    uint64_t x_buf_len, const hx_layout *x_layout, const void *weight,
+    uint64_t weight_len, const float *mean, uint64_t mean_len,
+    const float *rstd, uint64_t rstd_len, const void *residual_grad,
+    uint64_t residual_grad_buf_len, const hx_layout *residual_grad_layout,
+    void *grad_in, uint64_t grad_in_buf_len, const hx_layout *grad_in_layout,
+    float *grad_weight, uint64_t grad_weight_len, float *grad_bias,
+    uint64_t grad_bias_len, hx_stream stream);
+hx_status hx_prepare_layer_norm_backward(
+    hx_device *dev, hx_dtype dtype, const void *grad_out,
+    uint64_t grad_out_buf_len, const hx_layout *grad_out_layout, const void *x,
+    uint64_t x_buf_len, const hx_layout *x_layout, const void *weight,
+    uint64_t weight_len, const float *mean, uint64_t mean_len,
+    const float *rstd, uint64_t rstd_len, const void *residual_grad,
+    uint64_t residual_grad_buf_len, const hx_layout *residual_grad_layout,
+    void *grad_in, uint64_t grad_in_buf_len, const hx_layout *grad_in_layout,
+    float *grad_weight, uint64_t grad_weight_len, float *grad_bias,
+    uint64_t grad_bias_len, hx_plan **plan);
+
+/* Gated recurrence of each channel along the tokens:
+ *   f_t = 1 / (1 + exp(-gate_t)),  h_t = f_t * h_{t-1} + (1 - f_t) * x_t
+ * gate, x and out (h) are [batch, tokens, channels] of dtype, with at most
+ * 65535 sequences.  state_in and state_out are f32 views [batch, channels] of h
+ * before the first and after the last token, not rounded in between; either
+ * may be NULL (state_in: zeros), and they may be the very same view.  `lengths`
+ * (u32[batch], or NULL for `tokens` everywhere) counts each sequence's tokens,
+ * at most `tokens`: later rows of gate and x are not read into a result, later
+ * rows of out are 0, and a sequence of no tokens keeps its state.  An infinity
+ * or a NaN reaches the channel's later outputs, and no others; which of
+ * the two depends on how tokens are taken together. */
+hx_status hx_gated_recurrence(
+    hx_device *dev, hx_dtype dtype, const void *gate, uint64_t gate_buf_len,
+    const hx_layout *gate_layout, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const float *state_in,
+    uint64_t state_in_buf_len, const hx_layout *state_in_layout,
+    const uint32_t *lengths, uint64_t lengths_len, void *out,
+    uint64_t out_buf_len, const hx_layout *out_layout, float *state_out,
+    uint64_t state_out_buf_len, const hx_layout *state_out_layout,
+    hx_stream stream);
+hx_status hx_prepare_gated_recurrence(
+    hx_device *dev, hx_dtype dtype, const void *gate, uint64_t gate_buf_len,
+    const hx_layout *gate_layout, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const float *state_in,
+    uint64_t state_in_buf_len, const hx_layout *state_in_layout,
+    const uint32_t *lengths, uint64_t lengths_len, void *out,
+    uint64_t out_buf_len, const hx_layout *out_layout, float *state_out,
+    uint64_t state_out_buf_len, const hx_layout *state_out_layout,
+    hx_plan **plan);
+
+/* Its backward pass.  h is the forward pass's out, grad_out its gradient;
+ * grad_state_out (may be NULL: 0) is the gradient of state_out:
+ *   g_t = grad_out_t + f_{t+1} * g_{t+1}, after the last token grad_state_out
+ *   grad_x = (1 - f) * g,  grad_gate = f * (1 - f) * g * (h_{t-1} - x)
+ *   grad_state_in = f_0 * g_0
+ * with state_in in the place of h_{t-1} at the first token.  grad_gate and
+ * grad_x are [batch, tokens, channels] of dtype, 0 in rows past a sequence's
+ * length; grad_state_in (may be NULL) is an f32 view [batch, channels].  The
+ * gradient of a sequence of no tokens passes from grad_state_out to
+ * grad_state_in. */
+hx_status hx_gated_recurrence_backward(
+    hx_device *dev, hx_dtype dtype, const void *gate, uint64_t gate_buf_len,
+    const hx_layout *gate_layout, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *h, uint64_t h_buf_len,
+    const hx_layout *h_layout, const float *state_in,
+    uint64_t state_in_buf_len, const hx_layout *state_in_layout,
+    const uint32_t *lengths, uint64_t lengths_len, const void *grad_out,
+    uint64_t grad_out_buf_len, const hx_layout *grad_out_layout,
+    const float *grad_state_out, uint64_t grad_state_out_buf_len,
+    const hx_layout *grad_state_out_layout, void *grad_gate,
+    uint64_t grad_gate_buf_len, const hx_layout *grad_gate_layout, void *grad_x,
+    uint64_t grad_x_buf_len, const hx_layout *grad_x_layout,
+    float *grad_state_in, uint64_t grad_state_in_buf_len,
+    const hx_layout *grad_state_in_layout, hx_stream stream);
+hx_status hx_prepare_gated_recurrence_backward(
+    hx_device *dev, hx_dtype dtype, const void *gate, uint64_t gate_buf_len,
+    const hx_layout *gate_layout, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *h, uint64_t h_buf_len,
+    const hx_layout *h_layout, const float *state_in,
+    uint64_t state_in_buf_len, const hx_layout *state_in_layout,
+    const uint32_t *lengths, uint64_t lengths_len, const void *grad_out,
+    uint64_t grad_out_buf_len, const hx_layout *grad_out_layout,
+    const float *grad_state_out, uint64_t grad_state_out_buf_len,
+    const hx_layout *grad_state_out_layout, void *grad_gate,
+    uint64_t grad_gate_buf_len, const hx_layout *grad_gate_layout, void *grad_x,
+    uint64_t grad_x_buf_len, const hx_layout *grad_x_layout,
+    float *grad_state_in, uint64_t grad_state_in_buf_len,
+    const hx_layout *grad_state_in_layout, hx_plan **plan);
+
+/* Softmax cross entropy over a vocabulary of the logits that a head's product
+ * gives, which are not kept:
+ *   logits[r, v] = sum over the width of x[r, :] * weight[v, :]
+ *   lse[r]  = log of the sum over v of exp(logits[r, v])
+ *   loss[r] = lse[r] - logits[r, targets[r]]
+ * x is [rows, width], weight [vocab, width], both of dtype; targets is
+ * u32[rows].  A row whose target is not below vocab is left out: its loss is 0.
+ * loss and lse are f32[rows]; lse may be NULL.  A logit that is a NaN or plus
+ * infinity makes its row's loss and lse a NaN.  rows, vocab and width are below
+ * 2^28 each. */
+hx_status hx_linear_cross_entropy(
+    hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *weight, uint64_t weight_buf_len,
+    const hx_layout *weight_layout, const uint32_t *targets,
+    uint64_t targets_len, float *loss, uint64_t loss_len, float *lse,
+    uint64_t lse_len, hx_stream stream);
+hx_status hx_prepare_linear_cross_entropy(
+    hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *weight, uint64_t weight_buf_len,
+    const hx_layout *weight_layout, const uint32_t *targets,
+    uint64_t targets_len, float *loss, uint64_t loss_len, float *lse,
+    uint64_t lse_len, hx_plan **plan);
+
+/* Its backward pass, from the forward pass's lse and `grad`, the gradient of
+ * each row's loss (f32[rows]):
+ *   G[r, v] = grad[r] * (exp(logits[r, v] - lse[r]) - [v = targets[r]])
+ *   grad_x = G * weight,  grad_weight = G^T * x
+ * both of dtype, overwritten; either may be NULL.  A row that is left out has
+ * grad_x = 0 and adds nothing, whatever x, lse and grad hold there.  The logits
+ * are taken again, a piece of the vocabulary after another; G of a piece is kept
+ * in dtype (BF16: 8 bits a term of the sums), relative to the largest finite
+ * |grad|. */
+hx_status hx_linear_cross_entropy_backward(
+    hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *weight, uint64_t weight_buf_len,
+    const hx_layout *weight_layout, const uint32_t *targets,
+    uint64_t targets_len, const float *lse, uint64_t lse_len,
+    const float *grad, uint64_t grad_len, void *grad_x,
+    uint64_t grad_x_buf_len, const hx_layout *grad_x_layout,
+    void *grad_weight, uint64_t grad_weight_buf_len,
+    const hx_layout *grad_weight_layout, hx_stream stream);
+hx_status hx_prepare_linear_cross_entropy_backward(
+    hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
+    const hx_layout *x_layout, const void *weight, uint64_t weight_buf_len,
+    const hx_layout *weight_layout, const uint32_t *targets,
+    uint64_t targets_len, const float *lse, uint64_t lse_len,
+    const float *grad, uint64_t grad_len, void *grad_x,
+    uint64_t grad_x_buf_len, const hx_layout *grad_x_layout,
+    void *grad_weight, uint64_t grad_weight_buf_len,
+    const hx_layout *grad_weight_layout, hx_plan **plan);
 
 /* ---------------------------------------------------------------- plans */
 
