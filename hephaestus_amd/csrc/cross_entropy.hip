@@ -63,17 +63,16 @@ __device__ __forceinline__ float exp_of(float x) {
 }
 
 // ---------------------------------------------------------------- product
-// out[m, n] = Σ_k a[m, k]·b[n, k], handed to an epilogue in tiles of BM x BN.  The
-// tile's WM x WN waves each take a part.  A step's 128 bytes of k of each row
-// lie in LDS as eight chunks of 16, chunk c of row r at place c ^ (r % 8), so that the
-// 16 rows that a matrix instruction reads at one c fall on all banks.  Loads go from
-// memory to LDS without registers, S - 1 steps ahead; they need rows that begin
-// on dwords.
+// out[m, n] = Σ_k a(m, k)·b(n, k), handed to an epilogue in tiles of BM x BN.  An
+// operand lies in memory by rows of k, a row for each m or n, or across: a row for each
+// k.  A step is 128 bytes of k.  The tile's WM x WN waves each take a part of it.
+struct Operand {
+    const int8_t *rows;
+    int64_t stride; // bytes, of its rows in memory
+};
 struct Product {
-    const int8_t *a, *b;
-    uint64_t m, n;
-    uint32_t k;                // bytes
-    int64_t a_stride, b_stride; // bytes
+    Operand a, b;
+    uint64_t m, n, k; // elements
 };
 
 // The barrier between steps is written out: all of the wave's LDS reads and
@@ -82,27 +81,123 @@ template <int N> __device__ __forceinline__ void step_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
+// One operand's part of a step in LDS, WIDTH rows of m or n; loads go from memory
+// to LDS without registers, each wave's 64 chunks of 16 bytes side by side, so that the
+// exchange of places is made on the memory's side.  Rows begin on dwords.
+//
+// By rows: 128 bytes of each row, chunk c of row r at place c ^ (r % 8), so that
+// the rows that a matrix instruction reads at one c fall on all banks.
+// Across: WIDTH elements of each k, in segments of what 16 lanes take at once (32
+// bytes of bf16, 64 of f32); segment s of row k at place s ^ turn(k), for the same reason.
+// bf16 is turned by the read: 16 lanes that address 4 rows of 16 elements receive
+// a column's 4 elements each.
+template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
+    static constexpr int kBytes = WIDTH * kDepth, kLoads = WIDTH * 8 / THREADS;
+    static constexpr int kN = 16 / sizeof(T);              // elements of a chunk
+    static constexpr int kRow = ACROSS ? WIDTH * (int)sizeof(T) : kDepth;
+    static constexpr int kChunks = kRow / 16;              // of a row
+    static constexpr int kSegment = sizeof(T) == 2 ? 2 : 4; // chunks
+    static constexpr int kTurns = kChunks / kSegment < 8 ? kChunks / kSegment : 8;
+    static_assert(kLoads * THREADS == WIDTH * 8);
+
+    static __device__ __forceinline__ uint32_t turn(uint32_t k) {
+        if constexpr (sizeof(T) == 2) return (k % 4 + k / 8 % 2 * 4) % kTurns;
+        else return k / 4 % 4 % kTurns;
+    }
+
+    // What this thread loads: its chunks' addresses at k = 0.
+    const int8_t *src[kLoads];
+    uint32_t at_k; // by rows: bytes into the row, the same for all of them
+    int64_t stride;
+    __device__ __forceinline__ void open(const Operand &o, uint64_t first, uint64_t end, int wave, int lane) {
+        stride = o.stride;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const uint32_t q = (wave * kLoads + j) * kWave + lane, row = q / kChunks, place = q % kChunks;
+            if constexpr (ACROSS) {
+                const uint32_t chunk = (place / kSegment ^ turn(row)) * kSegment + place % kSegment;
+                // Columns past the end repeat the last chunk and are dropped at the end.
+                const uint64_t c = min(first + (uint64_t)chunk * kN, (end + kN - 1) / kN * kN - kN);
+                src[j] = o.rows + (int64_t)row * stride + (int64_t)(c * sizeof(T));
+            } else {
+                src[j] = o.rows + (int64_t)min(first + row, end - 1) * stride;
+                if (j == 0) at_k = (place ^ (row % 8)) * 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void fetch(int8_t *stage, uint32_t step, int wave) const {
+        int8_t *to = stage + wave * (kLoads * 1024);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int8_t *from = ACROSS ? src[j] + (int64_t)step * (kDepth / (int)sizeof(T)) * stride
+                                        : src[j] + (uint64_t)step * kDepth + at_k;
+            __builtin_amdgcn_global_load_lds((const void *)from, (lds_void *)(to + j * 1024), 16, 0, 0);
+        }
+    }
+    // The last, partial step: zeros past the end of k.
+    __device__ __forceinline__ void fetch_rest(int8_t *stage, uint32_t step, uint64_t k, int wave, int lane) const {
+        int8_t *to = stage + wave * (kLoads * 1024) + lane * 16;
+        for (int j = 0; j < kLoads; ++j) {
+            u32x4 v = {0, 0, 0, 0};
+            if constexpr (ACROSS) {
+                const uint32_t row = ((wave * kLoads + j) * kWave + lane) / kChunks;
+                const uint64_t at = (uint64_t)step * (kDepth / sizeof(T)) + row;
+                if (at < k) v = *(const u32x4_any *)(src[j] + (int64_t)step * (kDepth / (int)sizeof(T)) * stride);
+            } else {
+                v = load_bytes(src[j], step * kDepth + at_k, (uint32_t)(k * sizeof(T)));
+            }
+            *(u32x4 *)(to + j * 1024) = v;
+        }
+    }
+
+    // Where this lane reads: 16 bytes of k, half `s` of the step, of row `part` + 16·i + lane % 16.
+    uint32_t at;
+    __device__ __forceinline__ void place(uint32_t part, int lane) {
+        if constexpr (!ACROSS) at = (part + lane % 16) * kDepth + ((lane / 16 ^ lane % 8) * 16);
+        else if constexpr (sizeof(T) == 2)
+            at = (lane / 16 * 8 + lane % 16 / 4) * kRow + ((part / 16 ^ turn(lane / 16 * 8 + lane % 16 / 4)) * 32) + lane % 4 * 8;
+        else at = (lane / 16 * 4) * kRow + ((part / 16 ^ turn(lane / 16 * 4)) * 64) + lane % 16 * 4;
+    }
+    __device__ __forceinline__ u32x4 read(const int8_t *stage, int i, int s) const {
+        if constexpr (!ACROSS) return *(const u32x4 *)(stage + (at ^ (64 * s)) + i * (16 * kDepth));
+        else if constexpr (sizeof(T) == 2) {
+            typedef short Four __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) Four lds_four;
+            const int8_t *p = stage + (at ^ (32 * i)) + s * (32 * kRow);
+            const Four lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four *)p);
+            const Four hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four *)(p + 4 * kRow));
+            typedef short Eight __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(u32x4, (Eight)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            u32x4 v;
+            const int8_t *p = stage + (at ^ (64 * i)) + s * (16 * kRow);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *(const uint32_t *)(p + e * kRow);
+            return v;
+        }
+    }
+};
+
 template <int BM_, int BN_, int WM_, int WN_, int S_> struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
-    static constexpr int kWaves = WM * WN, kThreads = kWaves * kWave;
-    static constexpr int kRows = BM + BN, kStage = kRows * kDepth, kLds = kStage * S;
+    static constexpr int kThreads = WM * WN * kWave;
+    static constexpr int kStage = (BM + BN) * kDepth, kLds = kStage * S;
     static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    static constexpr int kLoads = kRows * 8 / kThreads; // chunks a thread and step
-    static_assert(kLds <= 160 * 1024 && kLoads * kThreads == kRows * 8 && (S - 2) * kLoads < 64);
+    static_assert(kLds <= 160 * 1024);
 };
 
 // What an epilogue knows of its place: lane l has, of fragment (i, j), the sums of
 // row m + 16·i and columns n + 16·j + 0..3.
 struct Place {
-    uint64_t m, n;      // this lane's first row and column
+    uint64_t m, n;       // this lane's first row and column
     uint64_t m0, tile_n; // the tile's first row; its place among the columns' tiles
-    int wave_m, wave_n;
+    int wave_n;
 };
 
-template <typename T, typename C, typename E>
-__global__ __launch_bounds__(C::kThreads, 2) void product_kernel(Product p, E epilogue, uint32_t tiles_m,
-                                                                uint32_t tiles_n) {
-    constexpr int BM = C::BM, BN = C::BN, FM = C::FM, FN = C::FN, kLoads = C::kLoads, S = C::S;
+template <typename T, typename C, bool ACROSS_A, bool ACROSS_B, typename E>
+__global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilogue, uint32_t tiles_m,
+                                                             uint32_t tiles_n) {
+    constexpr int BM = C::BM, BN = C::BN, FM = C::FM, FN = C::FN, S = C::S;
     extern __shared__ __align__(16) int8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 
@@ -115,72 +210,80 @@ __global__ __launch_bounds__(C::kThreads, 2) void product_kernel(Product p, E ep
     const uint32_t height = min(8u, tiles_m - 8 * strip);
     const uint64_t m0 = (uint64_t)(8 * strip + in_strip % height) * BM, n0 = (uint64_t)(in_strip / height) * BN;
 
-    const uint32_t k_end = p.k, steps = (k_end + kDepth - 1) / kDepth, whole = k_end / kDepth;
-    // A thread's chunk of each row that it loads: rows past the operands
-    // repeat the last one and are dropped at the end.
-    const uint32_t row0 = wave * (kLoads * 8) + lane / 8, chunk = (lane % 8 ^ (row0 % 8)) * 16;
-    const int8_t *src[kLoads];
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-        const uint32_t r = row0 + j * 8;
-        src[j] = r < BM ? p.a + (int64_t)min(m0 + r, p.m - 1) * p.a_stride
-                        : p.b + (int64_t)min(n0 + (r - BM), p.n - 1) * p.b_stride;
-    }
-    const uint32_t to = wave * (kLoads * 1024); // this wave's first row in a stage
-
+    constexpr uint32_t kStep = kDepth / sizeof(T);
+    const uint32_t steps = (uint32_t)((p.k + kStep - 1) / kStep), whole = (uint32_t)(p.k / kStep);
+    Staged<T, BM, C::kThreads, ACROSS_A> a;
+    Staged<T, BN, C::kThreads, ACROSS_B> b;
+    constexpr int kLoads = a.kLoads + b.kLoads;
+    static_assert((S - 1) * kLoads < 64);
+    a.open(p.a, m0, p.m, wave, lane);
+    b.open(p.b, n0, p.n, wave, lane);
     const int wm = wave / C::WN * (BM / C::WM), wn = wave % C::WN * (BN / C::WN);
-    const uint32_t swizzled = (lane / 16 ^ (lane % 8)) * 16; // of k bytes 0..63; 64..127: ^ 64
-    const uint32_t at_a = (wm + lane % 16) * kDepth + swizzled, at_b = (BM + wn + lane % 16) * kDepth + swizzled;
+    a.place(wm, lane);
+    b.place(wn, lane);
+
     f32x4 acc[FM][FN] = {};
-    const auto compute = [&](const int8_t *stage) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 fa[FM], fb[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = *(const u32x4 *)(stage + (at_b ^ (64 * s)) + j * (16 * kDepth));
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = *(const u32x4 *)(stage + (at_a ^ (64 * s)) + i * (16 * kDepth));
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
-        }
+    struct Half {
+        u32x4 a[FM], b[FN];
     };
-    // Whole steps: no branch in the loads.
+    const auto read = [&](Half &h, uint32_t t, int s) {
+        const int8_t *stage = lds + t % S * C::kStage;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) h.b[j] = b.read(stage + a.kBytes, j, s);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) h.a[i] = a.read(stage, i, s);
+    };
+    const auto compute = [&](const Half &h) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(h.b[j], h.a[i], acc[i][j]);
+    };
     const auto fetch = [&](uint32_t t) {
-        int8_t *stage = lds + t % S * C::kStage + to;
-        const uint32_t k = t * kDepth + chunk;
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j)
-            __builtin_amdgcn_global_load_lds((const void *)(src[j] + k), (lds_void *)(stage + j * 1024), 16, 0, 0);
+        int8_t *stage = lds + t % S * C::kStage;
+        a.fetch(stage, t, wave);
+        b.fetch(stage + a.kBytes, t, wave);
     };
-    // The step of the last, partial 128 bytes: zeros past the end of k.
     const auto fetch_any = [&](uint32_t t) {
         if (t < whole) {
             fetch(t);
         } else if (t < steps) {
-            int8_t *stage = lds + t % S * C::kStage + to;
-            for (int j = 0; j < kLoads; ++j)
-                *(u32x4 *)(stage + j * 1024 + lane * 16) = load_bytes(src[j], t * kDepth + chunk, k_end);
+            int8_t *stage = lds + t % S * C::kStage;
+            a.fetch_rest(stage, t, p.k, wave, lane);
+            b.fetch_rest(stage + a.kBytes, t, p.k, wave, lane);
         }
     };
-    for (int t = 0; t < S - 1; ++t) fetch_any(t);
-    // Step t has landed once no more loads are under way than those of the
-    // S - 2 steps behind it.
+    // A step's second half is read while the first is summed, the next step's
+    // first half while the second is.  Between the two the waves meet: all have read the
+    // step, so that its place is free, and the next step has landed once no more
+    // loads are under way than those of the S - 2 steps behind it.
+    Half first, second;
+    for (int t = 0; t < S; ++t) fetch_any(t);
+    if (steps > 0) {
+        if (S <= whole) step_barrier<(S - 1) * kLoads>();
+        else step_barrier<0>();
+        read(first, 0, 0);
+    }
     uint32_t t = 0;
-    for (; t + (S - 1) < whole; ++t) {
+    for (; t + S < whole; ++t) {
+        read(second, t, 1);
+        compute(first);
         step_barrier<(S - 2) * kLoads>();
-        fetch(t + S - 1);
-        compute(lds + t % S * C::kStage);
+        fetch(t + S);
+        read(first, t + 1, 0);
+        compute(second);
     }
     for (; t < steps; ++t) { // the last ones, not all of them direct loads
+        read(second, t, 1);
+        compute(first);
         step_barrier<0>();
-        if (t + S - 1 < steps) fetch_any(t + S - 1);
-        compute(lds + t % S * C::kStage);
+        if (t + S < steps) fetch_any(t + S);
+        if (t + 1 < steps) read(first, t + 1, 0);
+        compute(second);
     }
     __syncthreads(); // LDS is the epilogue's
-    epilogue.template finish<C>(acc, Place{m0 + wm + lane % 16, n0 + wn + lane / 16 * 4, m0, n0 / BN, wm, wave % C::WN},
-                                p, (float *)lds);
+    epilogue.template finish<C>(acc, Place{m0 + wm + lane % 16, n0 + wn + lane / 16 * 4, m0, n0 / BN, wave % C::WN}, p,
+                                (float *)lds);
 }
 
 // The largest logit of each row of the tile, the sum of e^(logit - largest), and the
@@ -233,10 +336,29 @@ struct TileStats {
     }
 };
 
-// G of a piece of the vocabulary that begins at `first`, by rows and by columns.
+// Four columns of a row at the alignment of the elements, those before `end`.
+typedef bf16 bf16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T> __device__ __forceinline__ void store_four(T *p, uint64_t n, uint64_t end, f32x4 v) {
+    if (n + 4 <= end) {
+        if constexpr (sizeof(T) == 4) {
+            *(f32x4_a4 *)p = v;
+        } else {
+            bf16x4_a2 r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = (bf16)v[e];
+            *(bf16x4_a2 *)p = r;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < end) p[e] = (T)v[e];
+    }
+}
+
+// G of a piece of the vocabulary that begins at `first`.
 template <typename T> struct TileGradient {
-    T *g, *gt;
-    uint64_t pitch, pitch_t; // elements
+    T *g;
+    uint64_t pitch; // elements
     uint64_t first, vocab;
     const uint32_t *targets;
     const float *lse, *grad, *most;
@@ -251,23 +373,21 @@ template <typename T> struct TileGradient {
             const float from = lse[row], weight = counts ? grad[row] / *most : 0.0f;
 #pragma unroll
             for (int j = 0; j < C::FN; ++j) {
-                float v[4];
+                const uint64_t n = at.n + 16 * j;
+                f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint64_t n = at.n + 16 * j + e;
-                    const float s = exp_of(acc[i][j][e] - from) - (first + n == target ? 1.0f : 0.0f);
+                    const float s = exp_of(acc[i][j][e] - from) - (first + n + e == target ? 1.0f : 0.0f);
                     v[e] = counts ? s * weight : 0.0f;
-                    if (n < p.n) {
-                        g[row * pitch + n] = (T)v[e];
-                        gt[n * pitch_t + row] = (T)v[e];
-                    }
                 }
+                store_four(g + row * pitch + n, n, p.n, v);
             }
         }
     }
 };
 
-// scale·(sum + what earlier pieces summed up): to `out`, or on to the next piece.
+// scale·(sum + what earlier pieces summed up): to `out`, or on to the next piece.  Rows
+// without a target get zeros where `targets` is given.
 template <typename T> struct TileOut {
     const float *scale;
     const float *before; // may be null
@@ -275,6 +395,8 @@ template <typename T> struct TileOut {
     T *out;
     uint64_t sum_pitch;
     int64_t out_stride;
+    const uint32_t *targets; // may be null
+    uint64_t vocab;
     template <typename C>
     __device__ __forceinline__ void finish(f32x4 (&acc)[C::FM][C::FN], const Place &at, const Product &p, float *) {
         const float by = *scale;
@@ -282,25 +404,28 @@ template <typename T> struct TileOut {
         for (int i = 0; i < C::FM; ++i) {
             const uint64_t row = at.m + 16 * i;
             if (row >= p.m) continue;
+            const bool is_left_out = targets && targets[row] >= vocab;
 #pragma unroll
             for (int j = 0; j < C::FN; ++j) {
                 const uint64_t n = at.n + 16 * j;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (n + e >= p.n) continue;
-                    float v = acc[i][j][e];
-                    if (before) v += before[row * sum_pitch + n + e];
-                    if (after) after[row * sum_pitch + n + e] = v;
-                    else out[(int64_t)row * out_stride + (int64_t)(n + e)] = (T)(v * by);
+                if (n >= p.n) continue;
+                f32x4 v = acc[i][j];
+                if (before) v += *(const f32x4 *)(before + row * sum_pitch + n); // the pitch is whole vectors
+                if (after) {
+                    *(f32x4 *)(after + row * sum_pitch + n) = v;
+                } else {
+                    v *= by;
+                    if (is_left_out) v = f32x4{0, 0, 0, 0};
+                    store_four(out + (int64_t)row * out_stride + (int64_t)n, n, p.n, v);
                 }
             }
         }
     }
 };
 
-template <typename T, typename C, typename E>
+template <typename T, typename C, bool ACROSS_A, bool ACROSS_B, typename E>
 hx_status launch_tiles(const Product &p, const E &epilogue, hipStream_t stream) {
-    const auto kernel = product_kernel<T, C, E>;
+    const auto kernel = product_kernel<T, C, ACROSS_A, ACROSS_B, E>;
     static std::atomic<uint64_t> allowed{0};
     HX_TRY(allow_lds((const void *)kernel, C::kLds, allowed));
     const uint64_t tm = ceil_div(p.m, C::BM), tn = ceil_div(p.n, C::BN);
@@ -310,48 +435,34 @@ hx_status launch_tiles(const Product &p, const E &epilogue, hipStream_t stream) 
                        (uint32_t)tm, (uint32_t)tn);
     return check_launch("product_kernel");
 }
-template <typename T, typename E> hx_status launch_product(const Product &p, const E &epilogue, hipStream_t stream) {
+template <typename T, bool ACROSS_A, bool ACROSS_B, typename E>
+hx_status launch_product(const Product &p, const E &epilogue, hipStream_t stream) {
     if (p.m == 0 || p.n == 0) return HX_OK;
     switch (product_tile(p.m, p.n)) {
-    case ProductTile::k256x256: return launch_tiles<T, Tile<256, 256, 2, 4, 2>>(p, epilogue, stream);
-    case ProductTile::k128x128: return launch_tiles<T, Tile<128, 128, 2, 2, 2>>(p, epilogue, stream);
-    case ProductTile::k64x64: return launch_tiles<T, Tile<64, 64, 4, 2, 4>>(p, epilogue, stream);
-    case ProductTile::k32x64: return launch_tiles<T, Tile<32, 64, 1, 4, 6>>(p, epilogue, stream);
+    case ProductTile::k256x256: return launch_tiles<T, Tile<256, 256, 2, 4, 2>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
+    case ProductTile::k128x128: return launch_tiles<T, Tile<128, 128, 2, 2, 2>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
+    case ProductTile::k64x64: return launch_tiles<T, Tile<64, 64, 4, 2, 4>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
+    case ProductTile::k32x64: return launch_tiles<T, Tile<32, 64, 1, 4, 6>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
     }
     return HX_OK;
 }
 
 // ------------------------------------------------------------------ rows
 
-// Rows at any byte, copied to rows of whole steps with zeros after their ends.
+// Rows at any byte, copied to rows of whole steps with zeros after their ends, and
+// zeros in the place of rows that have no target where `targets` is given: whatever such a
+// row holds, it adds nothing.
 __global__ __launch_bounds__(256) void copy_rows_kernel(const int8_t *from, int64_t stride, uint64_t rows, uint32_t bytes,
-                                                       int8_t *to, uint32_t pitch) {
+                                                       int8_t *to, uint32_t pitch, const uint32_t *targets,
+                                                       uint64_t vocab) {
     const uint32_t chunks = pitch / 16;
     for (uint64_t first = (uint64_t)blockIdx.x * 256; first < rows * chunks; first += (uint64_t)gridDim.x * 256) {
         const uint32_t i = (uint32_t)(first % chunks) + threadIdx.x, at = i % chunks * 16;
         const uint64_t r = first / chunks + i / chunks;
         if (r >= rows) return;
-        *(u32x4 *)(to + r * pitch + at) = load_bytes(from + (int64_t)r * stride, at, bytes);
-    }
-}
-
-// to[c][r] = from[r][c], with zeros in the rows that have no target where `targets`
-// is given: whatever such a row holds, it adds nothing.
-template <typename T>
-__global__ __launch_bounds__(256) void transpose_kernel(const T *from, int64_t stride, uint64_t rows, uint64_t cols,
-                                                        T *to, uint64_t pitch, const uint32_t *targets, uint64_t vocab) {
-    __shared__ T tile[64][65];
-    const uint64_t r0 = (uint64_t)blockIdx.x * 64, c0 = (uint64_t)blockIdx.y * 64;
-    for (int i = threadIdx.x / 64; i < 64; i += 4) {
-        const uint64_t r = r0 + i, c = c0 + threadIdx.x % 64;
-        T v = (T)0.0f;
-        if (r < rows && c < cols && (!targets || targets[r] < vocab)) v = from[(int64_t)r * stride + (int64_t)c];
-        tile[i][threadIdx.x % 64] = v;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x / 64; i < 64; i += 4) {
-        const uint64_t c = c0 + i, r = r0 + threadIdx.x % 64;
-        if (c < cols && r < rows) to[c * pitch + r] = tile[threadIdx.x % 64][i];
+        u32x4 v = {0, 0, 0, 0};
+        if (!targets || targets[r] < vocab) v = load_bytes(from + (int64_t)r * stride, at, bytes);
+        *(u32x4 *)(to + r * pitch + at) = v;
     }
 }
 
@@ -392,21 +503,14 @@ __global__ __launch_bounds__(1024) void most_kernel(const float *grad, const uin
 }
 
 template <typename T>
-hx_status copy_rows(const void *from, int64_t stride, uint64_t rows, uint64_t width, void *to, hipStream_t stream) {
+hx_status copy_rows(const void *from, int64_t stride, uint64_t rows, uint64_t width, void *to, const uint32_t *targets,
+                    uint64_t vocab, hipStream_t stream) {
     const uint32_t bytes = (uint32_t)(width * sizeof(T)), pitch = (uint32_t)round_up(bytes, kDepth);
     if (rows == 0 || pitch == 0) return HX_OK;
     const uint64_t blocks = std::min<uint64_t>(ceil_div(rows * (pitch / 16), 256), 1 << 22);
     hipLaunchKernelGGL(copy_rows_kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, (const int8_t *)from,
-                       stride * (int64_t)sizeof(T), rows, bytes, (int8_t *)to, pitch);
+                       stride * (int64_t)sizeof(T), rows, bytes, (int8_t *)to, pitch, targets, vocab);
     return check_launch("copy_rows_kernel");
-}
-template <typename T>
-hx_status transpose(const void *from, int64_t stride, uint64_t rows, uint64_t cols, void *to, uint64_t pitch,
-                    const uint32_t *targets, uint64_t vocab, hipStream_t stream) {
-    if (rows == 0 || cols == 0) return HX_OK;
-    hipLaunchKernelGGL(transpose_kernel<T>, dim3((uint32_t)ceil_div(rows, 64), (uint32_t)ceil_div(cols, 64)), dim3(256),
-                       0, stream, (const T *)from, stride, rows, cols, (T *)to, pitch, targets, vocab);
-    return check_launch("transpose_kernel");
 }
 
 template <typename T> hx_status launch(const CrossEntropyArgs &a, void *ws, hipStream_t stream) {
@@ -414,16 +518,16 @@ template <typename T> hx_status launch(const CrossEntropyArgs &a, void *ws, hipS
     char *base = (char *)ws;
     float2 *stats = (float2 *)(base + plan.stats);
     float *picked = (float *)(base + plan.picked);
-    Product p{(const int8_t *)a.x, (const int8_t *)a.weight, a.rows, a.vocab, (uint32_t)(a.width * sizeof(T)),
-              a.x_stride * (int64_t)sizeof(T), a.weight_stride * (int64_t)sizeof(T)};
+    const int64_t size = sizeof(T), row = (int64_t)round_up(a.width * size, kDepth);
+    Product p{{(const int8_t *)a.x, a.x_stride * size}, {(const int8_t *)a.weight, a.weight_stride * size}, a.rows,
+              a.vocab, a.width};
     if (plan.copies) {
-        HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, stream));
-        HX_TRY(copy_rows<T>(a.weight, a.weight_stride, a.vocab, a.width, base + plan.weight, stream));
-        p.a = (const int8_t *)base + plan.x;
-        p.b = (const int8_t *)base + plan.weight;
-        p.a_stride = p.b_stride = (int64_t)round_up(p.k, kDepth);
+        HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, nullptr, 0, stream));
+        HX_TRY(copy_rows<T>(a.weight, a.weight_stride, a.vocab, a.width, base + plan.weight, nullptr, 0, stream));
+        p.a = {(const int8_t *)base + plan.x, row};
+        p.b = {(const int8_t *)base + plan.weight, row};
     }
-    HX_TRY(launch_product<T>(p, TileStats{stats, picked, a.targets}, stream));
+    HX_TRY((launch_product<T, false, false>)(p, TileStats{stats, picked, a.targets}, stream));
     hipLaunchKernelGGL(join_stats_kernel, dim3((uint32_t)ceil_div(a.rows, 16)), dim3(256), 0, stream, stats, picked,
                        a.targets, a.vocab ? plan.tiles_n : 0, a.rows, a.vocab, a.loss, a.lse);
     return check_launch("join_stats_kernel");
@@ -435,50 +539,34 @@ template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, 
     float *most = (float *)base;
     hipLaunchKernelGGL(most_kernel, dim3(1), dim3(1024), 0, stream, a.grad, a.targets, a.rows, a.vocab, most);
     HX_TRY(check_launch("most_kernel"));
-    const int64_t size = sizeof(T);
-    const uint64_t row_bytes = round_up(a.width * size, kDepth);
-    Product logits{(const int8_t *)a.x, nullptr, a.rows, 0, (uint32_t)(a.width * size), a.x_stride * size,
-                   a.weight_stride * size};
-    if (plan.copies) {
-        HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, stream));
-        logits.a = (const int8_t *)base + plan.x;
-        logits.a_stride = logits.b_stride = (int64_t)row_bytes;
-    }
-    if (a.grad_weight)
-        HX_TRY(transpose<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x_columns, plan.rows_pitch, a.targets, a.vocab,
-                            stream));
+    const int64_t size = sizeof(T), row = (int64_t)round_up(a.width * size, kDepth);
+    const Operand x{(const int8_t *)base + plan.x, row};
+    HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, a.targets, a.vocab, stream));
     float *sums = (float *)(base + plan.sums);
-    T *g = (T *)(base + plan.g), *gt = (T *)(base + plan.g_columns);
+    T *g = (T *)(base + plan.g);
+    const Operand go{(const int8_t *)g, (int64_t)plan.piece_pitch * size};
     for (uint64_t first = 0; first < a.vocab || first == 0; first += plan.piece) {
         const uint64_t n = std::min<uint64_t>(plan.piece, a.vocab - first);
-        const T *w = (const T *)a.weight + (int64_t)first * a.weight_stride;
+        const T *from = (const T *)a.weight + (int64_t)first * a.weight_stride;
+        Operand w{(const int8_t *)from, a.weight_stride * size};
         if (plan.copies) {
-            HX_TRY(copy_rows<T>(w, a.weight_stride, n, a.width, base + plan.weight, stream));
-            logits.b = (const int8_t *)base + plan.weight;
-        } else {
-            logits.b = (const int8_t *)w;
+            HX_TRY(copy_rows<T>(from, a.weight_stride, n, a.width, base + plan.weight, nullptr, 0, stream));
+            w = {(const int8_t *)base + plan.weight, row};
         }
-        logits.n = n;
-        HX_TRY(launch_product<T>(logits, TileGradient<T>{g, gt, plan.piece_pitch, plan.rows_pitch, first, a.vocab,
-                                                         a.targets, a.lse, a.grad, most},
-                                 stream));
+        HX_TRY((launch_product<T, false, false>)(Product{x, w, a.rows, n, a.width},
+                                                 TileGradient<T>{g, plan.piece_pitch, first, a.vocab, a.targets, a.lse,
+                                                                 a.grad, most},
+                                                 stream));
         if (a.grad_x) {
-            HX_TRY(transpose<T>(w, a.weight_stride, n, a.width, base + plan.weight_columns, plan.piece_pitch, nullptr, 0,
-                                stream));
             const bool is_last = first + n >= a.vocab;
-            const Product p{(const int8_t *)g, (const int8_t *)base + plan.weight_columns, a.rows, a.width,
-                            (uint32_t)(n * size), (int64_t)plan.piece_pitch * size, (int64_t)plan.piece_pitch * size};
-            HX_TRY(launch_product<T>(p, TileOut<T>{most, first ? sums : nullptr, is_last ? nullptr : sums, (T *)a.grad_x,
-                                                   a.width, a.grad_x_stride},
-                                     stream));
+            const TileOut<T> out{most, first ? sums : nullptr, is_last ? nullptr : sums, (T *)a.grad_x, plan.sums_pitch,
+                                 a.grad_x_stride, a.targets, a.vocab};
+            HX_TRY((launch_product<T, false, true>)(Product{go, w, a.rows, a.width, n}, out, stream));
         }
         if (a.grad_weight) {
-            const Product p{(const int8_t *)gt, (const int8_t *)base + plan.x_columns, n, a.width,
-                            (uint32_t)(a.rows * size), (int64_t)plan.rows_pitch * size, (int64_t)plan.rows_pitch * size};
-            HX_TRY(launch_product<T>(p, TileOut<T>{most, nullptr, nullptr,
-                                                   (T *)a.grad_weight + (int64_t)first * a.grad_weight_stride, 0,
-                                                   a.grad_weight_stride},
-                                     stream));
+            const TileOut<T> out{most, nullptr, nullptr, (T *)a.grad_weight + (int64_t)first * a.grad_weight_stride, 0,
+                                 a.grad_weight_stride, nullptr, 0};
+            HX_TRY((launch_product<T, true, true>)(Product{go, x, n, a.width, a.rows}, out, stream));
         }
     }
     return HX_OK;

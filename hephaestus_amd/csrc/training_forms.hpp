@@ -168,10 +168,15 @@ inline ProductTile product_tile(uint64_t m, uint64_t n) {
     return ProductTile::k64x64;
 }
 
-// Rows off dwords are copied first.
-template <typename Args> bool cross_entropy_copies(const Args &a) {
+// Rows off dwords are copied first, and so are a weight's that end in part of 16 bytes
+// where the backward pass reads them across.
+inline bool cross_entropy_copies(const CrossEntropyArgs &a) {
     const uint64_t size = element_size(a.dtype);
     return (((uintptr_t)a.x | (uintptr_t)a.weight | (uint64_t)(a.x_stride | a.weight_stride) * size) & 3) != 0;
+}
+inline bool cross_entropy_copies(const CrossEntropyGradArgs &a) {
+    const uint64_t size = element_size(a.dtype);
+    return (((uintptr_t)a.weight | (uint64_t)a.weight_stride * size) & 3) != 0 || a.width * size % 16 != 0;
 }
 
 // Places of the workspace, in bytes.
@@ -196,8 +201,8 @@ inline CrossEntropyPlan cross_entropy_plan(const CrossEntropyArgs &a) {
 // one has at most 256 MiB.
 struct CrossEntropyGradPlan {
     bool copies;
-    uint64_t piece, piece_pitch, rows_pitch; // elements
-    uint64_t x, x_columns, weight, weight_columns, g, g_columns, sums, bytes;
+    uint64_t piece, piece_pitch, sums_pitch; // elements
+    uint64_t x, weight, g, sums, bytes;
 };
 inline CrossEntropyGradPlan cross_entropy_grad_plan(const CrossEntropyGradArgs &a) {
     CrossEntropyGradPlan p{};
@@ -207,20 +212,17 @@ inline CrossEntropyGradPlan cross_entropy_grad_plan(const CrossEntropyGradArgs &
     const uint64_t pieces = std::max<uint64_t>(1, ceil_div(a.vocab, most));
     p.piece = std::max<uint64_t>(256, round_up(ceil_div(a.vocab, pieces), 256));
     p.piece_pitch = round_up(std::min(p.piece, std::max<uint64_t>(1, a.vocab)), whole);
-    p.rows_pitch = round_up(std::max<uint64_t>(1, a.rows), whole);
-    uint64_t at = 256;
+    p.sums_pitch = round_up(a.width, 4);
+    uint64_t at = 256; // the largest gradient lies first
     const auto take = [&](bool is_used, uint64_t bytes) {
         const uint64_t here = at;
         if (is_used) at += round_up(bytes, 256);
         return here;
     };
-    p.x = take(p.copies, a.rows * row);
+    p.x = take(true, a.rows * row);
     p.weight = take(p.copies, p.piece * row);
-    p.x_columns = take(a.grad_weight, a.width * p.rows_pitch * size);
-    p.weight_columns = take(a.grad_x, a.width * p.piece_pitch * size);
     p.g = take(true, a.rows * p.piece_pitch * size);
-    p.g_columns = take(true, p.piece_pitch * p.rows_pitch * size);
-    p.sums = take(a.grad_x && p.piece < a.vocab, a.rows * a.width * 4);
+    p.sums = take(a.grad_x && p.piece < a.vocab, a.rows * p.sums_pitch * 4);
     p.bytes = at;
     return p;
 }
