@@ -23,7 +23,7 @@ namespace {
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kDepth = 128; // bytes of a row a step
+constexpr int kDepth = 128; // bytes of k a step
 
 // 16 bytes of k of 16 rows of either operand.  Of f32 these are four instructions,
 // each with an element of every lane: k in another order, the same for both.
@@ -65,7 +65,7 @@ __device__ __forceinline__ float exp_of(float x) {
 // ---------------------------------------------------------------- product
 // out[m, n] = Σ_k a(m, k)·b(n, k), handed to an epilogue in tiles of BM x BN.  An
 // operand lies in memory by rows of k, a row for each m or n, or across: a row for each
-// k.  A step is 128 bytes of k.  The tile's WM x WN waves each take a part of it.
+// k.  The tile's WM x WN waves each take a part of it.
 struct Operand {
     const int8_t *rows;
     int64_t stride; // bytes, of its rows in memory
@@ -105,34 +105,37 @@ template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
         else return k / 4 % 4 % kTurns;
     }
 
-    // What this thread loads: its chunks' addresses at k = 0.
-    const int8_t *src[kLoads];
-    uint32_t at_k; // by rows: bytes into the row, the same for all of them
-    int64_t stride;
+    // What this thread loads: its chunks' places from `base` on, the tile's first row or
+    // column at k = 0.  Strides are such that 32 bits hold them.
+    const int8_t *base;
+    uint32_t from[kLoads];
+    uint32_t stride;
     __device__ __forceinline__ void open(const Operand &o, uint64_t first, uint64_t end, int wave, int lane) {
-        stride = o.stride;
+        stride = (uint32_t)o.stride;
+        base = o.rows + (ACROSS ? first * sizeof(T) : first * (uint64_t)stride);
+        // Rows past the end repeat the last one, columns past it the last chunk; they
+        // are dropped at the end.
+        const uint32_t last = (uint32_t)min((uint64_t)WIDTH, end - first) - 1;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
             const uint32_t q = (wave * kLoads + j) * kWave + lane, row = q / kChunks, place = q % kChunks;
             if constexpr (ACROSS) {
                 const uint32_t chunk = (place / kSegment ^ turn(row)) * kSegment + place % kSegment;
-                // Columns past the end repeat the last chunk and are dropped at the end.
-                const uint64_t c = min(first + (uint64_t)chunk * kN, (end + kN - 1) / kN * kN - kN);
-                src[j] = o.rows + (int64_t)row * stride + (int64_t)(c * sizeof(T));
+                from[j] = row * stride + min(chunk, last / kN) * 16;
             } else {
-                src[j] = o.rows + (int64_t)min(first + row, end - 1) * stride;
-                if (j == 0) at_k = (place ^ (row % 8)) * 16;
+                from[j] = min(row, last) * stride + (place ^ (row % 8)) * 16;
             }
         }
     }
+    __device__ __forceinline__ const int8_t *at_step(uint32_t step) const {
+        return base + (uint64_t)step * (ACROSS ? kDepth / sizeof(T) * stride : kDepth);
+    }
     __device__ __forceinline__ void fetch(int8_t *stage, uint32_t step, int wave) const {
         int8_t *to = stage + wave * (kLoads * 1024);
+        const int8_t *p = at_step(step);
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const int8_t *from = ACROSS ? src[j] + (int64_t)step * (kDepth / (int)sizeof(T)) * stride
-                                        : src[j] + (uint64_t)step * kDepth + at_k;
-            __builtin_amdgcn_global_load_lds((const void *)from, (lds_void *)(to + j * 1024), 16, 0, 0);
-        }
+        for (int j = 0; j < kLoads; ++j)
+            __builtin_amdgcn_global_load_lds((const void *)(p + from[j]), (lds_void *)(to + j * 1024), 16, 0, 0);
     }
     // The last, partial step: zeros past the end of k.
     __device__ __forceinline__ void fetch_rest(int8_t *stage, uint32_t step, uint64_t k, int wave, int lane) const {
@@ -141,15 +144,17 @@ template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
             u32x4 v = {0, 0, 0, 0};
             if constexpr (ACROSS) {
                 const uint32_t row = ((wave * kLoads + j) * kWave + lane) / kChunks;
-                const uint64_t at = (uint64_t)step * (kDepth / sizeof(T)) + row;
-                if (at < k) v = *(const u32x4_any *)(src[j] + (int64_t)step * (kDepth / (int)sizeof(T)) * stride);
+                if ((uint64_t)step * (kDepth / sizeof(T)) + row < k) v = *(const u32x4_any *)(at_step(step) + from[j]);
             } else {
-                v = load_bytes(src[j], step * kDepth + at_k, (uint32_t)(k * sizeof(T)));
+                const uint32_t row = ((wave * kLoads + j) * kWave + lane) / kChunks, place = lane % kChunks;
+                const uint32_t at_k = (place ^ (row % 8)) * 16;
+                v = load_bytes(base + (from[j] - at_k), step * kDepth + at_k, (uint32_t)(k * sizeof(T)));
             }
             *(u32x4 *)(to + j * 1024) = v;
         }
     }
 
+    static constexpr int kReads = !ACROSS ? 1 : sizeof(T) == 2 ? 2 : 4; // instructions a read
     // Where this lane reads: 16 bytes of k, half `s` of the step, of row `part` + 16·i + lane % 16.
     uint32_t at;
     __device__ __forceinline__ void place(uint32_t part, int lane) {
@@ -184,6 +189,11 @@ template <int BM_, int BN_, int WM_, int WN_, int S_> struct Tile {
     static constexpr int kStage = (BM + BN) * kDepth, kLds = kStage * S;
     static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     static_assert(kLds <= 160 * 1024);
+    // Two waves on each SIMD, which take turns.
+    static constexpr bool kTurns = WM == 2 && WN == 4 && S == 2;
+    // Rows of tiles in a strip: 4 x 8 tiles of 256 x 256 at a time on an XCD's 32 CUs (a
+    // product of 8192 x 16384 x 4096 takes 1087 us, 1148 with 8 rows), 8 x 8 smaller ones.
+    static constexpr int kStrip = BM == 256 ? 4 : 8;
 };
 
 // What an epilogue knows of its place: lane l has, of fragment (i, j), the sums of
@@ -201,14 +211,14 @@ __global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilo
     extern __shared__ __align__(16) int8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 
-    // Blocks go to the eight XCDs in turn: each XCD takes a run of tiles, in
-    // strips of eight tiles of m so that its L2 serves both operands.
+    // Blocks go to the eight XCDs in turn.  Each XCD takes a run of tiles in strips of a
+    // few rows of tiles, so that its L2 serves both operands of those that are under way.
     const uint32_t total = tiles_m * tiles_n, share = total / 8, rest = total % 8;
     const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
     const uint32_t tile = xcd * share + min(xcd, rest) + turn;
-    const uint32_t strip = tile / (8 * tiles_n), in_strip = tile % (8 * tiles_n);
-    const uint32_t height = min(8u, tiles_m - 8 * strip);
-    const uint64_t m0 = (uint64_t)(8 * strip + in_strip % height) * BM, n0 = (uint64_t)(in_strip / height) * BN;
+    const uint32_t strip = tile / (C::kStrip * tiles_n), in_strip = tile % (C::kStrip * tiles_n);
+    const uint32_t height = min((uint32_t)C::kStrip, tiles_m - C::kStrip * strip);
+    const uint64_t m0 = (uint64_t)(C::kStrip * strip + in_strip % height) * BM, n0 = (uint64_t)(in_strip / height) * BN;
 
     constexpr uint32_t kStep = kDepth / sizeof(T);
     const uint32_t steps = (uint32_t)((p.k + kStep - 1) / kStep), whole = (uint32_t)(p.k / kStep);
@@ -253,33 +263,69 @@ __global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilo
             b.fetch_rest(stage + a.kBytes, t, p.k, wave, lane);
         }
     };
-    // A step's second half is read while the first is summed, the next step's
-    // first half while the second is.  Between the two the waves meet: all have read the
-    // step, so that its place is free, and the next step has landed once no more
-    // loads are under way than those of the S - 2 steps behind it.
-    Half first, second;
-    for (int t = 0; t < S; ++t) fetch_any(t);
-    if (steps > 0) {
-        if (S <= whole) step_barrier<(S - 1) * kLoads>();
-        else step_barrier<0>();
-        read(first, 0, 0);
-    }
-    uint32_t t = 0;
-    for (; t + S < whole; ++t) {
-        read(second, t, 1);
-        compute(first);
-        step_barrier<(S - 2) * kLoads>();
-        fetch(t + S);
-        read(first, t + 1, 0);
-        compute(second);
-    }
-    for (; t < steps; ++t) { // the last ones, not all of them direct loads
-        read(second, t, 1);
-        compute(first);
+    if constexpr (C::kTurns) {
+        // Of the two waves on a SIMD one reads and loads while the other one sums, and the
+        // waves meet between the turns: the second four are a turn behind the first four.
+        // A step has four turns of a wave: its first half is read, and summed, then its
+        // second half.  The step after next is loaded to the place of the step before,
+        // which all have read, and has landed two turns later.
+        const auto turn_end = [](auto reads) {
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (reads) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const auto sum = [&](const Half &h) {
+            __builtin_amdgcn_s_setprio(1);
+            compute(h);
+            __builtin_amdgcn_s_setprio(0);
+            turn_end(std::false_type{});
+        };
+        fetch_any(0);
+        fetch_any(1);
         step_barrier<0>();
-        if (t + S < steps) fetch_any(t + S);
-        if (t + 1 < steps) read(first, t + 1, 0);
-        compute(second);
+        if (wave >= 4) turn_end(std::false_type{});
+        Half h;
+        for (uint32_t t = 0; t < steps; ++t) {
+            read(h, t, 0);
+            if (t > 0) fetch_any(t + 1);
+            turn_end(std::true_type{});
+            sum(h);
+            read(h, t, 1);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            turn_end(std::true_type{});
+            sum(h);
+        }
+        if (wave < 4) turn_end(std::false_type{});
+    } else {
+        // A step's second half is read while the first is summed, the next step's
+        // first half while the second is.  Between the two the waves meet: all have read the
+        // step, so that its place is free, and the next step has landed once no more
+        // loads are under way than those of the S - 2 steps behind it.
+        Half first, second;
+        for (int t = 0; t < S; ++t) fetch_any(t);
+        if (steps > 0) {
+            if (S <= whole) step_barrier<(S - 1) * kLoads>();
+            else step_barrier<0>();
+            read(first, 0, 0);
+        }
+        uint32_t t = 0;
+        for (; t + S < whole; ++t) {
+            read(second, t, 1);
+            compute(first);
+            step_barrier<(S - 2) * kLoads>();
+            fetch(t + S);
+            read(first, t + 1, 0);
+            compute(second);
+        }
+        for (; t < steps; ++t) { // the last ones, not all of them direct loads
+            read(second, t, 1);
+            compute(first);
+            step_barrier<0>();
+            if (t + S < steps) fetch_any(t + S);
+            if (t + 1 < steps) read(first, t + 1, 0);
+            compute(second);
+        }
     }
     __syncthreads(); // LDS is the epilogue's
     epilogue.template finish<C>(acc, Place{m0 + wm + lane % 16, n0 + wn + lane / 16 * 4, m0, n0 / BN, wave % C::WN}, p,
@@ -438,6 +484,14 @@ hx_status launch_tiles(const Product &p, const E &epilogue, hipStream_t stream) 
 template <typename T, bool ACROSS_A, bool ACROSS_B, typename E>
 hx_status launch_product(const Product &p, const E &epilogue, hipStream_t stream) {
     if (p.m == 0 || p.n == 0) return HX_OK;
+    // A tile's places from its first row on are counted in 32 bits.
+    const auto fits = [&](const Operand &o, uint64_t rows, bool is_across) {
+        const uint64_t most = is_across ? std::min<uint64_t>(p.k, kDepth / sizeof(T)) : std::min<uint64_t>(rows, 256);
+        return o.stride >= 0 && (uint64_t)o.stride * most < 0xFFFF0000ull;
+    };
+    if (!fits(p.a, p.m, ACROSS_A) || !fits(p.b, p.n, ACROSS_B))
+        return fail(HX_ERR_DISPATCH_FAILED, "product of rows %lld and %lld bytes apart exceeds the range of a tile",
+                    (long long)p.a.stride, (long long)p.b.stride);
     switch (product_tile(p.m, p.n)) {
     case ProductTile::k256x256: return launch_tiles<T, Tile<256, 256, 2, 4, 2>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
     case ProductTile::k128x128: return launch_tiles<T, Tile<128, 128, 2, 2, 2>, ACROSS_A, ACROSS_B>(p, epilogue, stream);

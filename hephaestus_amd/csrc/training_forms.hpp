@@ -168,15 +168,22 @@ inline ProductTile product_tile(uint64_t m, uint64_t n) {
     return ProductTile::k64x64;
 }
 
-// Rows off dwords are copied first, and so are a weight's that end in part of 16 bytes
-// where the backward pass reads them across.
+// The widest rows: places in 256 of them are counted in 32 bits.
+constexpr uint64_t kCrossEntropyWidth = 1 << 20;
+
+// Rows that a product reads where they lie begin on dwords and follow each other by at
+// most 4 MiB; others are copied first.
+inline bool product_reads_rows(const void *rows, int64_t stride, uint64_t size) {
+    return ((uintptr_t)rows | (uint64_t)stride * size) % 4 == 0 && stride >= 0 && (uint64_t)stride * size <= 4 << 20;
+}
 inline bool cross_entropy_copies(const CrossEntropyArgs &a) {
     const uint64_t size = element_size(a.dtype);
-    return (((uintptr_t)a.x | (uintptr_t)a.weight | (uint64_t)(a.x_stride | a.weight_stride) * size) & 3) != 0;
+    return !product_reads_rows(a.x, a.x_stride, size) || !product_reads_rows(a.weight, a.weight_stride, size);
 }
+// x is copied in any case; the weight is read across too, 16 bytes at a time.
 inline bool cross_entropy_copies(const CrossEntropyGradArgs &a) {
     const uint64_t size = element_size(a.dtype);
-    return (((uintptr_t)a.weight | (uint64_t)a.weight_stride * size) & 3) != 0 || a.width * size % 16 != 0;
+    return !product_reads_rows(a.weight, a.weight_stride, size) || a.width * size % 16 != 0;
 }
 
 // Places of the workspace, in bytes.

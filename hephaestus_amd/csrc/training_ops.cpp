@@ -318,10 +318,12 @@ hx_status check_logits(Operands &ops, const View &x, const View &weight, const V
     HX_TRY(ops.in(x, 2, x_shape, size, "loss input"));
     HX_TRY(ops.in(weight, 2, w_shape, size, "vocabulary weight"));
     HX_TRY(ops.in(targets, *rows, 4, "targets"));
-    // Places in rows are counted in 32 bits; 2^31 targets would take 2^53 logits.
-    if (*rows >= 1ull << 28 || *vocab >= 1ull << 28 || *width >= 1ull << 28)
-        return fail(HX_ERR_DISPATCH_FAILED, "loss of %llu rows, a vocabulary of %llu and a width of %llu: each is below 2^28",
-                    (unsigned long long)*rows, (unsigned long long)*vocab, (unsigned long long)*width);
+    if (*rows >= 1ull << 28 || *vocab >= 1ull << 28)
+        return fail(HX_ERR_DISPATCH_FAILED, "loss of %llu rows over a vocabulary of %llu: each is below 2^28",
+                    (unsigned long long)*rows, (unsigned long long)*vocab);
+    if (*width > kCrossEntropyWidth)
+        return fail(HX_ERR_DISPATCH_FAILED, "loss of width %llu: at most %llu", (unsigned long long)*width,
+                    (unsigned long long)kCrossEntropyWidth);
     return HX_OK;
 }
 

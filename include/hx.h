@@ -765,8 +765,8 @@ hx_status hx_prepare_gated_recurrence_backward(
  * x is [rows, width], weight [vocab, width], both of dtype; targets is
  * u32[rows].  A row whose target is not below vocab is left out: its loss is 0.
  * loss and lse are f32[rows]; lse may be NULL.  A logit that is a NaN or plus
- * infinity makes its row's loss and lse a NaN.  rows, vocab and width are below
- * 2^28 each. */
+ * infinity makes its row's loss and lse a NaN.  rows and vocab are below 2^28,
+ * width is at most 2^20. */
 hx_status hx_linear_cross_entropy(
     hx_device *dev, hx_dtype dtype, const void *x, uint64_t x_buf_len,
     const hx_layout *x_layout, const void *weight, uint64_t weight_buf_len,

@@ -127,6 +127,8 @@ REFUSED = [
     (loss, {"x": view(place(0), N([4, 8], [8, 0]), F)}, DF, "contiguous last dimension"),
     (loss, {"x": view(place(0), N([1 << 28, 8], [0, 1]), F, 8), "targets": buffer(place(2), 1 << 28, U),
             "loss": buffer(place(30), 1 << 28, F), "lse": None}, DF, "each is below 2^28"),
+    (loss, {"x": view(place(0), L([4, (1 << 20) + 1]), F), "weight": view(place(1), L([9, (1 << 20) + 1]), F)}, DF,
+     "at most 1048576"),
     # loss, backward
     (loss_grad, {"grad": buffer(place(4), 4, B)}, IC, "gradient of the loss must be float32"),
     (loss_grad, {"grad_x": view(place(5), L([4, 8]), B)}, IC, "gradient of the loss input must be float32"),
