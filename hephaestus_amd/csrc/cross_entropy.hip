@@ -26,17 +26,24 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kDepth = 128; // bytes of k a step
 
 // 16 bytes of k of 16 rows of either operand.  Of f32 these are four instructions,
-// each with an element of every lane: k in another order, the same for both.
-template <typename T> __device__ __forceinline__ f32x4 mma(u32x4 b, u32x4 a, f32x4 sum) {
-    if constexpr (sizeof(T) == 2) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a),
-                                                       sum, 0, 0, 0);
-    } else {
-        const f32x4 fb = __builtin_bit_cast(f32x4, b), fa = __builtin_bit_cast(f32x4, a);
+// each with an element of every lane: k in another order, the same for both.  The
+// fragments' instructions of one element go first: no two in a row add to the same sums.
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void mma(const u32x4 (&b)[FN], const u32x4 (&a)[FM], f32x4 (&sum)[FM][FN]) {
+    constexpr int kEach = sizeof(T) == 2 ? 1 : 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[i], fa[i], sum, 0, 0, 0);
-        return sum;
-    }
+    for (int e = 0; e < kEach; ++e)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                if constexpr (sizeof(T) == 2)
+                    sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, b[j]), __builtin_bit_cast(bf16x8, a[i]), sum[i][j], 0, 0, 0);
+                else
+                    sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        __builtin_bit_cast(f32x4, b[j])[e], __builtin_bit_cast(f32x4, a[i])[e], sum[i][j], 0, 0, 0);
+            }
 }
 
 // 16 bytes of a row from `k` on, zeros from `end` on.
@@ -73,12 +80,63 @@ struct Operand {
 struct Product {
     Operand a, b;
     uint64_t m, n, k; // elements
+    uint64_t span;    // of k, of a part of the grid's second dimension
 };
 
 // The barrier between steps is written out: all of the wave's LDS reads and
 // writes and all but its last N loads have ended when it is passed.
 template <int N> __device__ __forceinline__ void step_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
+
+// Turned reads of LDS, two for each address: x[i] is a column's elements from 4 rows at
+// p[i] and from 4 rows NEXT bytes on.  The builtin would wait for all loads to LDS that
+// are under way, whichever place they go to; the block has the reads' own wait.
+template <int NEXT> __device__ __forceinline__ void read_turned(const uint32_t (&p)[1], u32x4 (&x)[1]) {
+    uint64_t v[2];
+    asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1])
+                 : "v"(p[0]), "n"(NEXT)
+                 : "memory");
+    __builtin_memcpy(x, v, sizeof(v));
+}
+template <int NEXT> __device__ __forceinline__ void read_turned(const uint32_t (&p)[2], u32x4 (&x)[2]) {
+    uint64_t v[4];
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                 : "v"(p[0]), "v"(p[1]), "n"(NEXT)
+                 : "memory");
+    __builtin_memcpy(x, v, sizeof(v));
+}
+template <int NEXT> __device__ __forceinline__ void read_turned(const uint32_t (&p)[4], u32x4 (&x)[4]) {
+    uint64_t v[8];
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),
+                   "=&v"(v[7])
+                 : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(NEXT)
+                 : "memory");
+    __builtin_memcpy(x, v, sizeof(v));
+}
+template <int NEXT> __device__ __forceinline__ void read_turned(const uint32_t (&p)[8], u32x4 (&x)[8]) {
+    uint64_t v[16];
+    asm volatile("ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %2, %17\n\tds_read_b64_tr_b16 %3, %17 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %8, %20\n\tds_read_b64_tr_b16 %9, %20 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %10, %21\n\tds_read_b64_tr_b16 %11, %21 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %12, %22\n\tds_read_b64_tr_b16 %13, %22 offset:%24\n\t"
+                 "ds_read_b64_tr_b16 %14, %23\n\tds_read_b64_tr_b16 %15, %23 offset:%24\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),
+                   "=&v"(v[7]), "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]),
+                   "=&v"(v[14]), "=&v"(v[15])
+                 : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "n"(NEXT)
+                 : "memory");
+    __builtin_memcpy(x, v, sizeof(v));
 }
 
 // One operand's part of a step in LDS, WIDTH rows of m or n; loads go from memory
@@ -154,7 +212,6 @@ template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
         }
     }
 
-    static constexpr int kReads = !ACROSS ? 1 : sizeof(T) == 2 ? 2 : 4; // instructions a read
     // Where this lane reads: 16 bytes of k, half `s` of the step, of row `part` + 16·i + lane % 16.
     uint32_t at;
     __device__ __forceinline__ void place(uint32_t part, int lane) {
@@ -163,22 +220,23 @@ template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
             at = (lane / 16 * 8 + lane % 16 / 4) * kRow + ((part / 16 ^ turn(lane / 16 * 8 + lane % 16 / 4)) * 32) + lane % 4 * 8;
         else at = (lane / 16 * 4) * kRow + ((part / 16 ^ turn(lane / 16 * 4)) * 64) + lane % 16 * 4;
     }
-    __device__ __forceinline__ u32x4 read(const int8_t *stage, int i, int s) const {
-        if constexpr (!ACROSS) return *(const u32x4 *)(stage + (at ^ (64 * s)) + i * (16 * kDepth));
-        else if constexpr (sizeof(T) == 2) {
-            typedef short Four __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) Four lds_four;
-            const int8_t *p = stage + (at ^ (32 * i)) + s * (32 * kRow);
-            const Four lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four *)p);
-            const Four hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four *)(p + 4 * kRow));
-            typedef short Eight __attribute__((ext_vector_type(8)));
-            return __builtin_bit_cast(u32x4, (Eight)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        } else {
-            u32x4 v;
-            const int8_t *p = stage + (at ^ (64 * i)) + s * (16 * kRow);
+    // N fragments of half `s`.
+    template <int N> __device__ __forceinline__ void read(const int8_t *stage, int s, u32x4 (&x)[N]) const {
+        if constexpr (!ACROSS) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = *(const uint32_t *)(p + e * kRow);
-            return v;
+            for (int i = 0; i < N; ++i) x[i] = *(const u32x4 *)(stage + (at ^ (64 * s)) + i * (16 * kDepth));
+        } else if constexpr (sizeof(T) == 2) {
+            uint32_t p[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                p[i] = (uint32_t)(uintptr_t)(lds_void *)(stage + s * (32 * kRow)) + (at ^ (32 * i));
+            read_turned<4 * kRow>(p, x);
+        } else {
+            const int8_t *p = stage + s * (16 * kRow);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = *(const uint32_t *)(p + (at ^ (64 * i)) + e * kRow);
         }
     }
 };
@@ -221,6 +279,10 @@ __global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilo
     const uint64_t m0 = (uint64_t)(C::kStrip * strip + in_strip % height) * BM, n0 = (uint64_t)(in_strip / height) * BN;
 
     constexpr uint32_t kStep = kDepth / sizeof(T);
+    const uint64_t k0 = blockIdx.y * p.span; // parts are whole steps
+    p.k = min(p.span, p.k - k0);
+    p.a.rows += k0 * (ACROSS_A ? (uint64_t)p.a.stride : sizeof(T));
+    p.b.rows += k0 * (ACROSS_B ? (uint64_t)p.b.stride : sizeof(T));
     const uint32_t steps = (uint32_t)((p.k + kStep - 1) / kStep), whole = (uint32_t)(p.k / kStep);
     Staged<T, BM, C::kThreads, ACROSS_A> a;
     Staged<T, BN, C::kThreads, ACROSS_B> b;
@@ -238,17 +300,10 @@ __global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilo
     };
     const auto read = [&](Half &h, uint32_t t, int s) {
         const int8_t *stage = lds + t % S * C::kStage;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) h.b[j] = b.read(stage + a.kBytes, j, s);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) h.a[i] = a.read(stage, i, s);
+        b.read(stage + a.kBytes, s, h.b);
+        a.read(stage, s, h.a);
     };
-    const auto compute = [&](const Half &h) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(h.b[j], h.a[i], acc[i][j]);
-    };
+    const auto compute = [&](const Half &h) { mma<T>(h.b, h.a, acc); };
     const auto fetch = [&](uint32_t t) {
         int8_t *stage = lds + t % S * C::kStage;
         a.fetch(stage, t, wave);
@@ -432,12 +487,13 @@ template <typename T> struct TileGradient {
     }
 };
 
-// scale·(sum + what earlier pieces summed up): to `out`, or on to the next piece.  Rows
-// without a target get zeros where `targets` is given.
+// scale·(sum + what earlier pieces summed up): to `out`, or, the sum alone, to `after`, where
+// it goes on to the next piece or is a part's.  Rows without a target get zeros where
+// `targets` is given.
 template <typename T> struct TileOut {
     const float *scale;
     const float *before; // may be null
-    float *after;        // may be null: this is the last piece
+    float *after;        // may be null
     T *out;
     uint64_t sum_pitch;
     int64_t out_stride;
@@ -458,7 +514,7 @@ template <typename T> struct TileOut {
                 f32x4 v = acc[i][j];
                 if (before) v += *(const f32x4 *)(before + row * sum_pitch + n); // the pitch is whole vectors
                 if (after) {
-                    *(f32x4 *)(after + row * sum_pitch + n) = v;
+                    *(f32x4 *)(after + (blockIdx.y * p.m + row) * sum_pitch + n) = v;
                 } else {
                     v *= by;
                     if (is_left_out) v = f32x4{0, 0, 0, 0};
@@ -469,20 +525,40 @@ template <typename T> struct TileOut {
     }
 };
 
+// The parts' sums of four columns of a row, added up in order, and on as TileOut does.
+template <typename T>
+__global__ __launch_bounds__(256) void fold_parts_kernel(const float *parts, uint32_t count, uint64_t m, uint64_t n,
+                                                        TileOut<T> out) {
+    const uint64_t vectors = out.sum_pitch / 4;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < m * vectors; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = i / vectors, c = i % vectors * 4, at = row * out.sum_pitch + c;
+        f32x4 v = *(const f32x4 *)(parts + at);
+        for (uint32_t p = 1; p < count; ++p) v += *(const f32x4 *)(parts + (uint64_t)p * m * out.sum_pitch + at);
+        if (out.before) v += *(const f32x4 *)(out.before + at);
+        if (out.after) {
+            *(f32x4 *)(out.after + at) = v;
+        } else {
+            v *= *out.scale;
+            if (out.targets && out.targets[row] >= out.vocab) v = f32x4{0, 0, 0, 0};
+            store_four(out.out + (int64_t)row * out.out_stride + (int64_t)c, c, n, v);
+        }
+    }
+}
+
 template <typename T, typename C, bool ACROSS_A, bool ACROSS_B, typename E>
-hx_status launch_tiles(const Product &p, const E &epilogue, hipStream_t stream) {
+hx_status launch_tiles(const Product &p, uint32_t parts, const E &epilogue, hipStream_t stream) {
     const auto kernel = product_kernel<T, C, ACROSS_A, ACROSS_B, E>;
     static std::atomic<uint64_t> allowed{0};
     HX_TRY(allow_lds((const void *)kernel, C::kLds, allowed));
     const uint64_t tm = ceil_div(p.m, C::BM), tn = ceil_div(p.n, C::BN);
     if (tm * tn * C::kThreads > 0xFFFFFFFFull)
         return fail(HX_ERR_DISPATCH_FAILED, "product of %llu tiles exceeds the grid range", (unsigned long long)(tm * tn));
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(C::kThreads), C::kLds, stream, p, epilogue,
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn), parts), dim3(C::kThreads), C::kLds, stream, p, epilogue,
                        (uint32_t)tm, (uint32_t)tn);
     return check_launch("product_kernel");
 }
 template <typename T, bool ACROSS_A, bool ACROSS_B, typename E>
-hx_status launch_product(const Product &p, const E &epilogue, hipStream_t stream) {
+hx_status launch_product(Product p, const ProductCut &cut, const E &epilogue, hipStream_t stream) {
     if (p.m == 0 || p.n == 0) return HX_OK;
     // A tile's places from its first row on are counted in 32 bits.
     const auto fits = [&](const Operand &o, uint64_t rows, bool is_across) {
@@ -492,13 +568,34 @@ hx_status launch_product(const Product &p, const E &epilogue, hipStream_t stream
     if (!fits(p.a, p.m, ACROSS_A) || !fits(p.b, p.n, ACROSS_B))
         return fail(HX_ERR_DISPATCH_FAILED, "product of rows %lld and %lld bytes apart exceeds the range of a tile",
                     (long long)p.a.stride, (long long)p.b.stride);
-    switch (product_tile(p.m, p.n)) {
-    case ProductTile::k256x256: return launch_tiles<T, Tile<256, 256, 2, 4, 2>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
-    case ProductTile::k128x128: return launch_tiles<T, Tile<128, 128, 2, 2, 2>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
-    case ProductTile::k64x64: return launch_tiles<T, Tile<64, 64, 4, 2, 4>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
-    case ProductTile::k32x64: return launch_tiles<T, Tile<32, 64, 1, 4, 6>, ACROSS_A, ACROSS_B>(p, epilogue, stream);
+    p.span = cut.span;
+    switch (cut.tile) {
+    case ProductTile::k256x256:
+        return launch_tiles<T, Tile<256, 256, 2, 4, 2>, ACROSS_A, ACROSS_B>(p, cut.parts, epilogue, stream);
+    case ProductTile::k128x128:
+        return launch_tiles<T, Tile<128, 128, 2, 4, 4>, ACROSS_A, ACROSS_B>(p, cut.parts, epilogue, stream);
+    case ProductTile::k64x128:
+        return launch_tiles<T, Tile<64, 128, 2, 4, 3>, ACROSS_A, ACROSS_B>(p, cut.parts, epilogue, stream);
+    case ProductTile::k64x64:
+        return launch_tiles<T, Tile<64, 64, 2, 2, 4>, ACROSS_A, ACROSS_B>(p, cut.parts, epilogue, stream);
+    case ProductTile::k32x64:
+        return launch_tiles<T, Tile<32, 64, 1, 4, 6>, ACROSS_A, ACROSS_B>(p, cut.parts, epilogue, stream);
     }
     return HX_OK;
+}
+// A product to `out`, in parts of k where that is shorter.
+template <typename T, bool ACROSS_A, bool ACROSS_B>
+hx_status launch_sums(const Product &p, const TileOut<T> &out, float *parts, hipStream_t stream) {
+    const ProductCut cut = product_cut(p.m, p.n, p.k, sizeof(T), true);
+    if (cut.parts <= 1 || p.m == 0 || p.n == 0) return launch_product<T, ACROSS_A, ACROSS_B>(p, cut, out, stream);
+    TileOut<T> part = out;
+    part.before = nullptr;
+    part.after = parts;
+    HX_TRY((launch_product<T, ACROSS_A, ACROSS_B>)(p, cut, part, stream));
+    const uint64_t blocks = std::min<uint64_t>(ceil_div(p.m * (out.sum_pitch / 4), 256), 1 << 16);
+    hipLaunchKernelGGL(fold_parts_kernel<T>, dim3((uint32_t)blocks), dim3(256), 0, stream, parts, cut.parts, p.m, p.n,
+                       out);
+    return check_launch("fold_parts_kernel");
 }
 
 // ------------------------------------------------------------------ rows
@@ -520,19 +617,28 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const int8_t *from, int6
     }
 }
 
-// The tiles' sums of a row, joined in one order: 16 rows a block.
+// The tiles' sums of a row, joined in one order: ROWS rows a block, 256 / ROWS threads a
+// row.  Many rows are read side by side, few rows by more threads.
+template <int ROWS>
 __global__ __launch_bounds__(256) void join_stats_kernel(const float2 *stats, const float *picked,
                                                          const uint32_t *targets, uint64_t tiles, uint64_t rows,
                                                          uint64_t vocab, float *loss, float *lse) {
-    __shared__ float2 part[16][17];
-    const uint64_t row = (uint64_t)blockIdx.x * 16 + threadIdx.x % 16;
+    constexpr int kThreads = 256 / ROWS;
+    __shared__ float2 part[kThreads][ROWS];
+    const uint64_t row = (uint64_t)blockIdx.x * ROWS + threadIdx.x % ROWS;
     float2 s = {-__builtin_inff(), 0.0f};
     if (row < rows)
-        for (uint64_t t = threadIdx.x / 16; t < tiles; t += 16) s = TileStats::join(s, stats[t * rows + row]);
-    part[threadIdx.x / 16][threadIdx.x % 16] = s;
-    __syncthreads();
-    if (threadIdx.x >= 16 || row >= rows) return;
-    for (int i = 1; i < 16; ++i) s = TileStats::join(s, part[i][threadIdx.x]);
+        for (uint64_t t = threadIdx.x / ROWS; t < tiles; t += kThreads) s = TileStats::join(s, stats[t * rows + row]);
+    part[threadIdx.x / ROWS][threadIdx.x % ROWS] = s;
+#pragma unroll
+    for (int half = kThreads / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if ((int)threadIdx.x / ROWS < half) {
+            s = TileStats::join(s, part[threadIdx.x / ROWS + half][threadIdx.x % ROWS]);
+            part[threadIdx.x / ROWS][threadIdx.x % ROWS] = s;
+        }
+    }
+    if (threadIdx.x >= ROWS || row >= rows) return;
     const float l = s.x + logf(s.y);
     if (lse) lse[row] = l;
     loss[row] = targets[row] < vocab ? l - picked[row] : 0.0f;
@@ -574,16 +680,21 @@ template <typename T> hx_status launch(const CrossEntropyArgs &a, void *ws, hipS
     float *picked = (float *)(base + plan.picked);
     const int64_t size = sizeof(T), row = (int64_t)round_up(a.width * size, kDepth);
     Product p{{(const int8_t *)a.x, a.x_stride * size}, {(const int8_t *)a.weight, a.weight_stride * size}, a.rows,
-              a.vocab, a.width};
+              a.vocab, a.width, 0};
     if (plan.copies) {
         HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, nullptr, 0, stream));
         HX_TRY(copy_rows<T>(a.weight, a.weight_stride, a.vocab, a.width, base + plan.weight, nullptr, 0, stream));
         p.a = {(const int8_t *)base + plan.x, row};
         p.b = {(const int8_t *)base + plan.weight, row};
     }
-    HX_TRY((launch_product<T, false, false>)(p, TileStats{stats, picked, a.targets}, stream));
-    hipLaunchKernelGGL(join_stats_kernel, dim3((uint32_t)ceil_div(a.rows, 16)), dim3(256), 0, stream, stats, picked,
-                       a.targets, a.vocab ? plan.tiles_n : 0, a.rows, a.vocab, a.loss, a.lse);
+    HX_TRY((launch_product<T, false, false>)(p, plan.cut, TileStats{stats, picked, a.targets}, stream));
+    const uint64_t tiles = a.vocab ? plan.tiles_n : 0;
+    if (a.rows >= 2048)
+        hipLaunchKernelGGL(join_stats_kernel<16>, dim3((uint32_t)ceil_div(a.rows, 16)), dim3(256), 0, stream, stats,
+                           picked, a.targets, tiles, a.rows, a.vocab, a.loss, a.lse);
+    else
+        hipLaunchKernelGGL(join_stats_kernel<1>, dim3((uint32_t)a.rows), dim3(256), 0, stream, stats, picked, a.targets,
+                           tiles, a.rows, a.vocab, a.loss, a.lse);
     return check_launch("join_stats_kernel");
 }
 
@@ -596,7 +707,7 @@ template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, 
     const int64_t size = sizeof(T), row = (int64_t)round_up(a.width * size, kDepth);
     const Operand x{(const int8_t *)base + plan.x, row};
     HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, a.targets, a.vocab, stream));
-    float *sums = (float *)(base + plan.sums);
+    float *sums = (float *)(base + plan.sums), *parts = (float *)(base + plan.parts);
     T *g = (T *)(base + plan.g);
     const Operand go{(const int8_t *)g, (int64_t)plan.piece_pitch * size};
     for (uint64_t first = 0; first < a.vocab || first == 0; first += plan.piece) {
@@ -607,7 +718,8 @@ template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, 
             HX_TRY(copy_rows<T>(from, a.weight_stride, n, a.width, base + plan.weight, nullptr, 0, stream));
             w = {(const int8_t *)base + plan.weight, row};
         }
-        HX_TRY((launch_product<T, false, false>)(Product{x, w, a.rows, n, a.width},
+        HX_TRY((launch_product<T, false, false>)(Product{x, w, a.rows, n, a.width, 0},
+                                                 product_cut(a.rows, n, a.width, sizeof(T), false),
                                                  TileGradient<T>{g, plan.piece_pitch, first, a.vocab, a.targets, a.lse,
                                                                  a.grad, most},
                                                  stream));
@@ -615,12 +727,12 @@ template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, 
             const bool is_last = first + n >= a.vocab;
             const TileOut<T> out{most, first ? sums : nullptr, is_last ? nullptr : sums, (T *)a.grad_x, plan.sums_pitch,
                                  a.grad_x_stride, a.targets, a.vocab};
-            HX_TRY((launch_product<T, false, true>)(Product{go, w, a.rows, a.width, n}, out, stream));
+            HX_TRY((launch_sums<T, false, true>)(Product{go, w, a.rows, a.width, n, 0}, out, parts, stream));
         }
         if (a.grad_weight) {
-            const TileOut<T> out{most, nullptr, nullptr, (T *)a.grad_weight + (int64_t)first * a.grad_weight_stride, 0,
+            const TileOut<T> out{most, nullptr, nullptr, (T *)a.grad_weight + (int64_t)first * a.grad_weight_stride, plan.sums_pitch,
                                  a.grad_weight_stride, nullptr, 0};
-            HX_TRY((launch_product<T, true, true>)(Product{go, x, n, a.width, a.rows}, out, stream));
+            HX_TRY((launch_sums<T, true, true>)(Product{go, x, n, a.width, a.rows, 0}, out, parts, stream));
         }
     }
     return HX_OK;

@@ -81,7 +81,7 @@ struct Map {
     }
     __device__ __forceinline__ void then_by(float by) {
         a = apply(by, a);
-        off = __builtin_signbit(by) ? __builtin_fmaf(-by, 1.0f - off, off) : 1.0f - by * (1.0f - off);
+        off = __builtin_signbit(by) ? __builtin_fmaf(-by, 1.0f - off, off) : __builtin_fmaf(-by, 1.0f - off, 1.0f);
     }
     __device__ __forceinline__ float by() const { return off <= 0.5f ? -off : a; }
 };
@@ -176,6 +176,7 @@ __global__ __launch_bounds__(WAVES *kWave) void recurrence_kernel(RecurrenceArgs
         state_at<V>(nullptr, 0, carry);
     } else if (p.parts > 1) {
         state_at(p.at(batch, p.parts - 1, 1), c, carry);
+#pragma unroll 8
         for (uint32_t i = 0; i < part; ++i) {
             float by[V], b[V];
             state_at(p.at(batch, i, 0), c, by);
@@ -299,6 +300,7 @@ __global__ __launch_bounds__(WAVES *kWave) void recurrence_grad_kernel(Recurrenc
         state_at(a.state_in ? a.state_in + (int64_t)batch * a.s_state_in : nullptr, c, before);
         if (p.parts > 1) {
             state_at(p.at(batch, 0, 1), c, carry);
+#pragma unroll 8
             for (uint32_t i = p.parts - 1; i > part; --i) {
                 float by[V], b[V];
                 state_at(p.at(batch, i, 0), c, by);
@@ -403,7 +405,7 @@ __global__ __launch_bounds__(WAVES *kWave) void recurrence_grad_kernel(Recurrenc
 
 template <typename T, int V, typename Args> hx_status launch(const Args &a, void *ws, hipStream_t stream) {
     constexpr bool kGrad = std::is_same<Args, RecurrenceGradArgs>::value;
-    const RecurrenceParts cut = recurrence_parts(a, V);
+    const RecurrenceParts cut = recurrence_parts(a, V, kGrad);
     const PartMaps p{(float *)ws, cut.parts, cut.span, a.channels};
     const uint64_t groups = ceil_div(a.channels, kWave * V);
     if (groups * cut.parts * 512 > 0xFFFFFFFFull)
@@ -418,7 +420,7 @@ template <typename T, int V, typename Args> hx_status launch(const Args &a, void
         switch (cut.tile) {
         case RecurrenceTile::kOne: return run(recurrence_grad_kernel<T, V, 1, 1, false>, 1);
         case RecurrenceTile::kFew: return run(recurrence_grad_kernel<T, V, 1, 8, false>, 1);
-        case RecurrenceTile::kMany:
+        default:
             if (cut.parts > 1) HX_TRY(run(recurrence_grad_kernel<T, V, 8, 8, true>, 8));
             return run(recurrence_grad_kernel<T, V, 8, 8, false>, 8);
         }
@@ -427,8 +429,9 @@ template <typename T, int V, typename Args> hx_status launch(const Args &a, void
         case RecurrenceTile::kOne: return run(recurrence_kernel<T, V, 1, 1, false>, 1);
         case RecurrenceTile::kFew: return run(recurrence_kernel<T, V, 1, 8, false>, 1);
         case RecurrenceTile::kMany:
-            if (cut.parts > 1) HX_TRY(run(recurrence_kernel<T, V, 8, 16, true>, 8));
-            return run(recurrence_kernel<T, V, 8, 16, false>, 8);
+            if (cut.parts > 1) HX_TRY(run(recurrence_kernel<T, V, 8, 8, true>, 8));
+            return run(recurrence_kernel<T, V, 8, 8, false>, 8);
+        case RecurrenceTile::kLong: return run(recurrence_kernel<T, V, 8, 16, false>, 8);
         }
     }
     return HX_OK;
@@ -442,7 +445,8 @@ template <typename Args> hx_status launch_any(const Args &a, void *ws, hipStream
 }
 template <typename Args> uint64_t maps_bytes(const Args &a) {
     if (a.batch == 0 || a.channels == 0) return 0;
-    const RecurrenceParts cut = recurrence_parts(a, recurrence_on_dwords(a) && a.dtype != HX_DTYPE_F32 ? 2 : 1);
+    const RecurrenceParts cut = recurrence_parts(a, recurrence_on_dwords(a) && a.dtype != HX_DTYPE_F32 ? 2 : 1,
+                                                 std::is_same<Args, RecurrenceGradArgs>::value);
     return cut.parts > 1 ? a.batch * cut.parts * 2 * a.channels * sizeof(float) : 0;
 }
 

@@ -316,20 +316,31 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
         vw[s] = place_part<T>(load_part((const T *)a.weight, c, cols), c, cols);
     }
     typename SumsOf<LANES>::type sums;
-    for (uint64_t row = first + group; row < end; row += kRows) {
+    struct Row {
+        u32x4 x[STEPS], dy[STEPS], past[STEPS];
+        float mean, rstd;
+    } now, next;
+    const auto fetch = [&](uint64_t row, Row &r) {
         const T *x = (const T *)a.x + (int64_t)row * a.x_stride;
         const T *dy = (const T *)a.grad_out + (int64_t)row * a.grad_out_stride;
         const T *past = (const T *)a.residual_grad + (int64_t)row * a.residual_grad_stride;
-        u32x4 vx[STEPS], vy[STEPS], vp[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const uint32_t c = ((uint32_t)s * LANES + lane) * N;
-            vx[s] = load_part(x, c, cols);
-            vy[s] = load_part(dy, c, cols);
-            vp[s] = u32x4{0, 0, 0, 0};
-            if (a.residual_grad) vp[s] = load_part(past, c, cols);
+            r.x[s] = load_part(x, c, cols);
+            r.dy[s] = load_part(dy, c, cols);
+            r.past[s] = u32x4{0, 0, 0, 0};
+            if (a.residual_grad) r.past[s] = load_part(past, c, cols);
         }
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        r.mean = a.mean[row];
+        r.rstd = a.rstd[row];
+    };
+    // The next row is on its way while this one is summed.
+    if (first + group < end) fetch(first + group, now);
+    for (uint64_t row = first + group; row < end; row += kRows, now = next) {
+        if (row + kRows < end) fetch(row + kRows, next);
+        u32x4(&vx)[STEPS] = now.x, (&vy)[STEPS] = now.dy, (&vp)[STEPS] = now.past;
+        const float mean = now.mean, rstd = now.rstd;
         float st = 0.0f, stu = 0.0f;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {

@@ -95,14 +95,20 @@ inline NormRow layer_norm_row(uint64_t cols, uint64_t size) {
     return NormRow::kLong;
 }
 
-// The backward pass: runs of rows, a block each.
+// The backward pass: runs of rows, a block each, in whole rounds of the 256 CUs where
+// the rows allow.  Blocks of few waves need more of them side by side.  Measured (us, with
+// the launch that adds up the blocks' sums):
+//   16384 x 8192 bf16  256 blocks 212   382 blocks 262   512 blocks 224   1024 blocks 263
+//   16384 x 2048 bf16  256 blocks 76    512 blocks 52    1024 blocks 53   2048 blocks 72
+//   16384 x 1024 bf16  256 blocks 29    512 blocks 26    1024 blocks 31
+//   1000 x 5001 f32    250 blocks 20    500 blocks 32    1000 blocks 50
 struct NormGradSplit {
     uint32_t blocks, rows_a_block;
 };
 inline NormGradSplit layer_norm_grad_split(const LayerNormGradArgs &a) {
     const uint64_t vectors = ceil_div(a.cols, 16 / element_size(a.dtype));
     const uint64_t at_once = vectors <= 16 ? 16 : vectors <= 128 ? 4 : 1; // rows of a block
-    const uint64_t most = 1024;
+    const uint64_t most = vectors <= 256 ? 512 : 256;
     const uint64_t rows = std::max<uint64_t>(at_once, round_up(ceil_div(a.rows, most), at_once));
     return {(uint32_t)std::max<uint64_t>(1, ceil_div(a.rows, rows)), (uint32_t)rows};
 }
@@ -124,48 +130,87 @@ inline bool recurrence_on_dwords(const RecurrenceGradArgs &a) {
     return bits % 2 == 0 && (strides & 1) == 0;
 }
 
-// Tokens that a block takes together: one wave's, or eight waves'.
-enum class RecurrenceTile : uint32_t { kOne, kFew, kMany };
-inline uint64_t recurrence_tile_tokens(const RecurrenceArgs &) { return 8 * 16; }
-inline uint64_t recurrence_tile_tokens(const RecurrenceGradArgs &) { return 8 * 8; }
+// Tokens that a block takes together: one wave's 1 or 8, or eight waves' 8 or 16 each.
+enum class RecurrenceTile : uint32_t { kOne, kFew, kMany, kLong };
 
+// Where sequences and channels give fewer blocks than half the card takes, the tokens
+// are cut into parts, at the price of reading two of the operands twice.  Tiles of 128 tokens
+// keep more loads under way in a block, tiles of 64 take fewer registers where two
+// blocks share a CU; the backward pass has no registers for 128.  Measured (us, both launches):
+//   8 x 4096 x 4096 bf16, 256 blocks   128 tokens 179   64 tokens 234   two parts 286
+//   4 x 2000 x 1600 bf16, 52 blocks    8 parts of 64-token tiles 39, of 128 46   4 parts 56
+//   1 x 65536 x 2048, backward, 16     32 parts 477   64 parts 500   16 parts 497
+//   8 x 4096 x 4096, backward, 256     one part 320   two parts 463
 struct RecurrenceParts {
     RecurrenceTile tile;
     uint32_t parts, span;
 };
 // `vector` channels a lane.
-template <typename Args> RecurrenceParts recurrence_parts(const Args &a, uint64_t vector) {
+template <typename Args> RecurrenceParts recurrence_parts(const Args &a, uint64_t vector, bool is_backward) {
     const uint64_t all = std::max<uint64_t>(1, a.tokens);
     if (a.tokens <= 1) return {RecurrenceTile::kOne, 1, (uint32_t)all};
     if (a.tokens <= 32) return {RecurrenceTile::kFew, 1, (uint32_t)all};
-    const uint64_t tile = recurrence_tile_tokens(a), blocks = a.batch * ceil_div(a.channels, 64 * vector);
-    const uint64_t tiles = ceil_div(all, tile);
-    uint64_t parts = 1;
-    if (blocks < 192) parts = std::min(ceil_div(512, blocks), ceil_div(tiles, 2));
-    const uint64_t span = ceil_div(tiles, std::max<uint64_t>(1, parts)) * tile;
+    const uint64_t blocks = a.batch * ceil_div(a.channels, 64 * vector), tiles = ceil_div(all, 64);
+    if (blocks >= 160 || tiles < 4) {
+        const bool is_long = !is_backward && all > 64;
+        return {is_long ? RecurrenceTile::kLong : RecurrenceTile::kMany, 1, (uint32_t)round_up(all, 64)};
+    }
+    const uint64_t parts = std::min<uint64_t>(512 / std::max<uint64_t>(1, blocks), tiles / 2);
+    const uint64_t span = ceil_div(tiles, parts) * 64;
     return {RecurrenceTile::kMany, (uint32_t)ceil_div(all, span), (uint32_t)span};
 }
 
 // ---------------------------------------------------------- cross entropy
 
-enum class ProductTile : uint32_t { k256x256, k128x128, k64x64, k32x64 };
-struct ProductTileSize {
+// Tiles of a product: rows x columns.
+enum class ProductTile : uint32_t { k256x256, k128x128, k64x128, k64x64, k32x64 };
+struct ProductTileRule {
     uint64_t m, n;
+    uint64_t at_once; // blocks that share a CU
+    // us for a step of 128 bytes of k with one block on each CU, and with all that share
+    // it: of bf16, as measured on products of 256 x 4096 x 4096 to 2048 x 8192 x 2048, by rows
+    // and across; of f32, where the matrix instructions bound all of them.
+    double one, all, one_f32, all_f32;
 };
-inline ProductTileSize product_tile_size(ProductTile t) {
-    switch (t) {
-    case ProductTile::k256x256: return {256, 256};
-    case ProductTile::k128x128: return {128, 128};
-    case ProductTile::k64x64: return {64, 64};
-    default: return {32, 64};
+constexpr ProductTileRule kProductTiles[] = {
+    {256, 256, 1, 1.70, 1.70, 7.60, 7.60}, {128, 128, 1, 0.56, 0.56, 2.00, 2.00}, {64, 128, 2, 0.34, 0.60, 1.08, 2.10},
+    {64, 64, 2, 0.30, 0.44, 0.60, 1.06},   {32, 64, 2, 0.23, 0.31, 0.33, 0.58}};
+
+// How a product is cut: into tiles, and along k into parts whose sums are added up by a
+// launch of their own.
+struct ProductCut {
+    ProductTile tile;
+    uint32_t parts;
+    uint64_t span; // k of a part, a whole number of steps
+};
+// The shortest by an estimate: rounds of blocks on the card's 256 CUs times a block's
+// steps, a launch and the parts' sums, written and read at 5 TB/s.  Measured (us):
+//   1000 x 5008 x 1040 bf16   64 x 128 25.6   128 x 128 28.8   256 x 256 37.7   64 x 64 29.4
+//   2048 x 8192 x 2048 bf16  256 x 256 59.9   128 x 128 77.0   64 x 128 83.6
+//   256 x 4096 x 4096 bf16    64 x 64 20.4     64 x 128 25.9   128 x 128 34.7
+//   1000 x 5008 x 1040 f32    64 x 64 100.6   128 x 128 145
+inline ProductCut product_cut(uint64_t m, uint64_t n, uint64_t k, uint64_t size, bool may_split) {
+    constexpr uint64_t kCus = 256;
+    const uint64_t step = 128 / size, steps = std::max<uint64_t>(1, ceil_div(k, step));
+    ProductCut best{ProductTile::k32x64, 1, steps * step};
+    double best_us = 0.0;
+    for (uint32_t t = 0; t < sizeof(kProductTiles) / sizeof(*kProductTiles); ++t) {
+        const ProductTileRule &r = kProductTiles[t];
+        const double one = size == 4 ? r.one_f32 : r.one, all = size == 4 ? r.all_f32 : r.all;
+        const uint64_t tiles = ceil_div(m, r.m) * ceil_div(n, r.n);
+        for (uint64_t parts = 1; parts <= (may_split ? 32 : 1) && (parts == 1 || steps / parts >= 4); parts *= 2) {
+            const uint64_t blocks = tiles * parts, full = blocks / (kCus * r.at_once), rest = blocks % (kCus * r.at_once);
+            const double rounds = full * all + (rest == 0 ? 0.0 : rest <= kCus ? one : all);
+            double us = rounds * ceil_div(steps, parts) + 2.0 * (full + 1);
+            if (parts > 1) us += 4.0 + (double)(m * n * parts) * 8 / 5e6;
+            if (best_us == 0.0 || us < best_us) {
+                best_us = us;
+                const uint64_t span = ceil_div(steps, parts) * step;
+                best = {(ProductTile)t, (uint32_t)std::max<uint64_t>(1, ceil_div(k, span)), span};
+            }
+        }
     }
-}
-inline ProductTile product_tile(uint64_t m, uint64_t n) {
-    const auto tiles = [&](uint64_t bm, uint64_t bn) { return ceil_div(m, bm) * ceil_div(n, bn); };
-    if (m <= 32) return ProductTile::k32x64;
-    if (tiles(256, 256) >= 160) return ProductTile::k256x256;
-    if (tiles(128, 128) >= 192) return ProductTile::k128x128;
-    return ProductTile::k64x64;
+    return best;
 }
 
 // The widest rows: places in 256 of them are counted in 32 bits.
@@ -189,13 +234,15 @@ inline bool cross_entropy_copies(const CrossEntropyGradArgs &a) {
 // Places of the workspace, in bytes.
 struct CrossEntropyPlan {
     bool copies;
+    ProductCut cut;
     uint64_t tiles_n, stats, picked, x, weight, bytes;
 };
 inline CrossEntropyPlan cross_entropy_plan(const CrossEntropyArgs &a) {
     CrossEntropyPlan p{};
     const uint64_t row = round_up(a.width * element_size(a.dtype), 128);
     p.copies = cross_entropy_copies(a);
-    p.tiles_n = ceil_div(a.vocab, product_tile_size(product_tile(a.rows, a.vocab)).n);
+    p.cut = product_cut(a.rows, a.vocab, a.width, element_size(a.dtype), false);
+    p.tiles_n = ceil_div(a.vocab, kProductTiles[(uint32_t)p.cut.tile].n);
     p.stats = 0;
     p.picked = round_up(p.tiles_n * a.rows * 8, 256);
     p.x = round_up(p.picked + a.rows * 4, 256);
@@ -209,7 +256,7 @@ inline CrossEntropyPlan cross_entropy_plan(const CrossEntropyArgs &a) {
 struct CrossEntropyGradPlan {
     bool copies;
     uint64_t piece, piece_pitch, sums_pitch; // elements
-    uint64_t x, weight, g, sums, bytes;
+    uint64_t x, weight, g, sums, parts, bytes;
 };
 inline CrossEntropyGradPlan cross_entropy_grad_plan(const CrossEntropyGradArgs &a) {
     CrossEntropyGradPlan p{};
@@ -230,6 +277,24 @@ inline CrossEntropyGradPlan cross_entropy_grad_plan(const CrossEntropyGradArgs &
     p.weight = take(p.copies, p.piece * row);
     p.g = take(true, a.rows * p.piece_pitch * size);
     p.sums = take(a.grad_x && p.piece < a.vocab, a.rows * p.sums_pitch * 4);
+    // Sums of parts of k, of grad_x or of a piece of grad_weight.
+    const uint64_t piece = std::min(p.piece, a.vocab);
+    uint64_t parts = 0;
+    if (a.grad_x) {
+        const uint64_t rest = a.vocab % p.piece ? a.vocab % p.piece : piece; // the last piece's cut may differ
+        for (uint64_t k : {piece, rest}) {
+            const uint32_t n = product_cut(a.rows, a.width, k, size, true).parts;
+            if (n > 1) parts = std::max(parts, n * a.rows * p.sums_pitch * 4);
+        }
+    }
+    if (a.grad_weight) {
+        const uint64_t rest = a.vocab % p.piece ? a.vocab % p.piece : piece;
+        for (uint64_t m : {piece, rest}) {
+            const uint32_t n = product_cut(m, a.width, a.rows, size, true).parts;
+            if (n > 1) parts = std::max(parts, n * m * p.sums_pitch * 4);
+        }
+    }
+    p.parts = take(parts > 0, parts);
     p.bytes = at;
     return p;
 }
