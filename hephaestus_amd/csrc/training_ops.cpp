@@ -10,6 +10,8 @@ using namespace hx;
 namespace {
 
 constexpr uint64_t kMost32 = 0x7FFFFFFFull;
+// Columns of the sums over rows: 65535 blocks of 1024 f32 in a grid's second dimension.
+constexpr uint64_t kMostNormGradCols = 65535ull * 1024;
 
 // An operand as the C ABI takes it.
 struct View {
@@ -182,7 +184,7 @@ hx_status plan_norm_grad(hx_dtype dtype, const View &grad_out, const View &x, co
     if (grad_weight.given()) HX_TRY(ops.out(grad_weight, shape[1], 4, "gradient of the norm weight"));
     if (grad_bias.given()) HX_TRY(ops.out(grad_bias, shape[1], 4, "gradient of the norm bias"));
     HX_TRY(ops.apart());
-    if (shape[0] > kMost32 || shape[1] > kMost32)
+    if (shape[0] > kMost32 || shape[1] > kMostNormGradCols)
         return fail(HX_ERR_DISPATCH_FAILED, "norm of shape %s exceeds the grid range", shape_string(*x.layout).c_str());
     LayerNormGradArgs &a = *args;
     a = LayerNormGradArgs{};

@@ -90,6 +90,9 @@ REFUSED = [
     (norm_grad, {"grad_in": view(place(6), N([4, 64], [-64, 1], 192), F)}, DF, "must be the view of gradient past the norm"),
     (norm_grad, {"grad_weight": buffer(place(8) + 64, 64, F)}, DF, "must not overlap"),
     (norm_grad, {"grad_weight": buffer(place(5) + 64, 64, F)}, DF, "must not overlap"),
+    (norm_grad, {k: view(place(i), L([1, 65535 * 1024 + 1]), F) for i, k in enumerate(("grad_out", "x", "grad_in"))} | {
+        "weight": buffer(place(12), 65535 * 1024 + 1, F), "mean": buffer(place(13), 1, F), "rstd": buffer(place(14), 1, F),
+        "residual_grad": None, "grad_weight": None, "grad_bias": None}, DF, "exceeds the grid range"),
     # recurrence
     (scan, {"gate": view(place(0), L([2, 5, 8]), B)}, IC, "recurrence gate must be float32"),
     (scan, {"state_in": view(place(3), L([2, 8]), B)}, IC, "recurrence state must be float32"),
