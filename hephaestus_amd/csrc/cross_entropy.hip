@@ -25,6 +25,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kDepth = 128; // bytes of k a step
 
+__device__ const u32x4 kZeros[1] = {{0, 0, 0, 0}}; // read in place of what lies past an end
+
 // 16 bytes of k of 16 rows of either operand.  Of f32 these are four instructions,
 // each with an element of every lane: k in another order, the same for both.  The
 // fragments' instructions of one element go first: no two in a row add to the same sums.
@@ -46,21 +48,25 @@ __device__ __forceinline__ void mma(const u32x4 (&b)[FN], const u32x4 (&a)[FM], 
             }
 }
 
-// 16 bytes of a row from `k` on, zeros from `end` on.
+// 16 bytes of a row from `k` on, zeros from `end` on: of rows of 16 bytes and more in one
+// load, the last 16 bytes' where it would pass the end.
 __device__ __forceinline__ u32x4 load_bytes(const int8_t *row, uint32_t k, uint32_t end) {
-    if (k + 16 <= end) return *(const u32x4_any *)(row + k);
-    u32x4 v = {0, 0, 0, 0};
-    if (k >= end) return v;
     if (end >= 16) {
-        const u32x4 last = *(const u32x4_any *)(row + end - 16);
-        return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, last) >> (8 * (k + 16 - end)));
+        const uint32_t from = min(k, end - 16), past = min(k - from, 16u);
+        const auto v = __builtin_bit_cast(unsigned __int128, (u32x4)*(const u32x4_any *)(row + from));
+        return past < 16 ? __builtin_bit_cast(u32x4, v >> (8 * past)) : u32x4{0, 0, 0, 0};
     }
+    u32x4 v = {0, 0, 0, 0};
     for (uint32_t i = 0; k + i < end; ++i) v[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
     return v;
 }
 
-// e^x for x of at most about 0, to a rounding or two: with the rest that the product
-// with log2(e) leaves.
+// e^x for x of at most about 0.  The product's rounding leaves a relative error of up to
+// |x|·2^-24: nothing in a sum of such terms, where e^x outweighs it, nor before a
+// rounding to 16 bits.
+__device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+
+// The same to a rounding or two, with the rest that the product with log2(e) leaves.
 __device__ __forceinline__ float exp_of(float x) {
     constexpr float kLog2e = 1.44269502f, kLow = 1.92596299e-8f;
     if (x < -120.0f) return 0.0f;
@@ -167,13 +173,13 @@ template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
     // column at k = 0.  Strides are such that 32 bits hold them.
     const int8_t *base;
     uint32_t from[kLoads];
-    uint32_t stride;
+    uint32_t stride, last;
     __device__ __forceinline__ void open(const Operand &o, uint64_t first, uint64_t end, int wave, int lane) {
         stride = (uint32_t)o.stride;
         base = o.rows + (ACROSS ? first * sizeof(T) : first * (uint64_t)stride);
         // Rows past the end repeat the last one, columns past it the last chunk; they
         // are dropped at the end.
-        const uint32_t last = (uint32_t)min((uint64_t)WIDTH, end - first) - 1;
+        last = (uint32_t)min((uint64_t)WIDTH, end - first) - 1;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
             const uint32_t q = (wave * kLoads + j) * kWave + lane, row = q / kChunks, place = q % kChunks;
@@ -195,20 +201,35 @@ template <typename T, int WIDTH, int THREADS, bool ACROSS> struct Staged {
         for (int j = 0; j < kLoads; ++j)
             __builtin_amdgcn_global_load_lds((const void *)(p + from[j]), (lds_void *)(to + j * 1024), 16, 0, 0);
     }
-    // The last, partial step: zeros past the end of k.
+    // The last, partial step: zeros past the end of k, from a line of them.  Only rows that
+    // end inside a chunk go through registers, few at a time: more would take them from
+    // the sums.
     __device__ __forceinline__ void fetch_rest(int8_t *stage, uint32_t step, uint64_t k, int wave, int lane) const {
-        int8_t *to = stage + wave * (kLoads * 1024) + lane * 16;
-        for (int j = 0; j < kLoads; ++j) {
-            u32x4 v = {0, 0, 0, 0};
-            if constexpr (ACROSS) {
-                const uint32_t row = ((wave * kLoads + j) * kWave + lane) / kChunks;
-                if ((uint64_t)step * (kDepth / sizeof(T)) + row < k) v = *(const u32x4_any *)(at_step(step) + from[j]);
-            } else {
+        int8_t *to = stage + wave * (kLoads * 1024);
+        const int8_t *p = at_step(step);
+        const uint32_t left = (uint32_t)(k - (uint64_t)step * (kDepth / sizeof(T))); // elements
+        if (ACROSS || left * sizeof(T) % 16 == 0) {
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
                 const uint32_t row = ((wave * kLoads + j) * kWave + lane) / kChunks, place = lane % kChunks;
-                const uint32_t at_k = (place ^ (row % 8)) * 16;
-                v = load_bytes(base + (from[j] - at_k), step * kDepth + at_k, (uint32_t)(k * sizeof(T)));
+                const bool is_in = ACROSS ? row < left : (place ^ (row % 8)) * 16 < left * sizeof(T);
+                __builtin_amdgcn_global_load_lds((const void *)(is_in ? p + from[j] : (const int8_t *)kZeros),
+                                                 (lds_void *)(to + j * 1024), 16, 0, 0);
             }
-            *(u32x4 *)(to + j * 1024) = v;
+            return;
+        }
+        constexpr int kTogether = kLoads % 2 ? 1 : 2;
+#pragma unroll 1
+        for (int first = 0; first < kLoads; first += kTogether) {
+            u32x4 v[kTogether];
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) {
+                const uint32_t row = ((wave * kLoads + first + j) * kWave + lane) / kChunks;
+                v[j] = load_bytes(base + min(row, last) * stride, step * kDepth + (lane % kChunks ^ (row % 8)) * 16,
+                                  (uint32_t)(k * sizeof(T)));
+            }
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) *(u32x4 *)(to + (first + j) * 1024 + lane * 16) = v[j];
         }
     }
 
@@ -387,8 +408,18 @@ __global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilo
                                 (float *)lds);
 }
 
+// The place of a target among a lane's columns from `first` on, 4 of every 16; ~0 where it
+// is none of them.
+template <int FN> __device__ __forceinline__ uint32_t place_among(uint64_t target, uint64_t first) {
+    const uint64_t d = target - first;
+    return d < 16 * FN && d % 16 < 4 ? (uint32_t)d : ~0u;
+}
+
 // The largest logit of each row of the tile, the sum of e^(logit - largest), and the
-// target's logit: [tiles of columns][rows].
+// target's logit: [tiles of columns][rows].  A tile of 256 x 256 has 128 logits a lane:
+// what few rows or the last columns alone need stands behind a wave's branch.  1427 x 47616
+// x 169 bf16 took 121 us where each logit was compared with the target and the end, and 93
+// so; it takes 57 with the last step's loads under way together.
 struct TileStats {
     float2 *stats;
     float *picked;
@@ -396,20 +427,35 @@ struct TileStats {
     template <typename C>
     __device__ __forceinline__ void finish(f32x4 (&acc)[C::FM][C::FN], const Place &at, const Product &p, float *lds) {
         float2 *joined = (float2 *)lds; // [WN][BM]
+        if (__any(at.n + 16 * (C::FN - 1) + 4 > p.n)) {
+#pragma unroll
+            for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at.n + 16 * j + e >= p.n) acc[i][j][e] = -__builtin_inff();
+        }
+        uint32_t row_targets[C::FM];
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i) row_targets[i] = targets[min(at.m + 16 * i, p.m - 1)];
 #pragma unroll
         for (int i = 0; i < C::FM; ++i) {
-            const uint64_t row = at.m + 16 * i;
-            const uint64_t target = targets[min(row, p.m - 1)];
+            const uint64_t row = at.m + 16 * i, target = row_targets[i];
+            const uint32_t hit = target < p.n && row < p.m ? place_among<C::FN>(target, at.n) : ~0u;
+            if (__any(hit != ~0u)) {
+                float logit = 0.0f;
+#pragma unroll
+                for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) logit = hit == 16u * j + e ? acc[i][j][e] : logit;
+                if (hit != ~0u) picked[row] = logit;
+            }
             float top = -__builtin_inff();
 #pragma unroll
             for (int j = 0; j < C::FN; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint64_t n = at.n + 16 * j + e;
-                    if (n == target && row < p.m && n < p.n) picked[row] = acc[i][j][e];
-                    if (n >= p.n) acc[i][j][e] = -__builtin_inff();
-                    top = fmaxf(top, acc[i][j][e]);
-                }
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             const float from = top > -__builtin_inff() ? top : 0.0f; // of no logits, or of none above -inf
@@ -417,7 +463,7 @@ struct TileStats {
 #pragma unroll
             for (int j = 0; j < C::FN; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += exp_of(acc[i][j][e] - from);
+                for (int e = 0; e < 4; ++e) sum += exp_near(acc[i][j][e] - from);
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (lane_id() < 16) joined[at.wave_n * C::BM + (int)(row - at.m0)] = float2{top, sum};
@@ -437,22 +483,61 @@ struct TileStats {
     }
 };
 
-// Four columns of a row at the alignment of the elements, those before `end`.
-typedef bf16 bf16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
-template <typename T> __device__ __forceinline__ void store_four(T *p, uint64_t n, uint64_t end, f32x4 v) {
-    if (n + 4 <= end) {
-        if constexpr (sizeof(T) == 4) {
-            *(f32x4_a4 *)p = v;
-        } else {
-            bf16x4_a2 r;
+// COUNT columns of a row at the alignment of the elements, those before `end`.
+template <typename T, int COUNT>
+__device__ __forceinline__ void store_columns(T *p, uint64_t n, uint64_t end, const T (&v)[COUNT]) {
+    typedef T any __attribute__((ext_vector_type(COUNT), aligned(sizeof(T))));
+    if (n + COUNT <= end) {
+        any all;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = (bf16)v[e];
-            *(bf16x4_a2 *)p = r;
-        }
+        for (int e = 0; e < COUNT; ++e) all[e] = v[e];
+        *(any *)p = all;
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < end) p[e] = (T)v[e];
+        for (int e = 0; e < COUNT; ++e)
+            if (n + e < end) p[e] = v[e];
+    }
+}
+
+// A wave's fragments of 16 rows to memory: `row` is this lane's row, from the tile's
+// columns of the wave on, which begin at column `n`.  Of bf16 a lane holds 8 bytes of each 32.
+// Two fragments are exchanged among the four lanes of a row, such that these store 64
+// bytes side by side: the fragments' and the lanes' places are bits that change places.
+// G of 4096 x 16384 x 64 takes 52.5 us with 8 bytes a lane and 42.5 with 16.
+template <typename T, int FN>
+__device__ __forceinline__ void store_fragments(T *row, bool is_in, uint64_t n, uint64_t end, const f32x4 (&v)[FN]) {
+    const int q = lane_id() / 16;
+    if constexpr (sizeof(T) == 4 || FN % 2 != 0) {
+        if (!is_in) return;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int c = 16 * j + 4 * q;
+            const T each[4] = {(T)v[j][0], (T)v[j][1], (T)v[j][2], (T)v[j][3]};
+            store_columns(row + c, n + c, end, each);
+        }
+    } else {
+        const auto pack = [](float a, float b) {
+            typedef bf16 pair __attribute__((ext_vector_type(2)));
+            return __builtin_bit_cast(uint32_t, pair{(bf16)a, (bf16)b});
+        };
+#pragma unroll
+        for (int h = 0; h < FN / 2; ++h) {
+            u32x4 all;
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const uint32_t first = pack(v[2 * h][2 * d], v[2 * h][2 * d + 1]);
+                const uint32_t second = pack(v[2 * h + 1][2 * d], v[2 * h + 1][2 * d + 1]);
+                const auto by_half = __builtin_amdgcn_permlane32_swap(first, second, false, false);
+                const auto by_row = __builtin_amdgcn_permlane16_swap(by_half[0], by_half[1], false, false);
+                all[d] = by_row[0];
+                all[2 + d] = by_row[1];
+            }
+            const int c = 32 * h + 8 * q;
+            struct Each {
+                T v[8];
+            };
+            if (is_in) store_columns(row + c, n + c, end, __builtin_bit_cast(Each, all).v);
+        }
     }
 }
 
@@ -465,24 +550,41 @@ template <typename T> struct TileGradient {
     const float *lse, *grad, *most;
     template <typename C>
     __device__ __forceinline__ void finish(f32x4 (&acc)[C::FM][C::FN], const Place &at, const Product &p, float *) {
+        // What all the rows need is asked for together.
+        uint32_t row_targets[C::FM];
+        float row_lse[C::FM], row_grad[C::FM];
+        const float largest = *most;
 #pragma unroll
         for (int i = 0; i < C::FM; ++i) {
-            const uint64_t row = at.m + 16 * i;
-            if (row >= p.m) continue;
-            const uint64_t target = targets[row];
+            const uint64_t row = min(at.m + 16 * i, p.m - 1);
+            row_targets[i] = targets[row], row_lse[i] = lse[row], row_grad[i] = grad[row];
+        }
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i) {
+            const uint64_t row = at.m + 16 * i, target = row_targets[i];
             const bool counts = target < vocab;
-            const float from = lse[row], weight = counts ? grad[row] / *most : 0.0f;
+            const float from = row_lse[i], weight = counts ? row_grad[i] / largest : 0.0f;
+            const uint32_t hit = place_among<C::FN>(target, first + at.n);
 #pragma unroll
-            for (int j = 0; j < C::FN; ++j) {
-                const uint64_t n = at.n + 16 * j;
-                f32x4 v;
+            for (int j = 0; j < C::FN; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float s = exp_of(acc[i][j][e] - from) - (first + n + e == target ? 1.0f : 0.0f);
-                    v[e] = counts ? s * weight : 0.0f;
-                }
-                store_four(g + row * pitch + n, n, p.n, v);
+                for (int e = 0; e < 4; ++e)
+                    acc[i][j][e] = sizeof(T) == 2 ? exp_near(acc[i][j][e] - from) : exp_of(acc[i][j][e] - from);
+            if (__any(hit != ~0u)) {
+#pragma unroll
+                for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] -= hit == 16u * j + e ? 1.0f : 0.0f;
             }
+#pragma unroll
+            for (int j = 0; j < C::FN; ++j) acc[i][j] *= weight;
+            if (__any(!counts)) { // whatever the logits were
+#pragma unroll
+                for (int j = 0; j < C::FN; ++j)
+                    if (!counts) acc[i][j] = f32x4{0, 0, 0, 0};
+            }
+            const uint64_t n = at.n - lane_id() / 16 * 4;
+            store_fragments(g + row * pitch + n, row < p.m, n, p.n, acc[i]);
         }
     }
 };
@@ -501,47 +603,112 @@ template <typename T> struct TileOut {
     uint64_t vocab;
     template <typename C>
     __device__ __forceinline__ void finish(f32x4 (&acc)[C::FM][C::FN], const Place &at, const Product &p, float *) {
-        const float by = *scale;
+        const float by = scale ? *scale : 1.0f; // parts have none
 #pragma unroll
         for (int i = 0; i < C::FM; ++i) {
             const uint64_t row = at.m + 16 * i;
-            if (row >= p.m) continue;
-            const bool is_left_out = targets && targets[row] >= vocab;
+            const bool is_in = row < p.m;
+            if (before || after) {
 #pragma unroll
-            for (int j = 0; j < C::FN; ++j) {
-                const uint64_t n = at.n + 16 * j;
-                if (n >= p.n) continue;
-                f32x4 v = acc[i][j];
-                if (before) v += *(const f32x4 *)(before + row * sum_pitch + n); // the pitch is whole vectors
-                if (after) {
-                    *(f32x4 *)(after + (blockIdx.y * p.m + row) * sum_pitch + n) = v;
-                } else {
-                    v *= by;
-                    if (is_left_out) v = f32x4{0, 0, 0, 0};
-                    store_four(out + (int64_t)row * out_stride + (int64_t)n, n, p.n, v);
+                for (int j = 0; j < C::FN; ++j) {
+                    const uint64_t n = at.n + 16 * j;
+                    if (!is_in || n >= p.n) continue;
+                    if (before) acc[i][j] += *(const f32x4 *)(before + row * sum_pitch + n); // the pitch is whole vectors
+                    if (after) *(f32x4 *)(after + (blockIdx.y * p.m + row) * sum_pitch + n) = acc[i][j];
                 }
+                if (after) continue;
             }
+            const bool is_left_out = is_in && targets && targets[row] >= vocab;
+#pragma unroll
+            for (int j = 0; j < C::FN; ++j) acc[i][j] = is_left_out ? f32x4{0, 0, 0, 0} : acc[i][j] * by;
+            const uint64_t n = at.n - lane_id() / 16 * 4;
+            store_fragments(out + (int64_t)row * out_stride + (int64_t)n, is_in, n, p.n, acc[i]);
         }
     }
 };
 
-// The parts' sums of four columns of a row, added up in order, and on as TileOut does.
+// The parts' sums of four columns, added up in order, eight asked for at a time.
+__device__ __forceinline__ f32x4 sum_of_parts(const float *at, uint32_t count, uint64_t apart) {
+    f32x4 v = *(const f32x4 *)at;
+    uint32_t p = 1;
+    for (; p + 8 <= count; p += 8) {
+        f32x4 more[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) more[i] = *(const f32x4 *)(at + (p + i) * apart);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += more[i];
+    }
+    for (; p < count; ++p) v += *(const f32x4 *)(at + p * apart);
+    return v;
+}
+
+// A wave's 64 vectors of the result, such that few of them are spread over many CUs.
 template <typename T>
-__global__ __launch_bounds__(256) void fold_parts_kernel(const float *parts, uint32_t count, uint64_t m, uint64_t n,
-                                                        TileOut<T> out) {
+__global__ __launch_bounds__(64) void fold_parts_kernel(const float *parts, uint32_t count, uint64_t m, uint64_t n,
+                                                       TileOut<T> out) {
     const uint64_t vectors = out.sum_pitch / 4;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < m * vectors; i += (uint64_t)gridDim.x * 256) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 64 + threadIdx.x; i < m * vectors; i += (uint64_t)gridDim.x * 64) {
         const uint64_t row = i / vectors, c = i % vectors * 4, at = row * out.sum_pitch + c;
-        f32x4 v = *(const f32x4 *)(parts + at);
-        for (uint32_t p = 1; p < count; ++p) v += *(const f32x4 *)(parts + (uint64_t)p * m * out.sum_pitch + at);
+        f32x4 v = sum_of_parts(parts + at, count, m * out.sum_pitch);
         if (out.before) v += *(const f32x4 *)(out.before + at);
         if (out.after) {
             *(f32x4 *)(out.after + at) = v;
         } else {
             v *= *out.scale;
             if (out.targets && out.targets[row] >= out.vocab) v = f32x4{0, 0, 0, 0};
-            store_four(out.out + (int64_t)row * out.out_stride + (int64_t)c, c, n, v);
+            const T each[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            store_columns(out.out + (int64_t)row * out.out_stride + (int64_t)c, c, n, each);
         }
+    }
+}
+
+// Logits of parts to what TileStats leaves of a tile: 1024 columns of a row, a block.
+__global__ __launch_bounds__(256) void fold_stats_kernel(const float *parts, uint32_t count, uint64_t m, uint64_t n,
+                                                        uint64_t pitch, TileStats out) {
+    __shared__ float2 joined[256 / kWave];
+    const uint64_t row = blockIdx.x, c = ((uint64_t)blockIdx.y * 256 + threadIdx.x) * 4, target = out.targets[row];
+    f32x4 v = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+    if (c < n) {
+        const f32x4 all = sum_of_parts(parts + row * pitch + c, count, m * pitch);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (c + e < n) v[e] = all[e];
+            if (c + e == target && target < n) out.picked[row] = all[e];
+        }
+    }
+    float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float from = top > -__builtin_inff() ? top : 0.0f;
+    float sum = exp_near(v[0] - from) + exp_near(v[1] - from) + exp_near(v[2] - from) + exp_near(v[3] - from);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane_id() == 0) joined[threadIdx.x / kWave] = float2{top, sum};
+    __syncthreads();
+    if (threadIdx.x) return;
+    float2 s = joined[0];
+#pragma unroll
+    for (int w = 1; w < 256 / kWave; ++w) s = TileStats::join(s, joined[w]);
+    out.stats[blockIdx.y * m + row] = s;
+}
+
+// Logits of parts to G, as TileGradient makes it.
+template <typename T>
+__global__ __launch_bounds__(64) void fold_gradient_kernel(const float *parts, uint32_t count, uint64_t m, uint64_t n,
+                                                          uint64_t pitch, TileGradient<T> out) {
+    const uint64_t vectors = pitch / 4;
+    for (uint64_t i = (uint64_t)blockIdx.x * 64 + threadIdx.x; i < m * vectors; i += (uint64_t)gridDim.x * 64) {
+        const uint64_t row = i / vectors, c = i % vectors * 4, target = out.targets[row];
+        const f32x4 v = sum_of_parts(parts + row * pitch + c, count, m * pitch);
+        const bool counts = target < out.vocab;
+        const float from = out.lse[row], weight = counts ? out.grad[row] / *out.most : 0.0f;
+        T each[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float s = exp_of(v[e] - from) - (out.first + c + e == target ? 1.0f : 0.0f);
+            each[e] = (T)(counts ? s * weight : 0.0f);
+        }
+        store_columns(out.g + row * out.pitch + c, c, n, each);
     }
 }
 
@@ -583,31 +750,69 @@ hx_status launch_product(Product p, const ProductCut &cut, const E &epilogue, hi
     }
     return HX_OK;
 }
-// A product to `out`, in parts of k where that is shorter.
+// A product's parts of k, [parts][m][pitch].
+template <typename T, bool ACROSS_A, bool ACROSS_B>
+hx_status launch_parts(const Product &p, const ProductCut &cut, float *parts, uint64_t pitch, hipStream_t stream) {
+    const TileOut<T> part{nullptr, nullptr, parts, nullptr, pitch, 0, nullptr, 0};
+    return launch_product<T, ACROSS_A, ACROSS_B>(p, cut, part, stream);
+}
+inline dim3 fold_blocks(uint64_t m, uint64_t pitch) {
+    return dim3((uint32_t)std::min<uint64_t>(ceil_div(m * (pitch / 4), 64), 1 << 18));
+}
+// A product to `out`, in parts where that is shorter.
 template <typename T, bool ACROSS_A, bool ACROSS_B>
 hx_status launch_sums(const Product &p, const TileOut<T> &out, float *parts, hipStream_t stream) {
-    const ProductCut cut = product_cut(p.m, p.n, p.k, sizeof(T), true);
+    const ProductCut cut = product_cut(p.m, p.n, p.k, sizeof(T));
     if (cut.parts <= 1 || p.m == 0 || p.n == 0) return launch_product<T, ACROSS_A, ACROSS_B>(p, cut, out, stream);
-    TileOut<T> part = out;
-    part.before = nullptr;
-    part.after = parts;
-    HX_TRY((launch_product<T, ACROSS_A, ACROSS_B>)(p, cut, part, stream));
-    const uint64_t blocks = std::min<uint64_t>(ceil_div(p.m * (out.sum_pitch / 4), 256), 1 << 16);
-    hipLaunchKernelGGL(fold_parts_kernel<T>, dim3((uint32_t)blocks), dim3(256), 0, stream, parts, cut.parts, p.m, p.n,
-                       out);
+    HX_TRY((launch_parts<T, ACROSS_A, ACROSS_B>)(p, cut, parts, out.sum_pitch, stream));
+    hipLaunchKernelGGL(fold_parts_kernel<T>, fold_blocks(p.m, out.sum_pitch), dim3(64), 0, stream, parts, cut.parts, p.m,
+                       p.n, out);
     return check_launch("fold_parts_kernel");
 }
 
 // ------------------------------------------------------------------ rows
 
+// The largest finite |grad| of a row that has a target; 1 where there is none.
+struct Largest {
+    const float *grad;
+    const uint32_t *targets;
+    uint64_t rows, vocab;
+    float *most; // null: not asked for
+    __device__ void find() const {
+        constexpr int kEach = 8;
+        float top = 0.0f;
+        for (uint64_t first = threadIdx.x; first < rows; first += 256 * kEach) {
+            float g[kEach];
+            uint32_t target[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const uint64_t r = min(first + i * 256, rows - 1);
+                g[i] = fabsf(grad[r]), target[i] = targets[r];
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (target[i] < vocab && g[i] < __builtin_inff()) top = fmaxf(top, g[i]);
+        }
+        __shared__ float tops[256 / kWave];
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        if (lane_id() == 0) tops[threadIdx.x / kWave] = top;
+        __syncthreads();
+        if (threadIdx.x) return;
+        for (int i = 1; i < 256 / kWave; ++i) top = fmaxf(top, tops[i]);
+        *most = top > 0.0f ? top : 1.0f;
+    }
+};
+
 // Rows at any byte, copied to rows of whole steps with zeros after their ends, and
 // zeros in the place of rows that have no target where `targets` is given: whatever such a
-// row holds, it adds nothing.
+// row holds, it adds nothing.  A last block looks for the largest gradient meanwhile.
 __global__ __launch_bounds__(256) void copy_rows_kernel(const int8_t *from, int64_t stride, uint64_t rows, uint32_t bytes,
                                                        int8_t *to, uint32_t pitch, const uint32_t *targets,
-                                                       uint64_t vocab) {
-    const uint32_t chunks = pitch / 16;
-    for (uint64_t first = (uint64_t)blockIdx.x * 256; first < rows * chunks; first += (uint64_t)gridDim.x * 256) {
+                                                       uint64_t vocab, Largest largest) {
+    const uint32_t chunks = pitch / 16, blocks = gridDim.x - (largest.most ? 1 : 0);
+    if (blockIdx.x == blocks) return largest.find();
+    for (uint64_t first = (uint64_t)blockIdx.x * 256; first < rows * chunks; first += (uint64_t)blocks * 256) {
         const uint32_t i = (uint32_t)(first % chunks) + threadIdx.x, at = i % chunks * 16;
         const uint64_t r = first / chunks + i / chunks;
         if (r >= rows) return;
@@ -644,32 +849,14 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const float2 *stats, co
     loss[row] = targets[row] < vocab ? l - picked[row] : 0.0f;
 }
 
-// The largest finite |grad| of a row that has a target; 1 where there is none.
-__global__ __launch_bounds__(1024) void most_kernel(const float *grad, const uint32_t *targets, uint64_t rows,
-                                                    uint64_t vocab, float *most) {
-    float top = 0.0f;
-    for (uint64_t r = threadIdx.x; r < rows; r += 1024) {
-        const float g = fabsf(grad[r]);
-        if (targets[r] < vocab && g < __builtin_inff()) top = fmaxf(top, g);
-    }
-    __shared__ float tops[16];
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane_id() == 0) tops[threadIdx.x / kWave] = top;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, tops[i]);
-    *most = top > 0.0f ? top : 1.0f;
-}
-
 template <typename T>
 hx_status copy_rows(const void *from, int64_t stride, uint64_t rows, uint64_t width, void *to, const uint32_t *targets,
-                    uint64_t vocab, hipStream_t stream) {
+                    uint64_t vocab, const Largest &largest, hipStream_t stream) {
     const uint32_t bytes = (uint32_t)(width * sizeof(T)), pitch = (uint32_t)round_up(bytes, kDepth);
-    if (rows == 0 || pitch == 0) return HX_OK;
-    const uint64_t blocks = std::min<uint64_t>(ceil_div(rows * (pitch / 16), 256), 1 << 22);
+    const uint64_t blocks = std::min<uint64_t>(ceil_div(rows * (pitch / 16), 256), 1 << 22) + (largest.most ? 1 : 0);
+    if (blocks == 0) return HX_OK;
     hipLaunchKernelGGL(copy_rows_kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, (const int8_t *)from,
-                       stride * (int64_t)sizeof(T), rows, bytes, (int8_t *)to, pitch, targets, vocab);
+                       stride * (int64_t)sizeof(T), rows, bytes, (int8_t *)to, pitch, targets, vocab, largest);
     return check_launch("copy_rows_kernel");
 }
 
@@ -682,12 +869,23 @@ template <typename T> hx_status launch(const CrossEntropyArgs &a, void *ws, hipS
     Product p{{(const int8_t *)a.x, a.x_stride * size}, {(const int8_t *)a.weight, a.weight_stride * size}, a.rows,
               a.vocab, a.width, 0};
     if (plan.copies) {
-        HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, nullptr, 0, stream));
-        HX_TRY(copy_rows<T>(a.weight, a.weight_stride, a.vocab, a.width, base + plan.weight, nullptr, 0, stream));
+        HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, nullptr, 0, {}, stream));
+        HX_TRY(copy_rows<T>(a.weight, a.weight_stride, a.vocab, a.width, base + plan.weight, nullptr, 0, {}, stream));
+        p.k = row / size; // zeros after the rows' ends
         p.a = {(const int8_t *)base + plan.x, row};
         p.b = {(const int8_t *)base + plan.weight, row};
     }
-    HX_TRY((launch_product<T, false, false>)(p, plan.cut, TileStats{stats, picked, a.targets}, stream));
+    const TileStats out{stats, picked, a.targets};
+    if (plan.cut.parts > 1) {
+        float *parts = (float *)(base + plan.parts);
+        const uint64_t pitch = round_up(a.vocab, 4);
+        HX_TRY((launch_parts<T, false, false>)(p, plan.cut, parts, pitch, stream));
+        hipLaunchKernelGGL(fold_stats_kernel, dim3((uint32_t)a.rows, (uint32_t)plan.tiles_n), dim3(256), 0, stream, parts,
+                           plan.cut.parts, a.rows, a.vocab, pitch, out);
+        HX_TRY(check_launch("fold_stats_kernel"));
+    } else {
+        HX_TRY((launch_product<T, false, false>)(p, plan.cut, out, stream));
+    }
     const uint64_t tiles = a.vocab ? plan.tiles_n : 0;
     if (a.rows >= 2048)
         hipLaunchKernelGGL(join_stats_kernel<16>, dim3((uint32_t)ceil_div(a.rows, 16)), dim3(256), 0, stream, stats,
@@ -702,11 +900,10 @@ template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, 
     const CrossEntropyGradPlan plan = cross_entropy_grad_plan(a);
     char *base = (char *)ws;
     float *most = (float *)base;
-    hipLaunchKernelGGL(most_kernel, dim3(1), dim3(1024), 0, stream, a.grad, a.targets, a.rows, a.vocab, most);
-    HX_TRY(check_launch("most_kernel"));
     const int64_t size = sizeof(T), row = (int64_t)round_up(a.width * size, kDepth);
     const Operand x{(const int8_t *)base + plan.x, row};
-    HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, a.targets, a.vocab, stream));
+    HX_TRY(copy_rows<T>(a.x, a.x_stride, a.rows, a.width, base + plan.x, a.targets, a.vocab,
+                        Largest{a.grad, a.targets, a.rows, a.vocab, most}, stream));
     float *sums = (float *)(base + plan.sums), *parts = (float *)(base + plan.parts);
     T *g = (T *)(base + plan.g);
     const Operand go{(const int8_t *)g, (int64_t)plan.piece_pitch * size};
@@ -715,14 +912,21 @@ template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, 
         const T *from = (const T *)a.weight + (int64_t)first * a.weight_stride;
         Operand w{(const int8_t *)from, a.weight_stride * size};
         if (plan.copies) {
-            HX_TRY(copy_rows<T>(from, a.weight_stride, n, a.width, base + plan.weight, nullptr, 0, stream));
+            HX_TRY(copy_rows<T>(from, a.weight_stride, n, a.width, base + plan.weight, nullptr, 0, {}, stream));
             w = {(const int8_t *)base + plan.weight, row};
         }
-        HX_TRY((launch_product<T, false, false>)(Product{x, w, a.rows, n, a.width, 0},
-                                                 product_cut(a.rows, n, a.width, sizeof(T), false),
-                                                 TileGradient<T>{g, plan.piece_pitch, first, a.vocab, a.targets, a.lse,
-                                                                 a.grad, most},
-                                                 stream));
+        const Product logits{x, w, a.rows, n, plan.copies ? row / size : a.width, 0};
+        const TileGradient<T> to{g, plan.piece_pitch, first, a.vocab, a.targets, a.lse, a.grad, most};
+        const ProductCut cut = product_cut(a.rows, n, a.width, size);
+        if (cut.parts > 1 && n > 0) {
+            const uint64_t pitch = round_up(n, 4);
+            HX_TRY((launch_parts<T, false, false>)(logits, cut, parts, pitch, stream));
+            hipLaunchKernelGGL(fold_gradient_kernel<T>, fold_blocks(a.rows, pitch), dim3(64), 0, stream, parts, cut.parts,
+                               a.rows, n, pitch, to);
+            HX_TRY(check_launch("fold_gradient_kernel"));
+        } else {
+            HX_TRY((launch_product<T, false, false>)(logits, cut, to, stream));
+        }
         if (a.grad_x) {
             const bool is_last = first + n >= a.vocab;
             const TileOut<T> out{most, first ? sums : nullptr, is_last ? nullptr : sums, (T *)a.grad_x, plan.sums_pitch,

@@ -167,14 +167,18 @@ enum class ProductTile : uint32_t { k256x256, k128x128, k64x128, k64x64, k32x64 
 struct ProductTileRule {
     uint64_t m, n;
     uint64_t at_once; // blocks that share a CU
+    // us that a round of blocks takes besides its steps: to its first step, and for what
+    // becomes of the sums, which at 256 x 256 no other block's steps hide.
+    double ends;
     // us for a step of 128 bytes of k with one block on each CU, and with all that share
     // it: of bf16, as measured on products of 256 x 4096 x 4096 to 2048 x 8192 x 2048, by rows
     // and across; of f32, where the matrix instructions bound all of them.
     double one, all, one_f32, all_f32;
 };
 constexpr ProductTileRule kProductTiles[] = {
-    {256, 256, 1, 1.70, 1.70, 7.60, 7.60}, {128, 128, 1, 0.56, 0.56, 2.00, 2.00}, {64, 128, 2, 0.34, 0.60, 1.08, 2.10},
-    {64, 64, 2, 0.30, 0.44, 0.60, 1.06},   {32, 64, 2, 0.23, 0.31, 0.33, 0.58}};
+    {256, 256, 1, 7.5, 1.70, 1.70, 7.60, 7.60}, {128, 128, 1, 3.4, 0.56, 0.56, 2.00, 2.00},
+    {64, 128, 2, 2.9, 0.34, 0.60, 1.08, 2.10},  {64, 64, 2, 2.1, 0.30, 0.44, 0.60, 1.06},
+    {32, 64, 2, 1.9, 0.23, 0.31, 0.33, 0.58}};
 
 // How a product is cut: into tiles, and along k into parts whose sums are added up by a
 // launch of their own.
@@ -189,7 +193,9 @@ struct ProductCut {
 //   2048 x 8192 x 2048 bf16  256 x 256 59.9   128 x 128 77.0   64 x 128 83.6
 //   256 x 4096 x 4096 bf16    64 x 64 20.4     64 x 128 25.9   128 x 128 34.7
 //   1000 x 5008 x 1040 f32    64 x 64 100.6   128 x 128 145
-inline ProductCut product_cut(uint64_t m, uint64_t n, uint64_t k, uint64_t size, bool may_split) {
+//   32 x 51200 x 64 bf16      64 x 128 5.4    128 x 128 8.8    256 x 256 9.3     64 x 64 6.7
+//   4096 x 16384 x 64 bf16   256 x 256 33.4   64 x 128 53.9    128 x 128 62.2    64 x 64 79.3
+inline ProductCut product_cut(uint64_t m, uint64_t n, uint64_t k, uint64_t size) {
     constexpr uint64_t kCus = 256;
     const uint64_t step = 128 / size, steps = std::max<uint64_t>(1, ceil_div(k, step));
     ProductCut best{ProductTile::k32x64, 1, steps * step};
@@ -198,10 +204,10 @@ inline ProductCut product_cut(uint64_t m, uint64_t n, uint64_t k, uint64_t size,
         const ProductTileRule &r = kProductTiles[t];
         const double one = size == 4 ? r.one_f32 : r.one, all = size == 4 ? r.all_f32 : r.all;
         const uint64_t tiles = ceil_div(m, r.m) * ceil_div(n, r.n);
-        for (uint64_t parts = 1; parts <= (may_split ? 32 : 1) && (parts == 1 || steps / parts >= 4); parts *= 2) {
+        for (uint64_t parts = 1; parts <= 32 && (parts == 1 || steps / parts >= 4); parts *= 2) {
             const uint64_t blocks = tiles * parts, full = blocks / (kCus * r.at_once), rest = blocks % (kCus * r.at_once);
             const double rounds = full * all + (rest == 0 ? 0.0 : rest <= kCus ? one : all);
-            double us = rounds * ceil_div(steps, parts) + 2.0 * (full + 1);
+            double us = rounds * ceil_div(steps, parts) + r.ends * (full + (rest > 0)) + 2.0;
             if (parts > 1) us += 4.0 + (double)(m * n * parts) * 8 / 5e6;
             if (best_us == 0.0 || us < best_us) {
                 best_us = us;
@@ -235,17 +241,18 @@ inline bool cross_entropy_copies(const CrossEntropyGradArgs &a) {
 struct CrossEntropyPlan {
     bool copies;
     ProductCut cut;
-    uint64_t tiles_n, stats, picked, x, weight, bytes;
+    uint64_t tiles_n, stats, picked, parts, x, weight, bytes;
 };
 inline CrossEntropyPlan cross_entropy_plan(const CrossEntropyArgs &a) {
     CrossEntropyPlan p{};
     const uint64_t row = round_up(a.width * element_size(a.dtype), 128);
     p.copies = cross_entropy_copies(a);
-    p.cut = product_cut(a.rows, a.vocab, a.width, element_size(a.dtype), false);
-    p.tiles_n = ceil_div(a.vocab, kProductTiles[(uint32_t)p.cut.tile].n);
+    p.cut = product_cut(a.rows, a.vocab, a.width, element_size(a.dtype));
+    p.tiles_n = ceil_div(a.vocab, p.cut.parts > 1 ? 1024 : kProductTiles[(uint32_t)p.cut.tile].n);
     p.stats = 0;
     p.picked = round_up(p.tiles_n * a.rows * 8, 256);
-    p.x = round_up(p.picked + a.rows * 4, 256);
+    p.parts = round_up(p.picked + a.rows * 4, 256);
+    p.x = round_up(p.parts + (p.cut.parts > 1 ? p.cut.parts * a.rows * round_up(a.vocab, 4) * 4 : 0), 256);
     p.weight = p.x + (p.copies ? a.rows * row : 0);
     p.bytes = p.weight + (p.copies ? a.vocab * row : 0);
     return p;
@@ -277,22 +284,17 @@ inline CrossEntropyGradPlan cross_entropy_grad_plan(const CrossEntropyGradArgs &
     p.weight = take(p.copies, p.piece * row);
     p.g = take(true, a.rows * p.piece_pitch * size);
     p.sums = take(a.grad_x && p.piece < a.vocab, a.rows * p.sums_pitch * 4);
-    // Sums of parts of k, of grad_x or of a piece of grad_weight.
-    const uint64_t piece = std::min(p.piece, a.vocab);
+    // Sums of parts of k: of a piece's logits, of grad_x, or of a piece of grad_weight.
     uint64_t parts = 0;
-    if (a.grad_x) {
-        const uint64_t rest = a.vocab % p.piece ? a.vocab % p.piece : piece; // the last piece's cut may differ
-        for (uint64_t k : {piece, rest}) {
-            const uint32_t n = product_cut(a.rows, a.width, k, size, true).parts;
-            if (n > 1) parts = std::max(parts, n * a.rows * p.sums_pitch * 4);
-        }
-    }
-    if (a.grad_weight) {
-        const uint64_t rest = a.vocab % p.piece ? a.vocab % p.piece : piece;
-        for (uint64_t m : {piece, rest}) {
-            const uint32_t n = product_cut(m, a.width, a.rows, size, true).parts;
-            if (n > 1) parts = std::max(parts, n * m * p.sums_pitch * 4);
-        }
+    const auto fold = [&](uint64_t m, uint64_t n, uint64_t k, uint64_t pitch) {
+        const uint32_t count = product_cut(m, n, k, size).parts;
+        if (count > 1) parts = std::max(parts, count * m * pitch * 4);
+    };
+    const uint64_t piece = std::min(p.piece, a.vocab);
+    for (uint64_t words : {piece, a.vocab % p.piece ? a.vocab % p.piece : piece}) { // the last piece's cut may differ
+        fold(a.rows, words, a.width, round_up(words, 4));
+        if (a.grad_x) fold(a.rows, a.width, words, p.sums_pitch);
+        if (a.grad_weight) fold(words, a.width, a.rows, p.sums_pitch);
     }
     p.parts = take(parts > 0, parts);
     p.bytes = at;

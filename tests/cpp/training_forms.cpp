@@ -33,8 +33,8 @@ void recurrence_form(int32_t f32, int32_t is_backward, uint64_t batch, uint64_t 
 }
 
 // [tile, parts] of a product.
-void product_form(uint64_t m, uint64_t n, uint64_t k, uint64_t size, int32_t may_split, uint64_t *form) {
-    const ProductCut cut = product_cut(m, n, k, size, may_split);
+void product_form(uint64_t m, uint64_t n, uint64_t k, uint64_t size, uint64_t *form) {
+    const ProductCut cut = product_cut(m, n, k, size);
     form[0] = (uint64_t)cut.tile;
     form[1] = cut.parts;
     form[2] = cut.span;

@@ -26,7 +26,7 @@ def rules(tmp_path_factory):
     lib = ctypes.CDLL(str(path))
     lib.norm_row.argtypes = [U64, U64]
     lib.recurrence_form.argtypes = [I32, I32, U64, U64, U64, U64, ctypes.POINTER(ctypes.c_uint32)]
-    lib.product_form.argtypes = [U64, U64, U64, U64, I32, ctypes.POINTER(U64)]
+    lib.product_form.argtypes = [U64, U64, U64, U64, ctypes.POINTER(U64)]
     lib.copies.argtypes = [U64, U64, I64, U64]
     lib.gradient_pieces.argtypes = [U64, U64, U64, U64, ctypes.POINTER(U64)]
     return lib
@@ -36,9 +36,9 @@ def names(enum):
     return re.findall(r"k\w+", re.search(rf"enum class {enum}[^{{]*\{{(.*?)\}}", FORMS.read_text(), re.S)[1])
 
 
-def product(rules, m, n, k, size, may_split):
+def product(rules, m, n, k, size):
     form = (U64 * 3)()
-    rules.product_form(m, n, k, size, may_split, form)
+    rules.product_form(m, n, k, size, form)
     return list(form)
 
 
@@ -54,20 +54,18 @@ def test_every_tile_of_products_is_reached(rules):
         assert list(by_tile) == tiles
         for place, tile in enumerate(tiles):
             for size in by_tile[tile]:
-                for may_split in (0, 1):
-                    assert product(rules, *size, SIZE[dtype], may_split)[:2] == [place, 1], (dtype, tile, size)
+                assert product(rules, *size, SIZE[dtype])[:2] == [place, 1], (dtype, tile, size)
         for tile, sizes in forms.PARTS[dtype].items():
             for size in sizes:
-                got = product(rules, *size, SIZE[dtype], 1)
+                got = product(rules, *size, SIZE[dtype])
                 assert got[0] == tiles.index(tile) and got[1] > 1, (dtype, tile, size, got)
-                assert product(rules, *size, SIZE[dtype], 0)[1] == 1
 
 
 def test_parts_of_products_hold_all_of_k(rules):
     for m, n in ((1, 1), (16, 2048), (300, 300), (8192, 4096)):
         for k in (0, 1, 63, 64, 1000, 32000, 130001):
             for size in (2, 4):
-                _, parts, span = product(rules, m, n, k, size, 1)
+                _, parts, span = product(rules, m, n, k, size)
                 assert span % (128 // size) == 0 and parts * span >= k and (parts - 1) * span < max(1, k), (m, n, k)
 
 
