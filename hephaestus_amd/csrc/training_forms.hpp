@@ -141,6 +141,13 @@ enum class RecurrenceTile : uint32_t { kOne, kFew, kMany, kLong };
 //   4 x 2000 x 1600 bf16, 52 blocks    8 parts of 64-token tiles 39, of 128 46   4 parts 56
 //   1 x 65536 x 2048, backward, 16     32 parts 477   64 parts 500   16 parts 497
 //   8 x 4096 x 4096, backward, 256     one part 320   two parts 463
+// A part may be a single tile: a block's own loads and join take longer than to follow
+// the maps of the parts in front of it.
+//   1 x 4406 x 96 bf16, backward       a tile each 23   two 30   four 41   one part 281
+//   6 x 1961 x 112 f32                 a tile each 16   two 18   four 25   one part 60
+//   1 x 300 x 64 bf16                  a tile each 10   two 19   one part 16
+//   2 x 130 x 512 bf16                 a tile each 9.8  one part 10.6
+//   1 x 65536 x 256 f32, 4 blocks      512 blocks 66    256 72   1024 80
 struct RecurrenceParts {
     RecurrenceTile tile;
     uint32_t parts, span;
@@ -151,11 +158,11 @@ template <typename Args> RecurrenceParts recurrence_parts(const Args &a, uint64_
     if (a.tokens <= 1) return {RecurrenceTile::kOne, 1, (uint32_t)all};
     if (a.tokens <= 32) return {RecurrenceTile::kFew, 1, (uint32_t)all};
     const uint64_t blocks = a.batch * ceil_div(a.channels, 64 * vector), tiles = ceil_div(all, 64);
-    if (blocks >= 160 || tiles < 4) {
+    if (blocks >= 160 || tiles < 3) {
         const bool is_long = !is_backward && all > 64;
         return {is_long ? RecurrenceTile::kLong : RecurrenceTile::kMany, 1, (uint32_t)round_up(all, 64)};
     }
-    const uint64_t parts = std::min<uint64_t>(512 / std::max<uint64_t>(1, blocks), tiles / 2);
+    const uint64_t parts = std::min<uint64_t>(512 / std::max<uint64_t>(1, blocks), tiles);
     const uint64_t span = ceil_div(tiles, parts) * 64;
     return {RecurrenceTile::kMany, (uint32_t)ceil_div(all, span), (uint32_t)span};
 }
