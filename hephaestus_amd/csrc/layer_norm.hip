@@ -299,6 +299,19 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void layer_norm_fold_kernel(cons
     out[c] = sum;
 }
 
+template <int N> __device__ __forceinline__ void store_sums(float *p, uint32_t c, uint32_t cols, const float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        if (c + i + 4 <= cols) {
+            *(f32x4_a4 *)(p + c + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + i + e < cols) p[c + i + e] = x[i + e];
+        }
+    }
+}
+
 // Block b goes through the rows of its run, `LANES` threads a row as forward.
 template <typename T, int LANES, int STEPS>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_kernel(LayerNormGradArgs a,
@@ -308,30 +321,43 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
     const uint32_t cols = (uint32_t)a.cols, lane = kRows > 1 ? threadIdx.x % LANES : threadIdx.x;
     const uint32_t group = kRows > 1 ? threadIdx.x / LANES : 0;
     const uint64_t first = (uint64_t)blockIdx.x * rows_a_block, end = min(a.rows, first + rows_a_block);
+    // Rows of 4 vectors a thread leave no registers for the weight, which lies in LDS, nor to
+    // fetch the gradient past the norm ahead: it is asked for while its own row is summed.
+    // 2282 x 14976 bf16 takes 81 us so, 159 where registers spilled.
+    constexpr bool kAhead = STEPS < 4;
+    __shared__ u32x4 weights[kAhead ? 1 : STEPS][LANES];
     u32x4 vw[STEPS];
     float dw[STEPS][N] = {}, db[STEPS][N] = {};
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const uint32_t c = ((uint32_t)s * LANES + lane) * N;
         vw[s] = place_part<T>(load_part((const T *)a.weight, c, cols), c, cols);
+        if constexpr (!kAhead) weights[s][lane] = vw[s]; // read by this lane alone
     }
+    const auto weight = [&](int s) { return kAhead ? vw[s] : weights[s][lane]; };
     typename SumsOf<LANES>::type sums;
     struct Row {
-        u32x4 x[STEPS], dy[STEPS], past[STEPS];
+        u32x4 x[STEPS], dy[STEPS], past[kAhead ? STEPS : 1];
         float mean, rstd;
     } now, next;
+    const auto fetch_past = [&](uint64_t row, u32x4 *past) {
+        const T *p = (const T *)a.residual_grad + (int64_t)row * a.residual_grad_stride;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            past[s] = u32x4{0, 0, 0, 0};
+            if (a.residual_grad) past[s] = load_part(p, ((uint32_t)s * LANES + lane) * N, cols);
+        }
+    };
     const auto fetch = [&](uint64_t row, Row &r) {
         const T *x = (const T *)a.x + (int64_t)row * a.x_stride;
         const T *dy = (const T *)a.grad_out + (int64_t)row * a.grad_out_stride;
-        const T *past = (const T *)a.residual_grad + (int64_t)row * a.residual_grad_stride;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const uint32_t c = ((uint32_t)s * LANES + lane) * N;
             r.x[s] = load_part(x, c, cols);
             r.dy[s] = load_part(dy, c, cols);
-            r.past[s] = u32x4{0, 0, 0, 0};
-            if (a.residual_grad) r.past[s] = load_part(past, c, cols);
         }
+        if constexpr (kAhead) fetch_past(row, r.past);
         r.mean = a.mean[row];
         r.rstd = a.rstd[row];
     };
@@ -339,7 +365,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
     if (first + group < end) fetch(first + group, now);
     for (uint64_t row = first + group; row < end; row += kRows, now = next) {
         if (row + kRows < end) fetch(row + kRows, next);
-        u32x4(&vx)[STEPS] = now.x, (&vy)[STEPS] = now.dy, (&vp)[STEPS] = now.past;
+        u32x4(&vx)[STEPS] = now.x, (&vy)[STEPS] = now.dy, late[STEPS], *vp = kAhead ? now.past : late;
         const float mean = now.mean, rstd = now.rstd;
         float st = 0.0f, stu = 0.0f;
 #pragma unroll
@@ -350,7 +376,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
             float h[N], g[N], w[N];
             unpack<T>(vx[s], h);
             unpack<T>(vy[s], g);
-            unpack<T>(vw[s], w);
+            unpack<T>(weight(s), w);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float u = (h[i] - mean) * rstd, t = g[i] * w[i];
@@ -360,6 +386,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
                 db[s][i] += g[i];
             }
         }
+        if constexpr (!kAhead) fetch_past(row, late);
         sums(st, stu);
         const float mt = st / cols, mtu = stu / cols;
         T *out = (T *)a.grad_in + (int64_t)row * a.grad_in_stride;
@@ -370,7 +397,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
             float h[N], g[N], w[N], p[N];
             unpack<T>(vx[s], h);
             unpack<T>(vy[s], g);
-            unpack<T>(vw[s], w);
+            unpack<T>(weight(s), w);
             unpack<T>(place_part<T>(vp[s], c, cols), p);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -403,14 +430,11 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_grad_ker
         }
     } else {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const uint32_t c = ((uint32_t)s * LANES + lane) * N + i;
-                if (c >= cols) continue;
-                mine[c] = dw[s][i];
-                mine[cols + c] = db[s][i];
-            }
+        for (int s = 0; s < STEPS; ++s) {
+            const uint32_t c = ((uint32_t)s * LANES + lane) * N;
+            store_sums(mine, c, cols, dw[s]);
+            store_sums(mine + cols, c, cols, db[s]);
+        }
     }
 }
 
@@ -486,12 +510,8 @@ __global__ __launch_bounds__(256) void layer_norm_grad_columns_kernel(LayerNormG
         }
     }
     float *mine = partial + (uint64_t)blockIdx.x * 2 * cols;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (c + i >= cols) break;
-        mine[c + i] = dw[i];
-        mine[cols + c + i] = db[i];
-    }
+    store_sums(mine, c, cols, dw);
+    store_sums(mine + cols, c, cols, db);
 }
 
 template <typename T> hx_status launch(const LayerNormGradArgs &a, void *ws, hipStream_t stream) {
