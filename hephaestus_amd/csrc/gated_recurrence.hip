@@ -13,6 +13,11 @@
 // the tokens are cut into parts: a first launch takes the parts' maps, which
 // every block of the second one follows up to its own part.  All sums have one
 // order: every run gives the same bits.
+//
+// Memory bounds the long ones: 8 x 4096 x 4096 bf16 takes 171 us (4.7 TB/s), 1 x 65536 x
+// 2048 backward 468 us, of which 160 take the parts' maps, so that the gate and dy are read
+// twice (4.6 TB/s of both launches' bytes).  A token of 64 x 4096 takes 3.7 us, a launch and a
+// wait.  Short ones in parts are two launches and their waits: 1 x 4406 x 96 backward 23 us.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 

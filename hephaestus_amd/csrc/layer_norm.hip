@@ -12,6 +12,12 @@
 //   dw = Σ dy·u,  db = Σ dy   over the rows.
 // A block goes through rows and keeps its share of dw and db in registers; the
 // blocks' shares are added up by a second launch, in one order.
+//
+// Memory bounds both: 16384 x 8192 bf16 with a residual takes 191 us forward (5.6 TB/s
+// of x, residual, h and out) and 210 us backward (5.1 TB/s and the sums' launch of 6 us),
+// where torch's copy of 1 GiB reaches 5.2 TB/s.  A single row of 4096 takes 3.3 us, a launch
+// and one wait for memory; 1000 x 5001 f32 takes 24 us backward, 250 blocks of 4 rows whose
+// loads lie off the 128-byte grid, and 6 us of the sums.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 

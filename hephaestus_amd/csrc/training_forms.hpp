@@ -98,10 +98,11 @@ inline NormRow layer_norm_row(uint64_t cols, uint64_t size) {
 // The backward pass: runs of rows, a block each, in whole rounds of the 256 CUs where
 // the rows allow.  Blocks of few waves need more of them side by side.  Measured (us, with
 // the launch that adds up the blocks' sums):
-//   16384 x 8192 bf16  256 blocks 212   382 blocks 262   512 blocks 224   1024 blocks 263
-//   16384 x 2048 bf16  256 blocks 76    512 blocks 52    1024 blocks 53   2048 blocks 72
-//   16384 x 1024 bf16  256 blocks 29    512 blocks 26    1024 blocks 31
-//   1000 x 5001 f32    250 blocks 20    500 blocks 32    1000 blocks 50
+//   16384 x 8192 bf16  256 blocks 167   382 blocks 216   512 blocks 180   1024 blocks 200
+//   16384 x 2048 bf16  256 blocks 76    512 blocks 51    1024 blocks 52   2048 blocks 71
+//   16384 x 1024 bf16  256 blocks 33    512 blocks 32    1024 blocks 43
+//   2282 x 14976 bf16  256 blocks 56    512 blocks 71
+//   1000 x 5001 f32    250 blocks 24    500 blocks 33    1000 blocks 44
 struct NormGradSplit {
     uint32_t blocks, rows_a_block;
 };

@@ -666,7 +666,7 @@ hx_status hx_prepare_layer_norm(
  * residual_grad (may be NULL) is the gradient that reaches h past the norm.
  * grad_in is the gradient of x and of residual alike, and may be the very view
  * of grad_out or of residual_grad.  grad_weight and grad_bias are f32[cols],
- * overwritten; each may be NULL. */
+ * overwritten; each may be NULL.  At most 65535 * 1024 columns. */
 hx_status hx_layer_norm_backward(
     hx_device *dev, hx_dtype dtype, const void *grad_out,
     uint64_t grad_out_buf_len, const hx_layout *grad_out_layout, const void *x,
