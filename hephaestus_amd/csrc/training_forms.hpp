@@ -96,12 +96,16 @@ inline NormRow layer_norm_row(uint64_t cols, uint64_t size) {
 }
 
 // The backward pass: runs of rows, a block each, in whole rounds of the 256 CUs where
-// the rows allow.  Blocks of few waves need more of them side by side.  Measured (us, with
+// the rows allow.  Blocks of few waves need more of them side by side, and so do those
+// of eight waves whose f32 rows leave registers for three on a CU.  Measured (us, with
 // the launch that adds up the blocks' sums):
 //   16384 x 8192 bf16  256 blocks 167   382 blocks 216   512 blocks 180   1024 blocks 200
 //   16384 x 2048 bf16  256 blocks 76    512 blocks 51    1024 blocks 52   2048 blocks 71
 //   16384 x 1024 bf16  256 blocks 33    512 blocks 32    1024 blocks 43
 //   2282 x 14976 bf16  256 blocks 56    512 blocks 71
+//   16384 x 4096 bf16  256 blocks 110   384 blocks 126   512 blocks 119   1024 blocks 137
+//   9971 x 1268 f32    256 blocks 68    384 blocks 56    512 blocks 49    1024 blocks 59
+//   8192 x 2048 f32    256 blocks 70    384 blocks 68    512 blocks 57    1024 blocks 70
 //   1000 x 5001 f32    250 blocks 24    500 blocks 33    1000 blocks 44
 struct NormGradSplit {
     uint32_t blocks, rows_a_block;
@@ -109,7 +113,7 @@ struct NormGradSplit {
 inline NormGradSplit layer_norm_grad_split(const LayerNormGradArgs &a) {
     const uint64_t vectors = ceil_div(a.cols, 16 / element_size(a.dtype));
     const uint64_t at_once = vectors <= 16 ? 16 : vectors <= 128 ? 4 : 1; // rows of a block
-    const uint64_t most = vectors <= 256 ? 512 : 256;
+    const uint64_t most = vectors <= (a.dtype == HX_DTYPE_F32 ? 512 : 256) ? 512 : 256;
     const uint64_t rows = std::max<uint64_t>(at_once, round_up(ceil_div(a.rows, most), at_once));
     return {(uint32_t)std::max<uint64_t>(1, ceil_div(a.rows, rows)), (uint32_t)rows};
 }
