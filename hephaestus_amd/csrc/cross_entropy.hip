@@ -3,7 +3,8 @@
 //
 // Forward: the product goes tile by tile; a tile leaves, for each of its rows, the
 // largest logit and the sum of the exponentials of the others' distances from it, and
-// the target's logit where it lies in the tile.  A second launch joins the tiles.
+// the target's logit where it lies in the tile.  A second launch joins the tiles.  Of few
+// tiles the logits are summed in parts of the width, in scratch, and then taken row by row.
 //
 // Backward, a piece of the vocabulary after another: the logits again, as
 //   G = (grad / most)·(e^(logit - lse) - [target]),   most = max |grad|,
