@@ -41,10 +41,13 @@ class Operands {
     hx_status out(const Vector &v, uint64_t want, uint32_t size, const char *what) {
         return vector(v, want, size, true, what);
     }
-    // An output that may be the very view of an input.
-    void may_be(const View &out, const View &in) {
-        same_[n_same_].out = out.layout;
-        same_[n_same_++].in = in.layout;
+    // The operand that was checked last.
+    uint32_t last() const { return n_ - 1; }
+    // An output that may be the very view of an input, by their places: views of one
+    // call may share a layout.
+    void may_be(uint32_t out, uint32_t in) {
+        same_[n_same_].out = out;
+        same_[n_same_++].in = in;
     }
     hx_status apart() const {
         for (uint32_t i = 0; i < n_; ++i) {
@@ -53,8 +56,7 @@ class Operands {
                 if (j == i || (all_[j].written && j < i) || !overlap(all_[i].span, all_[j].span)) continue;
                 bool allowed = false;
                 for (uint32_t s = 0; s < n_same_; ++s)
-                    allowed |= all_[i].span.layout && same_[s].out == all_[i].span.layout &&
-                               same_[s].in == all_[j].span.layout;
+                    allowed |= same_[s].out == i && same_[s].in == j;
                 if (!allowed)
                     return fail(HX_ERR_DISPATCH_FAILED, "%s must not overlap %s", all_[i].what, all_[j].what);
                 if (!same_view(all_[i].span, all_[j].span))
@@ -75,7 +77,7 @@ class Operands {
     One all_[kMost];
     uint32_t n_ = 0;
     struct {
-        const hx_layout *out, *in;
+        uint32_t out, in;
     } same_[4];
     uint32_t n_same_ = 0;
 
@@ -125,16 +127,18 @@ hx_status plan_norm(hx_dtype dtype, const View &x, const View &residual, const V
     const uint64_t shape[2] = {x.layout->shape[0], x.layout->shape[1]};
     Operands ops;
     HX_TRY(ops.in(x, 2, shape, size, "norm input"));
+    const uint32_t at_x = ops.last();
     HX_TRY(check_left_out(residual, "residual"));
     HX_TRY(check_left_out(residual_out, "residual output"));
     if (residual.layout) HX_TRY(ops.in(residual, 2, shape, size, "residual"));
+    const uint32_t at_residual = ops.last();
     HX_TRY(ops.in(weight, shape[1], size, "norm weight"));
     if (bias.given()) HX_TRY(ops.in(bias, shape[1], size, "norm bias"));
     if (residual_out.layout) {
         HX_TRY(ops.out(residual_out, 2, shape, size, "residual output"));
         // In place: each element of h is written by the thread that read it.
-        ops.may_be(residual_out, x);
-        if (residual.layout) ops.may_be(residual_out, residual);
+        ops.may_be(ops.last(), at_x);
+        if (residual.layout) ops.may_be(ops.last(), at_residual);
     }
     HX_TRY(ops.out(out, 2, shape, size, "norm output"));
     if (mean.given()) HX_TRY(ops.out(mean, shape[0], 4, "norm mean"));
@@ -173,14 +177,17 @@ hx_status plan_norm_grad(hx_dtype dtype, const View &grad_out, const View &x, co
     Operands ops;
     HX_TRY(ops.in(x, 2, shape, size, "norm input"));
     HX_TRY(ops.in(grad_out, 2, shape, size, "gradient of the norm output"));
+    const uint32_t at_grad_out = ops.last();
     HX_TRY(ops.in(weight, shape[1], size, "norm weight"));
     HX_TRY(ops.in(mean, shape[0], 4, "norm mean"));
     HX_TRY(ops.in(rstd, shape[0], 4, "norm rstd"));
     HX_TRY(check_left_out(residual_grad, "gradient past the norm"));
     if (residual_grad.layout) HX_TRY(ops.in(residual_grad, 2, shape, size, "gradient past the norm"));
+    const uint32_t at_past = ops.last();
     HX_TRY(ops.out(grad_in, 2, shape, size, "gradient of the norm input"));
-    ops.may_be(grad_in, grad_out); // in place: written by the thread that read it
-    if (residual_grad.layout) ops.may_be(grad_in, residual_grad);
+    const uint32_t at_grad_in = ops.last();
+    ops.may_be(at_grad_in, at_grad_out); // in place: written by the thread that read it
+    if (residual_grad.layout) ops.may_be(at_grad_in, at_past);
     if (grad_weight.given()) HX_TRY(ops.out(grad_weight, shape[1], 4, "gradient of the norm weight"));
     if (grad_bias.given()) HX_TRY(ops.out(grad_bias, shape[1], 4, "gradient of the norm bias"));
     HX_TRY(ops.apart());
@@ -231,9 +238,10 @@ hx_status plan_recurrence(hx_dtype dtype, const View &gate, const View &x, const
     HX_TRY(ops.in(gate, 3, shape, size, "recurrence gate"));
     if (lengths.given()) HX_TRY(ops.in(lengths, shape[0], 4, "sequence lengths"));
     HX_TRY(check_state(ops, state_in, states, false, "recurrence state"));
+    const uint32_t at_state_in = ops.last();
     HX_TRY(ops.out(out, 3, shape, size, "recurrence output"));
     HX_TRY(check_state(ops, state_out, states, true, "recurrence state output"));
-    if (state_in.layout && state_out.layout) ops.may_be(state_out, state_in);
+    if (state_in.layout && state_out.layout) ops.may_be(ops.last(), at_state_in);
     HX_TRY(ops.apart());
     HX_TRY(check_sequences(shape, *x.layout));
     RecurrenceArgs &a = *args;
