@@ -852,9 +852,11 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const float2 *stats, co
         }
     }
     if (threadIdx.x >= ROWS || row >= rows) return;
-    const float l = s.x + logf(s.y);
-    if (lse) lse[row] = l;
-    loss[row] = targets[row] < vocab ? l - picked[row] : 0.0f;
+    const float sum = logf(s.y);
+    if (lse) lse[row] = s.x + sum;
+    // Not lse - picked: where the target has the largest logit, the digits of `sum` would
+    // end at the logits' rounding.
+    loss[row] = targets[row] < vocab ? s.x - picked[row] + sum : 0.0f;
 }
 
 template <typename T>
