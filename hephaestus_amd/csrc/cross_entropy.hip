@@ -293,16 +293,16 @@ struct Place {
 
 template <typename T, typename C, bool ACROSS_A, bool ACROSS_B, typename E>
 __global__ __launch_bounds__(C::kThreads) void product_kernel(Product p, E epilogue, uint32_t tiles_m,
-                                                             uint32_t tiles_n) {
+                                                             uint32_t tiles_n, uint32_t first_tile) {
     constexpr int BM = C::BM, BN = C::BN, FM = C::FM, FN = C::FN, S = C::S;
     extern __shared__ __align__(16) int8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 
     // Blocks go to the eight XCDs in turn.  Each XCD takes a run of tiles in strips of a
     // few rows of tiles, so that its L2 serves both operands of those that are under way.
-    const uint32_t total = tiles_m * tiles_n, share = total / 8, rest = total % 8;
+    const uint32_t share = gridDim.x / 8, rest = gridDim.x % 8;
     const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
-    const uint32_t tile = xcd * share + min(xcd, rest) + turn;
+    const uint32_t tile = first_tile + xcd * share + min(xcd, rest) + turn;
     const uint32_t strip = tile / (C::kStrip * tiles_n), in_strip = tile % (C::kStrip * tiles_n);
     const uint32_t height = min((uint32_t)C::kStrip, tiles_m - C::kStrip * strip);
     const uint64_t m0 = (uint64_t)(C::kStrip * strip + in_strip % height) * BM, n0 = (uint64_t)(in_strip / height) * BN;
@@ -726,10 +726,13 @@ hx_status launch_tiles(const Product &p, uint32_t parts, const E &epilogue, hipS
     static std::atomic<uint64_t> allowed{0};
     HX_TRY(allow_lds((const void *)kernel, C::kLds, allowed));
     const uint64_t tm = ceil_div(p.m, C::BM), tn = ceil_div(p.n, C::BN);
-    if (tm * tn * C::kThreads > 0xFFFFFFFFull)
+    // Tiles are counted in 32 bits; no operands or workspace that fit a device have more.
+    if (tm * tn > 0xFFFFFFFFull)
         return fail(HX_ERR_DISPATCH_FAILED, "product of %llu tiles exceeds the grid range", (unsigned long long)(tm * tn));
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn), parts), dim3(C::kThreads), C::kLds, stream, p, epilogue,
-                       (uint32_t)tm, (uint32_t)tn);
+    constexpr uint64_t kMost = tiles_a_launch(C::kThreads);
+    for (uint64_t first = 0; first < tm * tn; first += kMost)
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)std::min(kMost, tm * tn - first), parts), dim3(C::kThreads), C::kLds,
+                           stream, p, epilogue, (uint32_t)tm, (uint32_t)tn, (uint32_t)first);
     return check_launch("product_kernel");
 }
 template <typename T, bool ACROSS_A, bool ACROSS_B, typename E>

@@ -231,6 +231,9 @@ inline ProductCut product_cut(uint64_t m, uint64_t n, uint64_t k, uint64_t size)
     return best;
 }
 
+// Blocks of a launch, whole turns of the eight XCDs: it has fewer than 2^32 threads.
+constexpr uint64_t tiles_a_launch(uint64_t threads) { return (1ull << 32) / threads - 8; }
+
 // The widest rows: places in 256 of them are counted in 32 bits.
 constexpr uint64_t kCrossEntropyWidth = 1 << 20;
 
