@@ -55,6 +55,15 @@ template <typename T, int V> struct Lane {
 __device__ __forceinline__ float apply(float by, float s) {
     return __builtin_fmaf(by, s, __builtin_signbit(by) ? s : 0.0f);
 }
+// An infinite s makes a NaN of s - (1 - A)·s.  Here only what is finite of it is taken away
+// and it stays what it is, as A·s does; two instructions more.  That is for the one
+// application a call of a few tokens: where every token has it, 8 x 4096 x 4096 bf16 takes
+// 184 us against 172, and 8 waves that join by it, or keep such states apart, 174 to 177
+// forward and 338 against 322 backward.
+__device__ __forceinline__ float apply_infinite(float by, float s) {
+    const bool is_near = __builtin_signbit(by);
+    return __builtin_fmaf(by, is_near ? __builtin_amdgcn_fmed3f(s, -__FLT_MAX__, __FLT_MAX__) : s, is_near ? s : 0.0f);
+}
 
 // f = 1 / (1 + e^-z), 1 - f, and f as it is applied, from e^-|z|.  For f32 the
 // exponential has the rest that the product with log2(e) leaves; a bf16 gate itself is off
@@ -116,7 +125,7 @@ __device__ __forceinline__ void join_tile(TileMaps<V, WAVES> &m, uint32_t turn, 
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             mine[v] = carry[v];
-            carry[v] = apply(map[v].by(), carry[v]) + map[v].b;
+            carry[v] = apply_infinite(map[v].by(), carry[v]) + map[v].b;
         }
     } else {
         const int lane = lane_id();

@@ -698,7 +698,9 @@ hx_status hx_prepare_layer_norm_backward(
  * at most `tokens`: later rows of gate and x are not read into a result, later
  * rows of out are 0, and a sequence of no tokens keeps its state.  An infinity
  * or a NaN reaches the channel's later outputs, and no others; which of
- * the two depends on how tokens are taken together. */
+ * the two depends on how tokens are taken together.  In calls of up to 32
+ * tokens an infinite state stays one, as f * h does, while the product of the
+ * call's factors is above 2^-126. */
 hx_status hx_gated_recurrence(
     hx_device *dev, hx_dtype dtype, const void *gate, uint64_t gate_buf_len,
     const hx_layout *gate_layout, const void *x, uint64_t x_buf_len,
