@@ -273,8 +273,9 @@ inline CrossEntropyPlan cross_entropy_plan(const CrossEntropyArgs &a) {
     return p;
 }
 
-// The backward pass takes the vocabulary in pieces of `piece` words, such that G of
-// one has at most 256 MiB.
+// The backward pass takes the vocabulary in pieces of `piece` words, such that G of one
+// has at most 256 MiB, but of no fewer than 256 words: past 524288 rows of bf16, 262144 of
+// f32, G has 256 words of every row.
 struct CrossEntropyGradPlan {
     bool copies;
     uint64_t piece, piece_pitch, sums_pitch; // elements

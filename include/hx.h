@@ -624,7 +624,25 @@ hx_status hx_prepare_linear_attention(
  * dimension is contiguous, outputs apart from each other and from inputs
  * except where stated, operands that may be NULL left out by a NULL layout
  * (vectors: NULL and length 0).  Results have one order of summation: every
- * run gives the same bits. */
+ * run gives the same bits.
+ *
+ * Workspaces, of a plan or of the stream that an immediate call goes to:
+ *   hx_layer_norm                    none
+ *   hx_layer_norm_backward           with a weight or bias gradient 8 * cols bytes
+ *                                    for each of up to min(rows, 512) runs of rows
+ *   hx_gated_recurrence[_backward]   at most 512 KiB, where tokens are cut into parts
+ *   hx_linear_cross_entropy          8 bytes for each row and tile of 64 to 256
+ *                                    words; copies of x and weight where rows of
+ *                                    either do not begin on dwords, go backwards
+ *                                    or lie more than 4 MiB apart; of few tiles up
+ *                                    to 32 parts of the logits in f32
+ *   hx_linear_cross_entropy_backward a copy of x; the logits' gradients of a piece
+ *                                    of the vocabulary, at most 256 MiB or, if that
+ *                                    is more, 256 words of every row, in dtype; the
+ *                                    sums of grad_x in f32 where there is more than
+ *                                    one piece; a copy of a piece of weight where
+ *                                    rows are as above or no multiple of 16 bytes;
+ *                                    of few tiles up to 32 parts of a product */
 
 /* Layer norm of rows, with the residual's addition.  x is [rows, cols]:
  *   h    = x + residual                      (residual may be NULL: h = x)

@@ -20,3 +20,22 @@ extern "C" void gradient_piece(uint64_t size, uint64_t rows, uint64_t vocab, uin
     form[1] = rows * p.piece_pitch * size;
     form[2] = p.bytes;
 }
+
+// Runs of rows of the norm's backward pass.
+extern "C" uint64_t norm_runs(uint64_t size, uint64_t rows, uint64_t cols) {
+    hx::LayerNormGradArgs a{};
+    a.dtype = size == 4 ? HX_DTYPE_F32 : HX_DTYPE_BF16;
+    a.rows = rows;
+    a.cols = cols;
+    return hx::layer_norm_grad_split(a).blocks;
+}
+
+// Bytes of the maps of a recurrence's parts, of dense operands.
+extern "C" uint64_t map_bytes(uint64_t vector, int is_backward, uint64_t batch, uint64_t tokens, uint64_t channels) {
+    hx::RecurrenceArgs a{};
+    a.batch = batch;
+    a.tokens = tokens;
+    a.channels = channels;
+    const uint32_t parts = hx::recurrence_parts(a, vector, is_backward != 0).parts;
+    return parts > 1 ? batch * parts * channels * 8 : 0;
+}
