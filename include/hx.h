@@ -48,10 +48,12 @@
  * and may grow their stream's buffers, so on a capturing stream they fail
  * with HX_ERR_DISPATCH_FAILED before anything is queued, and so do the
  * immediate layer and training operators that take scratch (hx_matmul_i8,
- * hx_linear_attention, hx_linear_cross_entropy and the backward passes;
- * hx_gated_recurrence where tokens are cut into parts); hx_scan_noalloc, the
- * vector forms, hx_copy_async, hx_fill_random, hx_rms_norm_quantize and
- * hx_layer_norm queue plain kernels and may be captured.
+ * hx_linear_attention, hx_linear_cross_entropy[_backward];
+ * hx_gated_recurrence[_backward] where tokens are cut into parts, never of up
+ * to 32 tokens; hx_layer_norm_backward with a weight or bias gradient);
+ * hx_scan_noalloc, the vector forms, hx_copy_async, hx_fill_random,
+ * hx_rms_norm_quantize, hx_layer_norm and the others of these operators queue
+ * plain kernels and may be captured.
  */
 #ifndef HX_H
 #define HX_H
