@@ -108,8 +108,8 @@ __device__ __forceinline__ float scaled_stats(const Each &each, Sums &sums, uint
     // The differences' own roundings, up to 2^-24 of each and often the same in all,
     // leave about that much of Σ|d| / n in the shift, beside a mean near 0 far more than
     // what the first sum was off: of 4096 bf16 elements 7e-7 of the mean against 9e-8
-    // (95 of 100 rows).  A shift past 4 times that corrects the mean.
-    r.mean = fabsf(shift) > 0x1p-22f * (far[2] / cols) ? mean + shift : mean;
+    // (95 of 100 rows).  A shift past 4 times that, or one that is a NaN, goes to the mean.
+    r.mean = fabsf(shift) <= 0x1p-22f * (far[2] / cols) ? mean : mean + shift;
     const float var = (far[1] - far[0] * shift) / cols;
     const float m = (var < 0.0f ? 0.0f : var) + epsilon * r.scale * r.scale; // a NaN stays
     r.rstd = m > 0.0f ? 1.0f / sqrtf(m) : m == 0.0f ? 0.0f : __builtin_nanf("");

@@ -50,3 +50,18 @@ def test_mean_far_from_zero_is_corrected(device, cols, size):
     got = forward(device, x, None, ones, zeros, keep_h=False, epsilon=EPSILON * size**2 if size < 2 else EPSILON)
     mean = as_float64(x).mean(1)
     assert np.all(np.abs(got["mean"] - mean) <= 2 * EPS32 * np.abs(mean))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", COLS + [1, 2])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_rows_that_are_not_finite_have_no_mean(device, dtype, cols, value):
+    """mean, rstd and out of such a row are NaN, those of its neighbours what they were."""
+    t, rng = TYPES[dtype], np.random.default_rng(cols)
+    values = as_float64(whole(rng, (3, cols), t))
+    values[1, cols // 2] = value
+    got = forward(device, rounded(values, t), None, rounded(np.ones(cols), t), rounded(np.zeros(cols), t), keep_h=False)
+    for name in ("mean", "rstd"):
+        assert np.isnan(got[name][1]) and np.isfinite(got[name][[0, 2]]).all()
+    y = as_float64(got["y"])
+    assert np.isnan(y[1]).all() and np.isfinite(y[[0, 2]]).all()
