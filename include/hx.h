@@ -655,7 +655,8 @@ hx_status hx_prepare_linear_attention(
  * view of x or of residual; out is taken from h before that rounding.  mean
  * and rstd are f32[rows], each may be NULL.  A row of equal elements has out =
  * bias, and rstd = 0 where epsilon is 0.  Rows whose sums or squares leave the
- * range of f32 are as exact as others; a row with a NaN or an infinity is NaN.
+ * range of f32 are as exact as others, but for an rstd past 2^128, which is
+ * infinite; a row with a NaN or an infinity is NaN.
  * cols = 0 leaves mean and rstd NaN. */
 hx_status hx_layer_norm(hx_device *dev, hx_dtype dtype, const void *x,
                         uint64_t x_buf_len, const hx_layout *x_layout,
@@ -686,7 +687,9 @@ hx_status hx_prepare_layer_norm(
  * residual_grad (may be NULL) is the gradient that reaches h past the norm.
  * grad_in is the gradient of x and of residual alike, and may be the very view
  * of grad_out or of residual_grad.  grad_weight and grad_bias are f32[cols],
- * overwritten; each may be NULL.  At most 65535 * 1024 columns. */
+ * overwritten; each may be NULL.  At most 65535 * 1024 columns.  x - mean and
+ * u are f32: a row where they leave its range (an infinite rstd) has gradients
+ * that are not finite. */
 hx_status hx_layer_norm_backward(
     hx_device *dev, hx_dtype dtype, const void *grad_out,
     uint64_t grad_out_buf_len, const hx_layout *grad_out_layout, const void *x,
