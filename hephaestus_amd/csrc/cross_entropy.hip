@@ -13,12 +13,13 @@
 // which are all alike, the factor is 1 and G keeps the places of e^(logit - lse):
 // a factor's rounding would be the same in every term of a sum and stay in it.
 //
-// The products bound large calls: 8192 x 32768 x 4096 bf16 takes 1.62 ms forward (1.36
-// PFLOP/s) and 5.3 ms backward (1.25), where the library's products of such sizes reach 1.24
+// The products bound large calls: 8192 x 32768 x 4096 bf16 takes 1.63 ms forward (1.35
+// PFLOP/s) and 5.4 ms backward (1.22), where the library's products of such sizes reach 1.24
 // to 1.40; the matrix units are busy 69% and 57 to 64% of the cycles, at the clock that
 // the power leaves, with no bank conflicts in LDS.  16 x 32000 x 2048 reads the weight at
-// 4.1 TB/s (32 us).  f32 is bound by its matrix instructions: 1000 x 5003 x 1025 takes 329 us
-// backward, 94 TFLOP/s of 154.
+// 4.1 TB/s (32 us).  f32 is bound by rounds of 512 tiles whose last one is short: 1000 x 5003 x
+// 1025 takes 329 us backward, 94 TFLOP/s, where a full round reaches 126 and the library's
+// product 154.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 

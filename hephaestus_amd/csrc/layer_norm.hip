@@ -13,11 +13,11 @@
 // A block goes through rows and keeps its share of dw and db in registers; the
 // blocks' shares are added up by a second launch, in one order.
 //
-// Memory bounds both: 16384 x 8192 bf16 with a residual takes 191 us forward (5.6 TB/s
+// Memory bounds both: 16384 x 8192 bf16 with a residual takes 192 us forward (5.6 TB/s
 // of x, residual, h and out) and 210 us backward (5.1 TB/s and the sums' launch of 6 us),
-// where torch's copy of 1 GiB reaches 5.2 TB/s.  A single row of 4096 takes 3.3 us, a launch
-// and one wait for memory; 1000 x 5001 f32 takes 24 us backward, 250 blocks of 4 rows whose
-// loads lie off the 128-byte grid, and 6 us of the sums.
+// where torch's copy of 1 GiB reaches 5.2 TB/s.  A single row of 4096 takes 3.7 us, 3.5 of
+// them the kernel's, a launch and one wait for memory; 1000 x 5001 f32 takes 24 us
+// backward, 250 blocks of 4 rows whose loads lie off the 128-byte grid, and 6 us of the sums.
 #include "hx_internal.hpp"
 #include "layer_device.hpp"
 
@@ -208,7 +208,9 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_kernel(L
     }
 }
 
-// Rows of any length, read three times by one block.
+// Rows of any length, read three times by one block: 1024 threads hold no more than 4 vectors
+// of x and of the residual each.  1500 x 40000 bf16 with a residual takes 144 us (3.3 TB/s of
+// what has to be moved), 2048 x 32768, in registers, 123 (4.4).
 template <typename T> __global__ __launch_bounds__(1024) void layer_norm_long_kernel(LayerNormArgs a) {
     constexpr int N = Pack16<T>::N;
     const uint64_t row = blockIdx.x;
