@@ -671,11 +671,12 @@ __global__ __launch_bounds__(64) void fold_parts_kernel(const float *parts, uint
     }
 }
 
-// Logits of parts to what TileStats leaves of a tile: 1024 columns of a row, a block.
+// Logits of parts to what TileStats leaves of a tile: 1024 columns of a row, a block.  The
+// rows from `first` on.
 __global__ __launch_bounds__(256) void fold_stats_kernel(const float *parts, uint32_t count, uint64_t m, uint64_t n,
-                                                        uint64_t pitch, TileStats out) {
+                                                        uint64_t pitch, TileStats out, uint64_t first) {
     __shared__ float2 joined[256 / kWave];
-    const uint64_t row = blockIdx.x, c = ((uint64_t)blockIdx.y * 256 + threadIdx.x) * 4, target = out.targets[row];
+    const uint64_t row = first + blockIdx.x, c = ((uint64_t)blockIdx.y * 256 + threadIdx.x) * 4, target = out.targets[row];
     f32x4 v = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
     if (c < n) {
         const f32x4 all = sum_of_parts(parts + row * pitch + c, count, m * pitch);
@@ -768,6 +769,7 @@ hx_status launch_parts(const Product &p, const ProductCut &cut, float *parts, ui
     const TileOut<T> part{nullptr, nullptr, parts, nullptr, pitch, 0, nullptr, 0};
     return launch_product<T, ACROSS_A, ACROSS_B>(p, cut, part, stream);
 }
+constexpr uint64_t kBlocksOf256 = tiles_a_launch(256); // of a launch
 inline dim3 fold_blocks(uint64_t m, uint64_t pitch) {
     return dim3((uint32_t)std::min<uint64_t>(ceil_div(m * (pitch / 4), 64), 1 << 18));
 }
@@ -835,14 +837,14 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const int8_t *from, int6
 }
 
 // The tiles' sums of a row, joined in one order: ROWS rows a block, 256 / ROWS threads a
-// row.  Many rows are read side by side, few rows by more threads.
+// row.  Many rows are read side by side, few rows by more threads.  The rows from `first` on.
 template <int ROWS>
 __global__ __launch_bounds__(256) void join_stats_kernel(const float2 *stats, const float *picked,
                                                          const uint32_t *targets, uint64_t tiles, uint64_t rows,
-                                                         uint64_t vocab, float *loss, float *lse) {
+                                                         uint64_t vocab, float *loss, float *lse, uint64_t first) {
     constexpr int kThreads = 256 / ROWS;
     __shared__ float2 part[kThreads][ROWS];
-    const uint64_t row = (uint64_t)blockIdx.x * ROWS + threadIdx.x % ROWS;
+    const uint64_t row = first + (uint64_t)blockIdx.x * ROWS + threadIdx.x % ROWS;
     float2 s = {-__builtin_inff(), 0.0f};
     if (row < rows)
         for (uint64_t t = threadIdx.x / ROWS; t < tiles; t += kThreads) s = TileStats::join(s, stats[t * rows + row]);
@@ -894,20 +896,23 @@ template <typename T> hx_status launch(const CrossEntropyArgs &a, void *ws, hipS
         float *parts = (float *)(base + plan.parts);
         const uint64_t pitch = round_up(a.vocab, 4);
         HX_TRY((launch_parts<T, false, false>)(p, plan.cut, parts, pitch, stream));
-        hipLaunchKernelGGL(fold_stats_kernel, dim3((uint32_t)a.rows, (uint32_t)plan.tiles_n), dim3(256), 0, stream, parts,
-                           plan.cut.parts, a.rows, a.vocab, pitch, out);
+        for (uint64_t first = 0; first < a.rows; first += kBlocksOf256)
+            hipLaunchKernelGGL(fold_stats_kernel, dim3((uint32_t)std::min(kBlocksOf256, a.rows - first), (uint32_t)plan.tiles_n),
+                               dim3(256), 0, stream, parts, plan.cut.parts, a.rows, a.vocab, pitch, out, first);
         HX_TRY(check_launch("fold_stats_kernel"));
     } else {
         HX_TRY((launch_product<T, false, false>)(p, plan.cut, out, stream));
     }
     const uint64_t tiles = a.vocab ? plan.tiles_n : 0;
-    if (a.rows >= 2048)
-        hipLaunchKernelGGL(join_stats_kernel<16>, dim3((uint32_t)ceil_div(a.rows, 16)), dim3(256), 0, stream, stats,
-                           picked, a.targets, tiles, a.rows, a.vocab, a.loss, a.lse);
-    else
-        hipLaunchKernelGGL(join_stats_kernel<1>, dim3((uint32_t)a.rows), dim3(256), 0, stream, stats, picked, a.targets,
-                           tiles, a.rows, a.vocab, a.loss, a.lse);
-    return check_launch("join_stats_kernel");
+    const auto join = [&](auto kernel, uint64_t rows) { // of a block
+        for (uint64_t first = 0; first < a.rows; first += kBlocksOf256 * rows) {
+            const uint64_t blocks = std::min(kBlocksOf256, ceil_div(a.rows - first, rows));
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, stats, picked, a.targets, tiles, a.rows,
+                               a.vocab, a.loss, a.lse, first);
+        }
+        return check_launch("join_stats_kernel");
+    };
+    return a.rows >= 2048 ? join(join_stats_kernel<16>, 16) : join(join_stats_kernel<1>, 1);
 }
 
 template <typename T> hx_status launch(const CrossEntropyGradArgs &a, void *ws, hipStream_t stream) {

@@ -43,3 +43,27 @@ def test_more_tiles_than_a_launch_takes(device):
     picked = logits[np.arange(rows), targets % period]
     assert np.all(np.abs(device.download_owned(loss) - (want - picked)) <= 2 * off)
 
+
+
+def test_the_most_rows(device):
+    """2^28 - 1 rows that are one row in memory: the join's last block of 16 rows is past
+    what one launch may have."""
+    rows, vocab, width = (1 << 28) - 1, 50, 8
+    rng = np.random.default_rng(7)
+    x, w = rounded(rng.normal(size=(1, width)), hx.bfloat16), rounded(rng.normal(size=(vocab, width)), hx.bfloat16)
+    same = StridedView(device.upload(x), Layout.try_new([rows, width], [0, 1]))
+    targets = device.alloc_zeroed(np.uint32, rows)
+    some = np.unique(np.concatenate([np.arange(40), rows - 1 - np.arange(40), rng.integers(0, rows, 40)]))
+    kinds = rng.integers(0, vocab + 1, len(some)).astype(np.uint32)  # `vocab` leaves a row out
+    for at, kind in zip(some, kinds):
+        device.write_sub_buffer(targets, int(at), np.array([kind], np.uint32))
+    loss = device.alloc_uninitialized(np.float32, rows)
+    hx.RocmLossOps().linear_cross_entropy_into(device, same, padded(device, w)[0], targets, loss)
+    device.synchronize()
+    logits = (as_float64(x) @ as_float64(w).T)[0]
+    want = np.append(np.log(np.exp(logits).sum()) - logits, 0.0)
+    off = EPS32 * (600 + 8 * np.abs(want).max()) + 2 * (width / 4 + 16) * EPS32 * (np.abs(as_float64(x)) @ np.abs(as_float64(w)).T).max()
+    got = device.download_owned(loss)
+    assert np.abs(got[some] - want[kinds]).max() <= off
+    got[some] = got[100]
+    assert abs(float(got[100]) - want[0]) <= off and np.all(got == got[100])
