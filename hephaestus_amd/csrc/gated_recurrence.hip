@@ -417,15 +417,30 @@ __global__ __launch_bounds__(WAVES *kWave) void recurrence_grad_kernel(Recurrenc
     }
 }
 
-template <typename T, int V, typename Args> hx_status launch(const Args &a, void *ws, hipStream_t stream) {
+// `count` channels from `first` on.
+template <typename T> void shift(const void *&p, uint64_t first) { p = (const T *)p + first; }
+template <typename T> void shift(void *&p, uint64_t first) { p = (T *)p + first; }
+inline void shift_state(const float *&p, uint64_t first) { p = p ? p + first : nullptr; }
+inline void shift_state(float *&p, uint64_t first) { p = p ? p + first : nullptr; }
+template <typename T> RecurrenceArgs channels_from(RecurrenceArgs a, uint64_t first, uint64_t count) {
+    shift<T>(a.gate, first), shift<T>(a.x, first), shift<T>(a.out, first);
+    shift_state(a.state_in, first), shift_state(a.state_out, first);
+    a.channels = count;
+    return a;
+}
+template <typename T> RecurrenceGradArgs channels_from(RecurrenceGradArgs a, uint64_t first, uint64_t count) {
+    shift<T>(a.gate, first), shift<T>(a.x, first), shift<T>(a.h, first), shift<T>(a.grad_out, first);
+    shift<T>(a.grad_gate, first), shift<T>(a.grad_x, first);
+    shift_state(a.state_in, first), shift_state(a.grad_state_out, first), shift_state(a.grad_state_in, first);
+    a.channels = count;
+    return a;
+}
+
+template <typename T, int V, typename Args>
+hx_status launch_channels(const Args &a, const RecurrenceParts &cut, void *ws, hipStream_t stream) {
     constexpr bool kGrad = std::is_same<Args, RecurrenceGradArgs>::value;
-    const RecurrenceParts cut = recurrence_parts(a, V, kGrad);
     const PartMaps p{(float *)ws, cut.parts, cut.span, a.channels};
-    const uint64_t groups = ceil_div(a.channels, kWave * V);
-    if (groups * cut.parts * 512 > 0xFFFFFFFFull)
-        return fail(HX_ERR_DISPATCH_FAILED, "recurrence of %llu channels exceeds the grid range",
-                    (unsigned long long)a.channels);
-    const dim3 grid((uint32_t)(groups * cut.parts), (uint32_t)a.batch);
+    const dim3 grid((uint32_t)(ceil_div(a.channels, kWave * V) * cut.parts), (uint32_t)a.batch);
     const auto run = [&](auto kernel, uint32_t waves) {
         hipLaunchKernelGGL(kernel, grid, dim3(waves * kWave), 0, stream, a, p);
         return check_launch("recurrence_kernel");
@@ -448,6 +463,16 @@ template <typename T, int V, typename Args> hx_status launch(const Args &a, void
         case RecurrenceTile::kLong: return run(recurrence_kernel<T, V, 8, 16, false>, 8);
         }
     }
+    return HX_OK;
+}
+
+template <typename T, int V, typename Args> hx_status launch(const Args &a, void *ws, hipStream_t stream) {
+    // Blocks of 512 threads, fewer than 2^32 of these in a launch: more channels take
+    // several, and far fewer are ever cut into parts.
+    constexpr uint64_t kMost = (uint64_t)kWave * V << 22;
+    const RecurrenceParts cut = recurrence_parts(a, V, std::is_same<Args, RecurrenceGradArgs>::value);
+    for (uint64_t first = 0; first < a.channels; first += kMost)
+        HX_TRY((launch_channels<T, V>(channels_from<T>(a, first, std::min(kMost, a.channels - first)), cut, ws, stream)));
     return HX_OK;
 }
 
