@@ -789,7 +789,10 @@ hx_status hx_prepare_gated_recurrence_backward(
  *   loss[r] = lse[r] - logits[r, targets[r]]
  * x is [rows, width], weight [vocab, width], both of dtype; targets is
  * u32[rows].  A row whose target is not below vocab is left out: its loss is 0.
- * loss and lse are f32[rows]; lse may be NULL.  A logit that is a NaN or plus
+ * loss and lse are f32[rows]; lse may be NULL.  The loss is not taken from the
+ * rounded lse: a row that is sure of its target keeps the digits of a small loss.
+ * The backward pass goes by lse, whose rounding (2^-24 of it) is a relative error
+ * of all of the row's probabilities there.  A logit that is a NaN or plus
  * infinity makes its row's loss and lse a NaN.  rows and vocab are below 2^28,
  * width is at most 2^20. */
 hx_status hx_linear_cross_entropy(
